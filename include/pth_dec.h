@@ -146,6 +146,19 @@ int pth_dec_decode(const pd_tensor* q, const pd_tensor* key_cache, const pd_tens
                    int64_t num_seqs, int64_t qmax, int64_t nsplit, int64_t window, int64_t causal,
                    hipStream_t stream, char* err, int errlen);
 
+/*
+ * pth_dec_decode that also stores each row's softmax logarithm, for callers that need the weights of single keys
+ * (pth_cache_key_weights) or merge the result with attention over other keys. No counterpart in the reference.
+ *   lse          fp32, contiguous [>= T, Hq]: ln(sum over the visible keys of e^(scale q . k)), -inf for a row
+ *                that sees no key; rows that out does not get are left alone
+ */
+int pth_dec_decode_lse(const pd_tensor* q, const pd_tensor* key_cache, const pd_tensor* value_cache,
+                       const pd_tensor* k_scale, const pd_tensor* v_scale, const pd_tensor* block_table,
+                       const pd_tensor* seq_lens, const pd_tensor* query_start_loc, const pd_tensor* out,
+                       double scale, const pd_tensor* part_o, const pd_tensor* part_m, const pd_tensor* part_l,
+                       const pd_tensor* lse, int64_t num_seqs, int64_t qmax, int64_t nsplit, int64_t window,
+                       int64_t causal, hipStream_t stream, char* err, int errlen);
+
 /* Library version string. */
 const char* pth_dec_version(void);
 
@@ -249,6 +262,65 @@ int64_t pth_fa_balanced_workspace(int64_t num_seqs, const int* query_start, int6
 int pth_cache_write(const pd_tensor* key, const pd_tensor* value, const pd_tensor* key_cache,
                     const pd_tensor* value_cache, const pd_tensor* k_scale, const pd_tensor* v_scale,
                     const pd_tensor* slot_mapping, hipStream_t stream, char* err, int errlen);
+
+/*
+ * Rotary positions and the cache write of a layer's new tokens in one launch. No counterpart in the reference, whose
+ * engine runs its own rotary kernel before the cache update.
+ *   query        fp16, bf16 or fp32 [T, Hq, 256], unit dim stride; rotated into query_out
+ *   query_out    [T, Hq, 256] of the query's dtype or fp16: the query itself (same data, dtype and strides: in place) or
+ *                a tensor that does not overlap it
+ *   key, value   [T, Hkv, 256] of the query's dtype, left as they are; the rotated key and the value are
+ *                quantised into the cache rows as pth_cache_write does
+ *   positions    int64 [>= T]; a token whose position lies outside cos_sin is skipped (query_out and cache row stay)
+ *   cos_sin      fp32 [positions, rotary_dim], rotary_dim a multiple of 8 up to 256: cosines of the
+ *                rotary_dim / 2 angles, then sines
+ *   interleaved  0: pair i is dims (i, i + rotary_dim / 2); else (2 i, 2 i + 1); the dims from rotary_dim on stay
+ *   slot_mapping int64 [>= T]; tokens with a slot below 0 or past the cache write no row (their query is rotated). No two
+ *                tokens of a call may have the same slot
+ * Rotation and quantisation are fp32, each product and sum rounded; the rotated key is not rounded to its dtype
+ * first. Rows are aligned to four elements. Returns 0, 1 (validation failure, message in err) or 2 (launch failure).
+ */
+int pth_cache_write_rotary(const pd_tensor* query, const pd_tensor* query_out, const pd_tensor* key,
+                           const pd_tensor* value, const pd_tensor* positions, const pd_tensor* cos_sin,
+                           const pd_tensor* key_cache, const pd_tensor* value_cache, const pd_tensor* k_scale,
+                           const pd_tensor* v_scale, const pd_tensor* slot_mapping, int64_t interleaved,
+                           hipStream_t stream, char* err, int errlen);
+
+/*
+ * Running attention weights of the cached keys: adds to weights[b, g, t] the softmax weight that the query rows of
+ * sequence b and kv head g gave key t, sum over rows of e^(scale q . k_t - lse). No counterpart in the reference.
+ *   q, key_cache .. query_start_loc, scale, num_seqs, qmax   as for pth_dec_decode (causal, no window)
+ *   lse          fp32, contiguous [>= T, Hq], of pth_dec_decode_lse on the same rows; a row of
+ *                -inf adds nothing
+ *   weights      fp32 [>= num_seqs, Hkv, keys], unit key stride; only keys below seq_len and below `keys` are touched
+ * Every weight is formed in a fixed order (no atomics). Returns 0, 1 or 2 as above.
+ */
+int pth_cache_key_weights(const pd_tensor* q, const pd_tensor* key_cache, const pd_tensor* value_cache,
+                    const pd_tensor* k_scale, const pd_tensor* v_scale, const pd_tensor* block_table,
+                    const pd_tensor* seq_lens, const pd_tensor* query_start_loc, const pd_tensor* lse,
+                    const pd_tensor* weights, double scale, int64_t num_seqs, int64_t qmax, hipStream_t stream,
+                    char* err, int errlen);
+
+/*
+ * Eviction by running weights: per sequence and kv head the last `recent` keys and the keep - recent others with the
+ * largest weights stay (equal weights: the lowest key; NaN counts as the largest), in the order of their positions. Their
+ * rows are copied into the blocks of new_block_table; the old blocks are left as they are. No counterpart in the reference.
+ *   weights      fp32 [>= num_seqs, Hkv, keys]; keys of a sequence past `keys` or past its block table are dropped
+ *   block_table, seq_lens   int32, the batch before; sequences of at most keep keys are copied whole
+ *   new_block_table         int32 [>= num_seqs, columns for keep keys]: blocks that no table row of the call reads
+ *                           and no two of its rows share, in the part that holds a sequence's min(seq_len, keep) keys
+ *   new_seq_lens            int32 [>= num_seqs], written: min(seq_len, keep)
+ *   new_weights             fp32 [>= num_seqs, Hkv, >= keep], written: the kept keys' weights, then zeros
+ *   kept                    int32, contiguous [>= num_seqs, Hkv, keep], written: the kept keys' numbers, then -1
+ *   keep, recent            keep >= 1, 0 <= recent <= keep
+ * The new tensors must not be the old ones. Rotated keys keep the positions they were rotated by; rows written later take
+ * positions (pth_cache_write_rotary) that count the evicted keys too. Returns 0, 1 or 2 as above.
+ */
+int pth_cache_evict(const pd_tensor* weights, const pd_tensor* key_cache, const pd_tensor* value_cache,
+              const pd_tensor* k_scale, const pd_tensor* v_scale, const pd_tensor* block_table,
+              const pd_tensor* seq_lens, const pd_tensor* new_block_table, const pd_tensor* new_seq_lens,
+              const pd_tensor* new_weights, const pd_tensor* kept, int64_t num_seqs, int64_t keep, int64_t recent,
+              hipStream_t stream, char* err, int errlen);
 
 #ifdef __cplusplus
 }

@@ -51,6 +51,7 @@ LaunchArgs make_args(const void* q, int64_t q_st, const void* kc, int64_t k_sb, 
     x.o_sh = o_sh;
     x.window = window;
     x.causal = causal;
+    x.lse = nullptr;
     return x;
 }
 
@@ -191,12 +192,19 @@ int pth_dec_supported_layout(const pd_tensor* key_cache, const pd_tensor* value_
     return layout_ok(key_cache, value_cache, k_scale, v_scale) ? 1 : 0;
 }
 
-int pth_dec_decode(const pd_tensor* q, const pd_tensor* key_cache, const pd_tensor* value_cache,
-                   const pd_tensor* k_scale, const pd_tensor* v_scale, const pd_tensor* block_table,
-                   const pd_tensor* seq_lens, const pd_tensor* query_start_loc, const pd_tensor* out, double scale,
-                   const pd_tensor* part_o, const pd_tensor* part_m, const pd_tensor* part_l, int64_t num_seqs,
-                   int64_t qmax, int64_t nsplit, int64_t window, int64_t causal, hipStream_t stream, char* err,
-                   int errlen) {
+// null if lse (may be null) can take the rows' logarithms, else why not
+static const char* lse_refused(const pd_tensor* lse, int64_t T, int64_t Hq) {
+    if (!lse) return nullptr;
+    const bool ok = lse->dtype == PD_DTYPE_FP32 && lse->ndim == 2 && lse->sizes[0] >= T && lse->sizes[1] == Hq && is_contig(lse);
+    return ok ? nullptr : "lse must be contiguous fp32 [T, Hq]";
+}
+
+static int decode_entry(const pd_tensor* q, const pd_tensor* key_cache, const pd_tensor* value_cache,
+                        const pd_tensor* k_scale, const pd_tensor* v_scale, const pd_tensor* block_table,
+                        const pd_tensor* seq_lens, const pd_tensor* query_start_loc, const pd_tensor* out, double scale,
+                        const pd_tensor* part_o, const pd_tensor* part_m, const pd_tensor* part_l, const pd_tensor* lse,
+                        int64_t num_seqs, int64_t qmax, int64_t nsplit, int64_t window, int64_t causal,
+                        hipStream_t stream, char* err, int errlen) {
     if (!q || !key_cache || !value_cache || !k_scale || !v_scale || !block_table || !seq_lens ||
         !query_start_loc || !out || !part_o || !part_m || !part_l)
         return fail(err, errlen, "null tensor descriptor");
@@ -233,8 +241,9 @@ int pth_dec_decode(const pd_tensor* q, const pd_tensor* key_cache, const pd_tens
     if (!(num_seqs >= 1 && seq_lens->sizes[0] >= num_seqs && query_start_loc->sizes[0] >= num_seqs + 1 &&
           block_table->sizes[0] >= num_seqs))
         return fail(err, errlen, "per-sequence tensors too small");
+    if (const char* why = lse_refused(lse, T, Hq)) return fail(err, errlen, why);
     if (T == 0) return 0;
-    const LaunchArgs x = make_args(
+    LaunchArgs x = make_args(
         q->data, q->strides[0], key_cache->data, key_cache->strides[0], key_cache->strides[1],
         key_cache->strides[2], static_cast<const int*>(block_table->data), block_table->strides[0],
         static_cast<const int*>(seq_lens->data), static_cast<const int*>(query_start_loc->data), (int)num_seqs,
@@ -242,6 +251,7 @@ int pth_dec_decode(const pd_tensor* q, const pd_tensor* key_cache, const pd_tens
         static_cast<float*>(const_cast<void*>(part_o->data)), static_cast<float*>(const_cast<void*>(part_m->data)),
         static_cast<float*>(const_cast<void*>(part_l->data)), (int)nseg, (int)nsplit, const_cast<void*>(out->data),
         out->strides[0], out->strides[1], (int)window, (int)causal);
+    x.lse = lse ? static_cast<float*>(const_cast<void*>(lse->data)) : nullptr;
     const hipError_t e = launch_all(x, stream, false);
     if (e != hipSuccess) {
         char msg[256];
@@ -250,6 +260,27 @@ int pth_dec_decode(const pd_tensor* q, const pd_tensor* key_cache, const pd_tens
         return 2;
     }
     return 0;
+}
+
+int pth_dec_decode(const pd_tensor* q, const pd_tensor* key_cache, const pd_tensor* value_cache,
+                   const pd_tensor* k_scale, const pd_tensor* v_scale, const pd_tensor* block_table,
+                   const pd_tensor* seq_lens, const pd_tensor* query_start_loc, const pd_tensor* out, double scale,
+                   const pd_tensor* part_o, const pd_tensor* part_m, const pd_tensor* part_l, int64_t num_seqs,
+                   int64_t qmax, int64_t nsplit, int64_t window, int64_t causal, hipStream_t stream, char* err,
+                   int errlen) {
+    return decode_entry(q, key_cache, value_cache, k_scale, v_scale, block_table, seq_lens, query_start_loc, out, scale,
+                        part_o, part_m, part_l, nullptr, num_seqs, qmax, nsplit, window, causal, stream, err, errlen);
+}
+
+int pth_dec_decode_lse(const pd_tensor* q, const pd_tensor* key_cache, const pd_tensor* value_cache,
+                       const pd_tensor* k_scale, const pd_tensor* v_scale, const pd_tensor* block_table,
+                       const pd_tensor* seq_lens, const pd_tensor* query_start_loc, const pd_tensor* out, double scale,
+                       const pd_tensor* part_o, const pd_tensor* part_m, const pd_tensor* part_l, const pd_tensor* lse,
+                       int64_t num_seqs, int64_t qmax, int64_t nsplit, int64_t window, int64_t causal,
+                       hipStream_t stream, char* err, int errlen) {
+    if (!lse) return fail(err, errlen, "null tensor descriptor");
+    return decode_entry(q, key_cache, value_cache, k_scale, v_scale, block_table, seq_lens, query_start_loc, out, scale,
+                        part_o, part_m, part_l, lse, num_seqs, qmax, nsplit, window, causal, stream, err, errlen);
 }
 
 static int fa_result(hipError_t e, char* err, int errlen) {
@@ -602,6 +633,204 @@ int pth_cache_write(const pd_tensor* key, const pd_tensor* value, const pd_tenso
         return 2;
     }
     return 0;
+}
+
+static int op_result(hipError_t e, const char* what, char* err, int errlen) {
+    if (e == hipSuccess) return 0;
+    char msg[256];
+    snprintf(msg, sizeof msg, "%s launch failed: %s", what, hipGetErrorString(e));
+    fail(err, errlen, msg);
+    return 2;
+}
+
+// Heads of 256 values that can be loaded four at a time: data and strides aligned to four elements.
+static bool heads_of_4(const pd_tensor* t, int64_t esz) {
+    return reinterpret_cast<uintptr_t>(t->data) % (uintptr_t)(4 * esz) == 0 && t->strides[0] % 4 == 0 && t->strides[1] % 4 == 0;
+}
+
+int pth_cache_write_rotary(const pd_tensor* query, const pd_tensor* query_out, const pd_tensor* key, const pd_tensor* value,
+                           const pd_tensor* positions, const pd_tensor* cos_sin, const pd_tensor* key_cache,
+                           const pd_tensor* value_cache, const pd_tensor* k_scale, const pd_tensor* v_scale,
+                           const pd_tensor* slot_mapping, int64_t interleaved, hipStream_t stream, char* err, int errlen) {
+    if (!query || !query_out || !key || !value || !positions || !cos_sin || !key_cache || !value_cache || !k_scale ||
+        !v_scale || !slot_mapping)
+        return fail(err, errlen, "null tensor descriptor");
+    if (!layout_ok(key_cache, value_cache, k_scale, v_scale))
+        return fail(err, errlen, "KV cache views do not have the int8 per-token-head row layout");
+    const int dt = query->dtype;
+    if (!((dt == PD_DTYPE_FP16 || dt == PD_DTYPE_BF16 || dt == PD_DTYPE_FP32) && key->dtype == dt && value->dtype == dt))
+        return fail(err, errlen, "query, key and value must be fp16, bf16 or fp32 of the same dtype");
+    if (!(query->ndim == 3 && query->sizes[1] > 0 && query->sizes[2] == kDim && query->strides[2] == 1))
+        return fail(err, errlen, "query must be [T, Hq, 256] with unit dim stride");
+    const int64_t T = query->sizes[0], Hq = query->sizes[1], Hkv = key_cache->sizes[2];
+    if (!(key->ndim == 3 && value->ndim == 3 && key->sizes[0] == T && value->sizes[0] == T && key->sizes[1] == Hkv &&
+          value->sizes[1] == Hkv && key->sizes[2] == kDim && value->sizes[2] == kDim && key->strides[2] == 1 &&
+          value->strides[2] == 1))
+        return fail(err, errlen, "key and value must be [T, Hkv, 256] with unit dim stride");
+    const int out_dt = query_out->dtype;
+    if (!((out_dt == dt || out_dt == PD_DTYPE_FP16) && query_out->ndim == 3 && query_out->sizes[0] == T &&
+          query_out->sizes[1] == Hq && query_out->sizes[2] == kDim && query_out->strides[2] == 1))
+        return fail(err, errlen, "query_out must be [T, Hq, 256] with unit dim stride, of the query's dtype or fp16");
+    if (Hq > (1 << 20) || Hkv > (1 << 20) || T > ((int64_t)1 << 30) || T * Hq > ((int64_t)1 << 30) || T * Hkv > ((int64_t)1 << 30))
+        return fail(err, errlen, "at most 2^30 (token, head) rows per call");
+    const int64_t esz = dt == PD_DTYPE_FP32 ? 4 : 2, osz = out_dt == PD_DTYPE_FP32 ? 4 : 2;
+    if (!(heads_of_4(query, esz) && heads_of_4(key, esz) && heads_of_4(value, esz) && heads_of_4(query_out, osz)))
+        return fail(err, errlen, "query, query_out, key and value rows must be aligned to 4 elements");
+    const bool in_place = query_out->data == query->data;
+    if (in_place && !(out_dt == dt && query_out->strides[0] == query->strides[0] && query_out->strides[1] == query->strides[1]))
+        return fail(err, errlen, "query_out must be the query itself or not overlap it");
+    if (!(positions->dtype == PD_DTYPE_INT64 && positions->ndim == 1 && positions->sizes[0] >= T &&
+          (positions->strides[0] == 1 || positions->sizes[0] <= 1)))
+        return fail(err, errlen, "positions must be a contiguous int64 [T]");
+    if (!(slot_mapping->dtype == PD_DTYPE_INT64 && slot_mapping->ndim == 1 && slot_mapping->sizes[0] >= T &&
+          (slot_mapping->strides[0] == 1 || slot_mapping->sizes[0] <= 1)))
+        return fail(err, errlen, "slot_mapping must be a contiguous int64 [T]");
+    const int64_t rd = cos_sin->ndim == 2 ? cos_sin->sizes[1] : 0;
+    if (!(cos_sin->dtype == PD_DTYPE_FP32 && cos_sin->ndim == 2 && rd >= 8 && rd <= kDim && rd % 8 == 0 &&
+          cos_sin->strides[1] == 1 && cos_sin->strides[0] % 4 == 0 && reinterpret_cast<uintptr_t>(cos_sin->data) % 16 == 0))
+        return fail(err, errlen, "cos_sin must be fp32 [positions, rotary_dim], 16-byte aligned rows, rotary_dim a multiple of 8 up to 256");
+    if (T == 0) return 0;
+    RotaryWriteParams p = {};
+    p.query = query->data;
+    p.query_out = const_cast<void*>(query_out->data);
+    p.key = key->data;
+    p.value = value->data;
+    p.q_st = query->strides[0];
+    p.q_sh = query->strides[1];
+    p.o_st = query_out->strides[0];
+    p.o_sh = query_out->strides[1];
+    p.k_st = key->strides[0];
+    p.k_sh = key->strides[1];
+    p.v_st = value->strides[0];
+    p.v_sh = value->strides[1];
+    p.positions = static_cast<const int64_t*>(positions->data);
+    p.cos_sin = static_cast<const float*>(cos_sin->data);
+    p.cs_st = cos_sin->strides[0];
+    p.max_positions = cos_sin->sizes[0];
+    p.kc = static_cast<int8_t*>(const_cast<void*>(key_cache->data));
+    p.c_sb = key_cache->strides[0];
+    p.c_ss = key_cache->strides[1];
+    p.c_sh = key_cache->strides[2];
+    p.slots = static_cast<const int64_t*>(slot_mapping->data);
+    p.num_slots = key_cache->sizes[0] * key_cache->sizes[1];
+    p.T = (int)T;
+    p.Hq = (int)Hq;
+    p.Hkv = (int)Hkv;
+    p.block_size = (int)key_cache->sizes[1];
+    p.rotary_dim = (int)rd;
+    p.interleaved = interleaved != 0;
+    p.in_place = in_place;
+    return op_result(launch_rotary_write(p, dt, out_dt, stream), "rotary cache write", err, errlen);
+}
+
+// The batch of a decode step as the weights and the eviction take it.
+static bool int_rows(const pd_tensor* t, int64_t n) { return t->dtype == PD_DTYPE_INT32 && t->ndim == 1 && is_contig(t) && t->sizes[0] >= n; }
+static bool int_table(const pd_tensor* t, int64_t n) {
+    return t->dtype == PD_DTYPE_INT32 && t->ndim == 2 && t->strides[1] == 1 && t->sizes[0] >= n && t->sizes[1] <= INT32_MAX;
+}
+// fp32 [>= num_seqs, Hkv, keys] with its keys side by side
+static bool weight_rows(const pd_tensor* t, int64_t n, int64_t hkv) {
+    return t->dtype == PD_DTYPE_FP32 && t->ndim == 3 && t->sizes[0] >= n && t->sizes[1] == hkv && t->sizes[2] <= INT32_MAX &&
+           (t->strides[2] == 1 || t->sizes[2] <= 1);
+}
+
+int pth_cache_key_weights(const pd_tensor* q, const pd_tensor* key_cache, const pd_tensor* value_cache, const pd_tensor* k_scale,
+                    const pd_tensor* v_scale, const pd_tensor* block_table, const pd_tensor* seq_lens,
+                    const pd_tensor* query_start_loc, const pd_tensor* lse, const pd_tensor* weights, double scale,
+                    int64_t num_seqs, int64_t qmax, hipStream_t stream, char* err, int errlen) {
+    if (!q || !key_cache || !value_cache || !k_scale || !v_scale || !block_table || !seq_lens || !query_start_loc || !lse ||
+        !weights)
+        return fail(err, errlen, "null tensor descriptor");
+    if (!(q->dtype == PD_DTYPE_FP16 && q->ndim == 3 && q->sizes[2] == 256 && q->strides[2] == 1 &&
+          q->strides[1] == 256 && q->strides[0] % 2 == 0 && (reinterpret_cast<uintptr_t>(q->data) % 4) == 0))
+        return fail(err, errlen, "q must be fp16 [T, Hq, 256] with contiguous heads");
+    if (!layout_ok(key_cache, value_cache, k_scale, v_scale))
+        return fail(err, errlen, "KV cache views do not have the int8 per-token-head row layout");
+    const int64_t T = q->sizes[0], Hq = q->sizes[1], Hkv = key_cache->sizes[2], bs = key_cache->sizes[1];
+    if (!(Hkv > 0 && Hq > 0 && Hq % Hkv == 0 && T <= INT32_MAX && Hq <= INT32_MAX && Hkv <= 65535))
+        return fail(err, errlen, "heads_q must be a multiple of heads_kv");
+    if (!(qmax >= 1 && qmax <= INT32_MAX && qmax * (Hq / Hkv) <= 16 * kMaxRowBlocks))
+        return fail(err, errlen, "qmax * (Hq / Hkv) must be in [1, 48]");
+    if (!(num_seqs >= 1 && num_seqs <= 65535 && int_table(block_table, num_seqs) && int_rows(seq_lens, num_seqs) &&
+          int_rows(query_start_loc, num_seqs + 1)))
+        return fail(err, errlen, "block_table / seq_lens / query_start_loc must be int32 with a row for each of 1 to 65535 sequences");
+    if (const char* why = lse_refused(lse, T, Hq)) return fail(err, errlen, why);
+    if (!weight_rows(weights, num_seqs, Hkv)) return fail(err, errlen, "weights must be fp32 [num_seqs, Hkv, keys] with unit key stride");
+    if (T == 0 || weights->sizes[2] == 0) return 0;
+    KeyWeightsParams p = {};
+    p.q = static_cast<const _Float16*>(q->data);
+    p.q_st = q->strides[0];
+    p.kc = static_cast<const int8_t*>(key_cache->data);
+    p.k_sb = key_cache->strides[0];
+    p.k_ss = key_cache->strides[1];
+    p.k_sh = key_cache->strides[2];
+    p.block_table = static_cast<const int*>(block_table->data);
+    p.bt_stride = block_table->strides[0];
+    p.seq_lens = static_cast<const int*>(seq_lens->data);
+    p.qsl = static_cast<const int*>(query_start_loc->data);
+    p.lse = static_cast<const float*>(lse->data);
+    p.weights = static_cast<float*>(const_cast<void*>(weights->data));
+    p.w_sb = weights->strides[0];
+    p.w_sh = weights->strides[1];
+    p.max_keys = (int)weights->sizes[2];
+    p.block_size = (int)bs;
+    p.bs_shift = (bs & (bs - 1)) == 0 ? __builtin_ctz((unsigned)bs) : -1;
+    p.G = (int)(Hq / Hkv);
+    p.Hq = (int)Hq;
+    p.qmax = (int)qmax;
+    p.table_keys = block_table->sizes[1] * bs;
+    p.scale_log2 = (float)scale * 1.4426950408889634f;
+    return op_result(launch_key_weights(p, (int)num_seqs, (int)Hkv, stream), "key weights", err, errlen);
+}
+
+int pth_cache_evict(const pd_tensor* weights, const pd_tensor* key_cache, const pd_tensor* value_cache, const pd_tensor* k_scale,
+              const pd_tensor* v_scale, const pd_tensor* block_table, const pd_tensor* seq_lens,
+              const pd_tensor* new_block_table, const pd_tensor* new_seq_lens, const pd_tensor* new_weights,
+              const pd_tensor* kept, int64_t num_seqs, int64_t keep, int64_t recent, hipStream_t stream, char* err, int errlen) {
+    if (!weights || !key_cache || !value_cache || !k_scale || !v_scale || !block_table || !seq_lens || !new_block_table ||
+        !new_seq_lens || !new_weights || !kept)
+        return fail(err, errlen, "null tensor descriptor");
+    if (!layout_ok(key_cache, value_cache, k_scale, v_scale))
+        return fail(err, errlen, "KV cache views do not have the int8 per-token-head row layout");
+    const int64_t Hkv = key_cache->sizes[2], bs = key_cache->sizes[1];
+    if (!(keep >= 1 && keep <= INT32_MAX && recent >= 0 && recent <= keep))
+        return fail(err, errlen, "keep must be at least 1 and recent in [0, keep]");
+    if (!(num_seqs >= 1 && num_seqs <= 65535 && Hkv >= 1 && Hkv <= 65535 && int_table(block_table, num_seqs) &&
+          int_rows(seq_lens, num_seqs) && int_table(new_block_table, num_seqs) && int_rows(new_seq_lens, num_seqs)))
+        return fail(err, errlen, "block tables and sequence lengths must be int32 with a row for each of 1 to 65535 sequences");
+    if (new_block_table->sizes[1] * bs < keep) return fail(err, errlen, "new_block_table must hold keep keys");
+    if (!(weight_rows(weights, num_seqs, Hkv) && weight_rows(new_weights, num_seqs, Hkv) && new_weights->sizes[2] >= keep))
+        return fail(err, errlen, "weights and new_weights must be fp32 [num_seqs, Hkv, keys] with unit key stride, new_weights of at least keep keys");
+    if (!(kept->dtype == PD_DTYPE_INT32 && kept->ndim == 3 && kept->sizes[0] >= num_seqs && kept->sizes[1] == Hkv &&
+          kept->sizes[2] == keep && is_contig(kept)))
+        return fail(err, errlen, "kept must be contiguous int32 [num_seqs, Hkv, keep]");
+    if (new_weights->data == weights->data || new_seq_lens->data == seq_lens->data || new_block_table->data == block_table->data)
+        return fail(err, errlen, "the new tensors must not be the old ones: eviction copies to other blocks");
+    EvictParams p = {};
+    p.weights = static_cast<const float*>(weights->data);
+    p.w_sb = weights->strides[0];
+    p.w_sh = weights->strides[1];
+    p.new_weights = static_cast<float*>(const_cast<void*>(new_weights->data));
+    p.n_sb = new_weights->strides[0];
+    p.n_sh = new_weights->strides[1];
+    p.max_keys = (int)std::min(weights->sizes[2], block_table->sizes[1] * bs);
+    p.new_keys = (int)new_weights->sizes[2];
+    p.kept = static_cast<int*>(const_cast<void*>(kept->data));
+    p.seq_lens = static_cast<const int*>(seq_lens->data);
+    p.new_lens = static_cast<int*>(const_cast<void*>(new_seq_lens->data));
+    p.kc = static_cast<int8_t*>(const_cast<void*>(key_cache->data));
+    p.k_sb = key_cache->strides[0];
+    p.k_ss = key_cache->strides[1];
+    p.k_sh = key_cache->strides[2];
+    p.block_table = static_cast<const int*>(block_table->data);
+    p.bt_stride = block_table->strides[0];
+    p.new_table = static_cast<const int*>(new_block_table->data);
+    p.nt_stride = new_block_table->strides[0];
+    p.block_size = (int)bs;
+    p.Hkv = (int)Hkv;
+    p.keep = (int)keep;
+    p.recent = (int)recent;
+    return op_result(launch_evict(p, (int)num_seqs, stream), "evict", err, errlen);
 }
 
 const char* pth_dec_version(void) { return "pth_dec-gfx950 0.2"; }

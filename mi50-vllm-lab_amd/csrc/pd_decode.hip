@@ -1101,7 +1101,8 @@ __device__ __forceinline__ float group_sum(float v) {
 // that covers nsplit up to 64, so that few splits do not cost loads of clamped duplicates.
 // kLive (after pd_balanced_kernel, whose items have few segments each): the partial rows are loaded
 // once the m of the first 64 splits have said which of them hold anything.
-template <int kCols, int kPer, bool kLive>
+// kLse: the row's ln(sum_p 2^(m_p - M) l_p) + M ln 2 is stored as well (-inf where no key was seen).
+template <int kCols, int kPer, bool kLive, bool kLse>
 __global__ void __launch_bounds__(256) pd_combine_kernel(const CombineParams a) {
     constexpr int kCW = kCols / 4;  // float4 columns per wave
     constexpr int kSG = 64 / kCW;   // lanes sharing a column (segment groups)
@@ -1204,6 +1205,10 @@ __global__ void __launch_bounds__(256) pd_combine_kernel(const CombineParams a) 
                            (_Float16)(acc.w * inv)};
         _Float16* o = a.out + (int64_t)tok * a.o_st + (int64_t)head * a.o_sh + part * 4 * kCols + 4 * col;
         __builtin_memcpy(o, &h, 8);
+        if constexpr (kLse) {
+            if (part == 0 && tid == 0)
+                a.lse[(int64_t)tok * Hq + head] = L > 0.f ? (M + __builtin_amdgcn_logf(L)) * 0.6931471805599453f : kNegInf;
+        }
     }
 }
 
@@ -1338,21 +1343,21 @@ hipError_t launch_partial(const LaunchArgs& x, hipStream_t stream, int* balanced
     return launch_partial_nrb<3>(p, grid, stream, fast);
 }
 
-template <int kCols>
+template <int kCols, bool kLse>
 static void launch_combine_cols(const CombineParams& c, dim3 grid, hipStream_t stream, bool live) {
     constexpr int kSG = 64 / (kCols / 4), kMost = 64 / kSG;  // lanes per column; splits per lane for 64
     const int need = (min(c.nsplit, 64) + kSG - 1) / kSG;  // splits per lane to cover
     const dim3 block(256);
     if (live)
-        hipLaunchKernelGGL((pd_combine_kernel<kCols, 2, true>), grid, block, 0, stream, c);
+        hipLaunchKernelGGL((pd_combine_kernel<kCols, 2, true, kLse>), grid, block, 0, stream, c);
     else if (need <= 1)
-        hipLaunchKernelGGL((pd_combine_kernel<kCols, 1, false>), grid, block, 0, stream, c);
+        hipLaunchKernelGGL((pd_combine_kernel<kCols, 1, false, kLse>), grid, block, 0, stream, c);
     else if (need <= 2)
-        hipLaunchKernelGGL((pd_combine_kernel<kCols, 2, false>), grid, block, 0, stream, c);
+        hipLaunchKernelGGL((pd_combine_kernel<kCols, 2, false, kLse>), grid, block, 0, stream, c);
     else if (need <= 4 || kMost < 8)
-        hipLaunchKernelGGL((pd_combine_kernel<kCols, (kMost < 4 ? kMost : 4), false>), grid, block, 0, stream, c);
+        hipLaunchKernelGGL((pd_combine_kernel<kCols, (kMost < 4 ? kMost : 4), false, kLse>), grid, block, 0, stream, c);
     else
-        hipLaunchKernelGGL((pd_combine_kernel<kCols, (kMost < 8 ? kMost : 8), false>), grid, block, 0, stream, c);
+        hipLaunchKernelGGL((pd_combine_kernel<kCols, (kMost < 8 ? kMost : 8), false, kLse>), grid, block, 0, stream, c);
 }
 
 // `balanced`: the segments per row of a balanced partial pass, 0 after pd_partial_kernel.
@@ -1373,10 +1378,15 @@ hipError_t launch_combine(const LaunchArgs& x, hipStream_t stream, int balanced)
     // Few rows: a quarter row per workgroup for parallelism; many rows: half rows, fewer
     // workgroups (4 windowed sequences x 8 tokens x 24 heads, 768 rows: 31.3 -> 29.7 us per layer;
     // 24 rows: 12.2 against 12.6).
-    if ((int64_t)x.num_tokens * x.heads_q <= 256)
-        launch_combine_cols<16>(c, dim3(x.num_tokens, x.heads_q, 4), stream, balanced != 0);
+    const bool quarters = (int64_t)x.num_tokens * x.heads_q <= 256;
+    const dim3 grid(x.num_tokens, x.heads_q, quarters ? 4 : 2);
+    c.lse = x.lse;
+    if (x.lse)
+        quarters ? launch_combine_cols<16, true>(c, grid, stream, balanced != 0)
+                 : launch_combine_cols<32, true>(c, grid, stream, balanced != 0);
     else
-        launch_combine_cols<32>(c, dim3(x.num_tokens, x.heads_q, 2), stream, balanced != 0);
+        quarters ? launch_combine_cols<16, false>(c, grid, stream, balanced != 0)
+                 : launch_combine_cols<32, false>(c, grid, stream, balanced != 0);
     return hipGetLastError();
 }
 

@@ -1,5 +1,6 @@
 // Internal interface of libpthdec.so between the C ABI (pd_api.hip) and the kernel files
-// (pd_decode.hip, pd_prefill.hip, pd_prefill_wide.hip, pd_cache_write.hip): the parameter block each kernel takes and
+// (pd_decode.hip, pd_prefill.hip, pd_prefill_wide.hip, pd_cache_write.hip, pd_rotary_write.hip, pd_key_weights.hip,
+// pd_evict.hip): the parameter block each kernel takes and
 // the host functions that launch them. The public interface is include/pth_dec.h; nothing here
 // is exported from the library.
 #pragma once
@@ -61,6 +62,7 @@ struct CombineParams {
     int nseg;
     int nsplit;
     int qmax;
+    float* lse;              // [T, Hq] logarithms of the rows' softmax sums (may be null)
 };
 
 // Chunked prefill (pd_prefill_kernel).
@@ -111,6 +113,62 @@ struct CacheWriteParams {
     int T, Hkv, block_size;
 };
 
+// Rotary positions and the cache write (pd_rotary_write_kernel).
+struct RotaryWriteParams {
+    const void* query;
+    void* query_out;
+    const void* key;
+    const void* value;
+    int64_t q_st, q_sh, o_st, o_sh, k_st, k_sh, v_st, v_sh;  // elements between tokens / heads
+    const int64_t* positions;
+    const float* cos_sin;            // [max_positions, rotary_dim]
+    int64_t cs_st, max_positions;
+    int8_t* kc;
+    int64_t c_sb, c_ss, c_sh;        // cache bytes between blocks / slots / kv heads
+    const int64_t* slots;
+    int64_t num_slots;
+    int T, Hq, Hkv, block_size, rotary_dim, interleaved;
+    int in_place;                    // query_out is query: its other dims are there already
+    int kv_groups;                   // workgroups that take key/value rows (set by the launch)
+};
+
+// Running attention weights (pd_key_weights_kernel).
+struct KeyWeightsParams {
+    const _Float16* q;
+    int64_t q_st;
+    const int8_t* kc;
+    int64_t k_sb, k_ss, k_sh;
+    const int* block_table;
+    int64_t bt_stride;
+    const int* seq_lens;
+    const int* qsl;
+    const float* lse;                // [T, Hq], natural logarithms
+    float* weights;                  // [num_seqs, Hkv, max_keys]
+    int64_t w_sb, w_sh;
+    int max_keys, block_size, bs_shift, G, Hq, qmax;
+    int64_t table_keys;              // block table columns x block size
+    float scale_log2;
+};
+
+// Eviction (pd_evict_select_kernel, pd_evict_copy_kernel).
+struct EvictParams {
+    const float* weights;
+    int64_t w_sb, w_sh;
+    float* new_weights;
+    int64_t n_sb, n_sh;
+    int max_keys, new_keys;          // columns of weights (and the old table's keys), of new_weights
+    int* kept;                       // [num_seqs, Hkv, keep]
+    const int* seq_lens;
+    int* new_lens;
+    int8_t* kc;
+    int64_t k_sb, k_ss, k_sh;
+    const int* block_table;
+    int64_t bt_stride;
+    const int* new_table;
+    int64_t nt_stride;
+    int block_size, Hkv, keep, recent;
+};
+
 // The decode launch as the C ABI describes it (pointers, strides in bytes or elements as the
 // entry points take them).
 struct LaunchArgs {
@@ -132,6 +190,7 @@ struct LaunchArgs {
     void* out;
     int64_t o_st, o_sh;
     int window, causal;
+    float* lse;              // [num_tokens, heads_q], or null
 };
 
 // Row blocks of 16 keys never straddle a page when block_size is a multiple of 16: then every
@@ -168,6 +227,12 @@ int compute_units(hipStream_t stream);
 inline int64_t prefill_workspace_floats(int64_t B, int64_t Sq, int64_t Hq, int64_t nsplit) {
     return B * Sq * Hq * nsplit * (kDim + 2);
 }
+
+// rotary positions with the cache write (pd_rotary_write.hip); PD_DTYPE_* of query, key and value, and of query_out
+hipError_t launch_rotary_write(const RotaryWriteParams& p, int dtype, int out_dtype, hipStream_t stream);
+// running attention weights (pd_key_weights.hip) and eviction by them (pd_evict.hip)
+hipError_t launch_key_weights(const KeyWeightsParams& p, int num_seqs, int heads_kv, hipStream_t stream);
+hipError_t launch_evict(const EvictParams& p, int num_seqs, hipStream_t stream);
 
 // cache writer (pd_cache_write.hip); dtype is a PD_DTYPE_* code of key and value
 hipError_t launch_cache_write(const CacheWriteParams& p, int dtype, hipStream_t stream);

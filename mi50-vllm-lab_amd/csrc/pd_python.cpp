@@ -269,6 +269,101 @@ PyObject* cache_write(PyObject*, PyObject* const* a, Py_ssize_t n) {
     });
 }
 
+// Whether all tensors lie on the first one's GPU; false with a Python error set.
+bool same_gpu(PyObject* const* o, int n) {
+    const c10::Device dev = THPVariable_Unpack(o[0]).device();
+    bool ok = dev.is_cuda();
+    for (int i = 1; i < n; ++i) ok = ok && THPVariable_Unpack(o[i]).device() == dev;
+    if (!ok) PyErr_SetString(PyExc_RuntimeError, "all tensors must be on one GPU");
+    return ok;
+}
+
+// decode_lse(entry, q, key_cache, value_cache, k_scale, v_scale, block_table, seq_lens, query_start_loc, out, part_o,
+//            part_m, part_l, lse, scale, num_seqs, qmax, nsplit, window, causal)
+PyObject* decode_lse(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    return guarded([&]() -> PyObject* {
+        decltype(&pth_dec_decode_lse) fn;
+        pd_tensor t[13];
+        double scale;
+        int64_t v[5];
+        if (!count_is(n, 20) || !entry(a[0], fn) || !describe_all(a + 1, t, 13) || !same_gpu(a + 1, 13) || !as_double(a[14], scale))
+            return nullptr;
+        for (int i = 0; i < 5; ++i)
+            if (!as_int64(a[15 + i], v[i])) return nullptr;
+        char err[256] = "";
+        OnDevice dev(a[1]);
+        int rc;
+        Py_BEGIN_ALLOW_THREADS;
+        rc = fn(&t[0], &t[1], &t[2], &t[3], &t[4], &t[5], &t[6], &t[7], &t[8], scale, &t[9], &t[10], &t[11], &t[12], v[0], v[1],
+                v[2], v[3], v[4], dev.stream, err, (int)sizeof err);
+        Py_END_ALLOW_THREADS;
+        return done(rc, err);
+    });
+}
+
+// rotary_cache_write(entry, query, query_out, key, value, positions, cos_sin, key_cache, value_cache, k_scale, v_scale,
+//                    slot_mapping, interleaved)
+PyObject* rotary_cache_write(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    return guarded([&]() -> PyObject* {
+        decltype(&pth_cache_write_rotary) fn;
+        pd_tensor t[11];
+        int64_t interleaved;
+        if (!count_is(n, 13) || !entry(a[0], fn) || !describe_all(a + 1, t, 11) || !same_gpu(a + 1, 11) || !as_int64(a[12], interleaved))
+            return nullptr;
+        char err[256] = "";
+        OnDevice dev(a[1]);
+        int rc;
+        Py_BEGIN_ALLOW_THREADS;
+        rc = fn(&t[0], &t[1], &t[2], &t[3], &t[4], &t[5], &t[6], &t[7], &t[8], &t[9], &t[10], interleaved, dev.stream, err,
+                (int)sizeof err);
+        Py_END_ALLOW_THREADS;
+        return done(rc, err);
+    });
+}
+
+// key_weights(entry, q, key_cache, value_cache, k_scale, v_scale, block_table, seq_lens, query_start_loc, lse, weights, scale,
+//             num_seqs, qmax)
+PyObject* key_weights(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    return guarded([&]() -> PyObject* {
+        decltype(&pth_cache_key_weights) fn;
+        pd_tensor t[10];
+        double scale;
+        int64_t num_seqs, qmax;
+        if (!count_is(n, 14) || !entry(a[0], fn) || !describe_all(a + 1, t, 10) || !same_gpu(a + 1, 10) || !as_double(a[11], scale) ||
+            !as_int64(a[12], num_seqs) || !as_int64(a[13], qmax))
+            return nullptr;
+        char err[256] = "";
+        OnDevice dev(a[1]);
+        int rc;
+        Py_BEGIN_ALLOW_THREADS;
+        rc = fn(&t[0], &t[1], &t[2], &t[3], &t[4], &t[5], &t[6], &t[7], &t[8], &t[9], scale, num_seqs, qmax, dev.stream, err,
+                (int)sizeof err);
+        Py_END_ALLOW_THREADS;
+        return done(rc, err);
+    });
+}
+
+// evict(entry, weights, key_cache, value_cache, k_scale, v_scale, block_table, seq_lens, new_block_table, new_seq_lens,
+//       new_weights, kept, num_seqs, keep, recent)
+PyObject* evict(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    return guarded([&]() -> PyObject* {
+        decltype(&pth_cache_evict) fn;
+        pd_tensor t[11];
+        int64_t num_seqs, keep, recent;
+        if (!count_is(n, 15) || !entry(a[0], fn) || !describe_all(a + 1, t, 11) || !same_gpu(a + 1, 11) || !as_int64(a[12], num_seqs) ||
+            !as_int64(a[13], keep) || !as_int64(a[14], recent))
+            return nullptr;
+        char err[256] = "";
+        OnDevice dev(a[1]);
+        int rc;
+        Py_BEGIN_ALLOW_THREADS;
+        rc = fn(&t[0], &t[1], &t[2], &t[3], &t[4], &t[5], &t[6], &t[7], &t[8], &t[9], &t[10], num_seqs, keep, recent, dev.stream,
+                err, (int)sizeof err);
+        Py_END_ALLOW_THREADS;
+        return done(rc, err);
+    });
+}
+
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 // The lengths of a batch on the host: a contiguous int32 or int64 CPU tensor.
@@ -465,6 +560,10 @@ PyMethodDef methods[] = {
     PD_METHOD(prefill_split, "pth_fa_forward_split on torch tensors"),
     PD_METHOD(prefill_balanced, "pth_fa_forward_balanced on torch tensors"),
     PD_METHOD(cache_write, "pth_cache_write on torch tensors"),
+    PD_METHOD(decode_lse, "pth_dec_decode_lse on torch tensors"),
+    PD_METHOD(rotary_cache_write, "pth_cache_write_rotary on torch tensors"),
+    PD_METHOD(key_weights, "pth_cache_key_weights on torch tensors"),
+    PD_METHOD(evict, "pth_cache_evict on torch tensors"),
     PD_METHOD(plan_decode, "split count of a decode batch"),
     PD_METHOD(deal_pays, "whether a batch of unsplit sequences is dealt instead"),
     PD_METHOD(plan_prefill, "key splits of a prefill launch"),

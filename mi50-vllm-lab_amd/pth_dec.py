@@ -50,6 +50,7 @@ EXPORTED_SYMBOLS = (
     "pth_dec_launch_combine",
     "pth_dec_supported_layout",
     "pth_dec_decode",
+    "pth_dec_decode_lse",
     "pth_dec_version",
     "pth_fa_forward",
     "pth_fa_forward_exact",
@@ -57,6 +58,9 @@ EXPORTED_SYMBOLS = (
     "pth_fa_forward_balanced",
     "pth_fa_balanced_workspace",
     "pth_cache_write",
+    "pth_cache_write_rotary",
+    "pth_cache_key_weights",
+    "pth_cache_evict",
 )
 
 
@@ -140,11 +144,20 @@ def load_library(path: str | None = None) -> ctypes.CDLL:
     lib.pth_fa_balanced_workspace.restype = ctypes.c_int64
     lib.pth_cache_write.argtypes = [tp] * 7 + [vp, ctypes.c_char_p, c_int]
     lib.pth_cache_write.restype = c_int
+    lib.pth_dec_decode_lse.argtypes = [tp] * 9 + [c_double, tp, tp, tp, tp] + [ctypes.c_int64] * 5 + [vp, ctypes.c_char_p, c_int]
+    lib.pth_dec_decode_lse.restype = c_int
+    lib.pth_cache_write_rotary.argtypes = [tp] * 11 + [ctypes.c_int64, vp, ctypes.c_char_p, c_int]
+    lib.pth_cache_write_rotary.restype = c_int
+    lib.pth_cache_key_weights.argtypes = [tp] * 10 + [c_double, ctypes.c_int64, ctypes.c_int64, vp, ctypes.c_char_p, c_int]
+    lib.pth_cache_key_weights.restype = c_int
+    lib.pth_cache_evict.argtypes = [tp] * 11 + [ctypes.c_int64] * 3 + [vp, ctypes.c_char_p, c_int]
+    lib.pth_cache_evict.restype = c_int
     lib.pth_dec_version.argtypes = []
     lib.pth_dec_version.restype = ctypes.c_char_p
     _entries.update({name: ctypes.cast(getattr(lib, name), vp).value
                      for name in ("pth_dec_decode", "pth_fa_forward", "pth_fa_forward_exact", "pth_fa_forward_split",
-                                  "pth_fa_forward_balanced", "pth_fa_balanced_workspace", "pth_cache_write")})
+                                  "pth_fa_forward_balanced", "pth_fa_balanced_workspace", "pth_cache_write", "pth_dec_decode_lse",
+                                  "pth_cache_write_rotary", "pth_cache_key_weights", "pth_cache_evict")})
     _lib, _lib_path = lib, os.path.realpath(p)
     return lib
 
@@ -183,7 +196,7 @@ def decode(q: torch.Tensor, key_cache: torch.Tensor, value_cache: torch.Tensor, 
            v_scale: torch.Tensor, block_table: torch.Tensor, seq_lens: torch.Tensor,
            query_start_loc: torch.Tensor, out: torch.Tensor, scale: float, part_o: torch.Tensor,
            part_m: torch.Tensor, part_l: torch.Tensor, num_seqs: int, qmax: int, nsplit: int,
-           window: int = -1, causal: bool = True) -> None:
+           window: int = -1, causal: bool = True, lse: torch.Tensor | None = None) -> None:
     """Split-K decode attention over the int8 per-token-head paged KV cache, written into `out`.
 
     q: fp16 [T, Hq, 256] with head stride 256; out: fp16 [T, Hq, 256] with unit dim stride;
@@ -191,10 +204,17 @@ def decode(q: torch.Tensor, key_cache: torch.Tensor, value_cache: torch.Tensor, 
     query_start_loc int32 [>= num_seqs + 1]; every sequence has <= qmax query tokens;
     part_o fp32 [>= T, Hq, NSEG, 256], part_m / part_l fp32 [>= T, Hq, NSEG] (caller-owned
     scratch, vLLM's softmax segment buffers); 1 <= nsplit <= NSEG.
+    lse (fp32 [>= T, Hq], no counterpart in the reference): also receives ln(sum over the visible keys of
+    e^(scale q . k)) of each row, -inf for a row that sees none (pth_dec_decode_lse); key_weights reads it.
     Reference: kernels/pth_dec/pth_dec.cpp:43-91.
     """
     if not q.is_cuda:
         raise RuntimeError("q must be fp16 [T, Hq, 256] with contiguous heads")
+    if lse is not None:
+        native().decode_lse(_entry("pth_dec_decode_lse"), q, key_cache, value_cache, k_scale, v_scale, block_table, seq_lens,
+                            query_start_loc, out, part_o, part_m, part_l, lse, scale, int(num_seqs), int(qmax), int(nsplit),
+                            int(window), 1 if causal else 0)
+        return
     native().decode(_entry("pth_dec_decode"), q, key_cache, value_cache, k_scale, v_scale, block_table, seq_lens,
                     query_start_loc, out, scale, part_o, part_m, part_l, int(num_seqs), int(qmax), int(nsplit),
                     int(window), 1 if causal else 0)
@@ -362,6 +382,55 @@ def cache_write(key: torch.Tensor, value: torch.Tensor, key_cache: torch.Tensor,
     if not key.is_cuda:
         raise RuntimeError("key and value must be fp16, bf16 or fp32 of the same dtype")
     native().cache_write(_entry("pth_cache_write"), key, value, key_cache, value_cache, k_scale, v_scale, slot_mapping)
+
+
+def rotary_cache_write(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor, positions: torch.Tensor,
+                       cos_sin: torch.Tensor, key_cache: torch.Tensor, value_cache: torch.Tensor, k_scale: torch.Tensor,
+                       v_scale: torch.Tensor, slot_mapping: torch.Tensor, interleaved: bool = False,
+                       query_out: torch.Tensor | None = None) -> None:
+    """Rotary positions on the new tokens' query and key heads and the cache write, in one launch (no counterpart in
+    the reference, whose engine rotates in a kernel of its own before the cache update).
+
+    query [T, Hq, 256], key and value [T, Hkv, 256]: fp16, bf16 or fp32 views (of a fused projection, say); positions
+    int64 [T]; cos_sin fp32 [positions, rotary_dim] (rotary.rotary_table). The query is rotated in place or into query_out
+    (its dtype, or fp16 for the decode operator); the key is rotated in fp32 and quantised with the value into the
+    int8 rows at slot_mapping, as cache_write does; key and value themselves stay as they are. interleaved: pairs are
+    dims (2 i, 2 i + 1) instead of (i, i + rotary_dim / 2). Tokens at positions outside the table are skipped, negative
+    slots (padding) write no row.
+    """
+    native().rotary_cache_write(_entry("pth_cache_write_rotary"), query, query if query_out is None else query_out, key, value,
+                                positions, cos_sin, key_cache, value_cache, k_scale, v_scale, slot_mapping, 1 if interleaved else 0)
+
+
+def key_weights(q: torch.Tensor, key_cache: torch.Tensor, value_cache: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor,
+                block_table: torch.Tensor, seq_lens: torch.Tensor, query_start_loc: torch.Tensor, lse: torch.Tensor,
+                weights: torch.Tensor, scale: float, num_seqs: int, qmax: int) -> None:
+    """Adds to weights [num_seqs, Hkv, keys] (fp32) the softmax weight that a decode step's query rows gave each
+    cached key, summed over the rows of the kv head (no counterpart in the reference).
+
+    The arguments up to query_start_loc, scale, num_seqs and qmax are decode's, of a causal step without window; lse
+    [>= T, Hq] is what decode(..., lse=) or decode_shared(..., lse=) stored for it. Keys past the last column of weights are
+    not counted. evict keeps the keys with the largest sums.
+    """
+    native().key_weights(_entry("pth_cache_key_weights"), q, key_cache, value_cache, k_scale, v_scale, block_table, seq_lens,
+                         query_start_loc, lse, weights, scale, int(num_seqs), int(qmax))
+
+
+def evict(weights: torch.Tensor, key_cache: torch.Tensor, value_cache: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor,
+          block_table: torch.Tensor, seq_lens: torch.Tensor, new_block_table: torch.Tensor, new_seq_lens: torch.Tensor,
+          new_weights: torch.Tensor, kept: torch.Tensor, num_seqs: int, keep: int, recent: int) -> None:
+    """Cuts each sequence down to `keep` keys per kv head: the last `recent` and the others with the largest weights, ties to
+    the lowest key, in the order of their positions (no counterpart in the reference).
+
+    The kept rows are copied into the blocks of new_block_table (int32 [>= num_seqs, columns for keep keys]), which must not
+    be among those that the call reads; the old blocks stay as they are, also where other sequences share
+    them, and are free once the call is done. Written: new_seq_lens (int32, min(seq_len, keep)), new_weights (fp32
+    [>= num_seqs, Hkv, >= keep]: the kept keys' sums, then zeros, as key_weights goes on with them) and kept (int32 [>=
+    num_seqs, Hkv, keep]: their numbers, then -1). Sequences of at most keep keys are copied whole. The keys stay rotated
+    by their own positions; tokens written later go on counting from the sequence's full length.
+    """
+    native().evict(_entry("pth_cache_evict"), weights, key_cache, value_cache, k_scale, v_scale, block_table, seq_lens, new_block_table,
+                   new_seq_lens, new_weights, kept, int(num_seqs), int(keep), int(recent))
 
 
 def _ptr(t: torch.Tensor, ctype):
