@@ -159,6 +159,27 @@ int pth_dec_decode_lse(const pd_tensor* q, const pd_tensor* key_cache, const pd_
                        const pd_tensor* lse, int64_t num_seqs, int64_t qmax, int64_t nsplit, int64_t window,
                        int64_t causal, hipStream_t stream, char* err, int errlen);
 
+/*
+ * Decode attention of a batch whose sequences share their first prefix_len keys (a common prompt or document, samples of
+ * one prompt): pth_dec_decode's causal attention without window, with the shared keys read once for the whole batch. No
+ * counterpart in the reference.
+ *   q .. part_l, num_seqs, qmax   as for pth_dec_decode; at least 4 segments in the partial buffers
+ *   lse          null, or as for pth_dec_decode_lse
+ *   prefix_len   >= 0, within the block table; the tables of the sequences that hold the prefix and their query tokens
+ *                behind it (seq_len - q_len >= prefix_len) name the same keys for it (the same blocks, or for a block that
+ *                the prefix ends in, blocks that agree on its keys): the table of the first such sequence is
+ *                read. Sequences that do not are computed from their own table alone.
+ * At most 2^25 (token, head) rows and 2^30 / heads_kv key tiles that the block table can hold. Each shared key's weight
+ * enters P.V as one fp16 (as pth_fa_forward's) when the batch has more than 32 rows per kv head, else as the decode's
+ * hi + lo; the own keys' always as hi + lo. Returns 0, 1 or 2 as above.
+ */
+int pth_dec_decode_shared(const pd_tensor* q, const pd_tensor* key_cache, const pd_tensor* value_cache,
+                          const pd_tensor* k_scale, const pd_tensor* v_scale, const pd_tensor* block_table,
+                          const pd_tensor* seq_lens, const pd_tensor* query_start_loc, const pd_tensor* out,
+                          double scale, const pd_tensor* part_o, const pd_tensor* part_m, const pd_tensor* part_l,
+                          const pd_tensor* lse, int64_t num_seqs, int64_t qmax, int64_t prefix_len,
+                          hipStream_t stream, char* err, int errlen);
+
 /* Library version string. */
 const char* pth_dec_version(void);
 
@@ -290,7 +311,7 @@ int pth_cache_write_rotary(const pd_tensor* query, const pd_tensor* query_out, c
  * Running attention weights of the cached keys: adds to weights[b, g, t] the softmax weight that the query rows of
  * sequence b and kv head g gave key t, sum over rows of e^(scale q . k_t - lse). No counterpart in the reference.
  *   q, key_cache .. query_start_loc, scale, num_seqs, qmax   as for pth_dec_decode (causal, no window)
- *   lse          fp32, contiguous [>= T, Hq], of pth_dec_decode_lse on the same rows; a row of
+ *   lse          fp32, contiguous [>= T, Hq], of pth_dec_decode_lse or _shared on the same rows; a row of
  *                -inf adds nothing
  *   weights      fp32 [>= num_seqs, Hkv, keys], unit key stride; only keys below seq_len and below `keys` are touched
  * Every weight is formed in a fixed order (no atomics). Returns 0, 1 or 2 as above.

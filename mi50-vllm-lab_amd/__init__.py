@@ -6,8 +6,8 @@ The directory name is not a Python identifier; load it with `load_package()` fro
 `__graft_entry__` / `tests/conftest.py`, which registers it as `mi50_vllm_lab_amd`.
 """
 from . import kvcache, pth_dec, rotary, vllm_shim  # noqa: F401
-from .pth_dec import cache_write, decode, evict, forward_pth, key_weights, rotary_cache_write, supported_layout  # noqa: F401
+from .pth_dec import cache_write, decode, decode_shared, evict, forward_pth, key_weights, rotary_cache_write, supported_layout  # noqa: F401
 from .rotary import rotary_table  # noqa: F401
 
-__all__ = ["cache_write", "decode", "evict", "forward_pth", "key_weights", "rotary_cache_write", "rotary_table",
+__all__ = ["cache_write", "decode", "decode_shared", "evict", "forward_pth", "key_weights", "rotary_cache_write", "rotary_table",
            "supported_layout", "kvcache", "pth_dec", "rotary", "vllm_shim"]

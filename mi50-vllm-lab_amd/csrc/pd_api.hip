@@ -199,12 +199,15 @@ static const char* lse_refused(const pd_tensor* lse, int64_t T, int64_t Hq) {
     return ok ? nullptr : "lse must be contiguous fp32 [T, Hq]";
 }
 
+static int64_t cache_span(const pd_tensor* kc);
+
+// The decode entries' body; prefix >= 0: the shared-prefix decode (nsplit is not looked at beyond its check).
 static int decode_entry(const pd_tensor* q, const pd_tensor* key_cache, const pd_tensor* value_cache,
                         const pd_tensor* k_scale, const pd_tensor* v_scale, const pd_tensor* block_table,
                         const pd_tensor* seq_lens, const pd_tensor* query_start_loc, const pd_tensor* out, double scale,
                         const pd_tensor* part_o, const pd_tensor* part_m, const pd_tensor* part_l, const pd_tensor* lse,
                         int64_t num_seqs, int64_t qmax, int64_t nsplit, int64_t window, int64_t causal,
-                        hipStream_t stream, char* err, int errlen) {
+                        hipStream_t stream, char* err, int errlen, int64_t prefix = -1) {
     if (!q || !key_cache || !value_cache || !k_scale || !v_scale || !block_table || !seq_lens ||
         !query_start_loc || !out || !part_o || !part_m || !part_l)
         return fail(err, errlen, "null tensor descriptor");
@@ -242,6 +245,16 @@ static int decode_entry(const pd_tensor* q, const pd_tensor* key_cache, const pd
           block_table->sizes[0] >= num_seqs))
         return fail(err, errlen, "per-sequence tensors too small");
     if (const char* why = lse_refused(lse, T, Hq)) return fail(err, errlen, why);
+    if (prefix >= 0) {
+        const int64_t bs = key_cache->sizes[1], cols = block_table->sizes[1];
+        if (nseg < kSharedMinSegments) return fail(err, errlen, "a shared-prefix decode needs at least 4 segments");
+        if (!(prefix <= INT32_MAX && bs > 0 && cols <= INT32_MAX && prefix <= cols * bs))
+            return fail(err, errlen, "prefix_len must be within the block table");
+        // 32 bits number the rows and the line of own key tiles
+        const int64_t tiles = cols * bs / 32 + 16;
+        if (!(Hq >= 1 && T <= ((int64_t)1 << 25) / Hq && tiles <= INT32_MAX / 2 && tiles * num_seqs <= INT32_MAX / (2 * Hkv)))
+            return fail(err, errlen, "a shared-prefix decode takes at most 2^25 (token, head) rows and 2^30 key tiles");
+    }
     if (T == 0) return 0;
     LaunchArgs x = make_args(
         q->data, q->strides[0], key_cache->data, key_cache->strides[0], key_cache->strides[1],
@@ -252,7 +265,9 @@ static int decode_entry(const pd_tensor* q, const pd_tensor* key_cache, const pd
         static_cast<float*>(const_cast<void*>(part_l->data)), (int)nseg, (int)nsplit, const_cast<void*>(out->data),
         out->strides[0], out->strides[1], (int)window, (int)causal);
     x.lse = lse ? static_cast<float*>(const_cast<void*>(lse->data)) : nullptr;
-    const hipError_t e = launch_all(x, stream, false);
+    // (16-key block offsets fit a 32-bit LDS table in 8-byte units when the cache spans less than 2^35 bytes)
+    const hipError_t e = prefix < 0 ? launch_all(x, stream, false)
+                                    : launch_shared(x, (int)prefix, cache_span(key_cache) < ((int64_t)1 << 35), stream);
     if (e != hipSuccess) {
         char msg[256];
         snprintf(msg, sizeof msg, "pth_dec launch failed: %s", hipGetErrorString(e));
@@ -281,6 +296,16 @@ int pth_dec_decode_lse(const pd_tensor* q, const pd_tensor* key_cache, const pd_
     if (!lse) return fail(err, errlen, "null tensor descriptor");
     return decode_entry(q, key_cache, value_cache, k_scale, v_scale, block_table, seq_lens, query_start_loc, out, scale,
                         part_o, part_m, part_l, lse, num_seqs, qmax, nsplit, window, causal, stream, err, errlen);
+}
+
+int pth_dec_decode_shared(const pd_tensor* q, const pd_tensor* key_cache, const pd_tensor* value_cache,
+                          const pd_tensor* k_scale, const pd_tensor* v_scale, const pd_tensor* block_table,
+                          const pd_tensor* seq_lens, const pd_tensor* query_start_loc, const pd_tensor* out, double scale,
+                          const pd_tensor* part_o, const pd_tensor* part_m, const pd_tensor* part_l, const pd_tensor* lse,
+                          int64_t num_seqs, int64_t qmax, int64_t prefix_len, hipStream_t stream, char* err, int errlen) {
+    if (prefix_len < 0) return fail(err, errlen, "prefix_len must be within the block table");
+    return decode_entry(q, key_cache, value_cache, k_scale, v_scale, block_table, seq_lens, query_start_loc, out, scale,
+                        part_o, part_m, part_l, lse, num_seqs, qmax, 1, -1, 1, stream, err, errlen, prefix_len);
 }
 
 static int fa_result(hipError_t e, char* err, int errlen) {

@@ -1,6 +1,6 @@
 // Internal interface of libpthdec.so between the C ABI (pd_api.hip) and the kernel files
 // (pd_decode.hip, pd_prefill.hip, pd_prefill_wide.hip, pd_cache_write.hip, pd_rotary_write.hip, pd_key_weights.hip,
-// pd_evict.hip): the parameter block each kernel takes and
+// pd_evict.hip, pd_shared.hip): the parameter block each kernel takes and
 // the host functions that launch them. The public interface is include/pth_dec.h; nothing here
 // is exported from the library.
 #pragma once
@@ -63,6 +63,18 @@ struct CombineParams {
     int nsplit;
     int qmax;
     float* lse;              // [T, Hq] logarithms of the rows' softmax sums (may be null)
+};
+
+// Shared-prefix decode (pd_shared_kernel, pd_shared_combine_kernel): the decode's own parameters (nsplit: the segments
+// of a row that may be used, the last of them for the row's own note) and the prefix.
+struct SharedParams {
+    PartialParams p;
+    int num_tokens;          // rows of q and out
+    int prefix;              // keys that every sequence begins with
+    int bt32;                // every K row lies within 2^35 bytes of the cache base
+    _Float16* out;
+    int64_t o_st, o_sh;
+    float* lse;              // may be null
 };
 
 // Chunked prefill (pd_prefill_kernel).
@@ -206,6 +218,10 @@ hipError_t launch_all(const LaunchArgs& x, hipStream_t stream, bool strict);
 // the device array behind pth_dec_launch_noalloc, and its address on the current device
 constexpr size_t kScratchBytes = size_t(32) << 20;
 hipError_t scratch_address(void** out);
+
+// shared-prefix decode (pd_shared.hip)
+constexpr int kSharedMinSegments = 4;  // prefix, two for a sequence's own keys, the note
+hipError_t launch_shared(const LaunchArgs& x, int prefix, int bt32, hipStream_t stream);
 
 // chunked prefill (pd_prefill.hip)
 // exact: K converted to fp16 without the widening bias and P' as fp16 hi + lo (pth_fa_forward_exact)

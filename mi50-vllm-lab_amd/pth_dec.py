@@ -51,6 +51,7 @@ EXPORTED_SYMBOLS = (
     "pth_dec_supported_layout",
     "pth_dec_decode",
     "pth_dec_decode_lse",
+    "pth_dec_decode_shared",
     "pth_dec_version",
     "pth_fa_forward",
     "pth_fa_forward_exact",
@@ -146,6 +147,8 @@ def load_library(path: str | None = None) -> ctypes.CDLL:
     lib.pth_cache_write.restype = c_int
     lib.pth_dec_decode_lse.argtypes = [tp] * 9 + [c_double, tp, tp, tp, tp] + [ctypes.c_int64] * 5 + [vp, ctypes.c_char_p, c_int]
     lib.pth_dec_decode_lse.restype = c_int
+    lib.pth_dec_decode_shared.argtypes = [tp] * 9 + [c_double, tp, tp, tp, tp] + [ctypes.c_int64] * 3 + [vp, ctypes.c_char_p, c_int]
+    lib.pth_dec_decode_shared.restype = c_int
     lib.pth_cache_write_rotary.argtypes = [tp] * 11 + [ctypes.c_int64, vp, ctypes.c_char_p, c_int]
     lib.pth_cache_write_rotary.restype = c_int
     lib.pth_cache_key_weights.argtypes = [tp] * 10 + [c_double, ctypes.c_int64, ctypes.c_int64, vp, ctypes.c_char_p, c_int]
@@ -157,7 +160,7 @@ def load_library(path: str | None = None) -> ctypes.CDLL:
     _entries.update({name: ctypes.cast(getattr(lib, name), vp).value
                      for name in ("pth_dec_decode", "pth_fa_forward", "pth_fa_forward_exact", "pth_fa_forward_split",
                                   "pth_fa_forward_balanced", "pth_fa_balanced_workspace", "pth_cache_write", "pth_dec_decode_lse",
-                                  "pth_cache_write_rotary", "pth_cache_key_weights", "pth_cache_evict")})
+                                  "pth_dec_decode_shared", "pth_cache_write_rotary", "pth_cache_key_weights", "pth_cache_evict")})
     _lib, _lib_path = lib, os.path.realpath(p)
     return lib
 
@@ -218,6 +221,23 @@ def decode(q: torch.Tensor, key_cache: torch.Tensor, value_cache: torch.Tensor, 
     native().decode(_entry("pth_dec_decode"), q, key_cache, value_cache, k_scale, v_scale, block_table, seq_lens,
                     query_start_loc, out, scale, part_o, part_m, part_l, int(num_seqs), int(qmax), int(nsplit),
                     int(window), 1 if causal else 0)
+
+
+def decode_shared(q: torch.Tensor, key_cache: torch.Tensor, value_cache: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor,
+                  block_table: torch.Tensor, seq_lens: torch.Tensor, query_start_loc: torch.Tensor, out: torch.Tensor, scale: float,
+                  part_o: torch.Tensor, part_m: torch.Tensor, part_l: torch.Tensor, num_seqs: int, qmax: int, prefix_len: int,
+                  lse: torch.Tensor | None = None) -> None:
+    """decode's causal attention (no window) for a batch whose sequences share their first prefix_len keys, which are read once
+    for the whole batch instead of once per sequence (no counterpart in the reference).
+
+    The arguments up to qmax are decode's, without nsplit: the work is dealt over the GPU by the lengths on the device; the
+    partial buffers need NSEG >= 4. prefix_len keys, within the block table's width: the tables of all sequences that hold them
+    before their query tokens name the same blocks for them (a block that the prefix ends in may be each sequence's own
+    copy). A sequence that does not hold them, seq_len - q_len < prefix_len, is computed from its own table alone, and a padded
+    one (seq_len 0 or no query tokens) is left alone. lse: as decode's.
+    """
+    native().decode_shared(_entry("pth_dec_decode_shared"), q, key_cache, value_cache, k_scale, v_scale, block_table, seq_lens,
+                           query_start_loc, out, part_o, part_m, part_l, lse, scale, int(num_seqs), int(qmax), int(prefix_len))
 
 
 PREFILL_ROWS_PER_WORKGROUP = 192  # query rows (tokens x heads of one kv head) per prefill workgroup

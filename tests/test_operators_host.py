@@ -187,6 +187,48 @@ def test_decode_lse_refusals(lib):
     assert rc == 1 and "q must be fp16" in text
 
 
+def test_decode_shared_refusals(lib):
+    case = make()
+    c = case.cache
+    table = case.block_table.shape[1] * 16
+    front = [case.q, c.key_cache, c.value_cache, c.k_scale, c.v_scale, case.block_table, case.seq_lens, case.query_start_loc,
+             torch.zeros((4, 12, 256), dtype=torch.float16)]
+
+    def run(prefix=32, nseg=4, qmax=3, num_seqs=2, lse=None, at=None, t=None):
+        ts = list(front)
+        if at is not None:
+            ts[at] = t
+        d = lambda xs: [None if x is None else ctypes.byref(pth_dec.describe(x)) for x in xs]  # noqa: E731
+        err = ctypes.create_string_buffer(256)
+        rc = lib.pth_dec_decode_shared(*d(ts), ctypes.c_double(0.1), *d([*kvc.partial_buffers(4, 12, nseg, "cpu"), lse]), num_seqs, qmax,
+                                       prefix, None, err, len(err))
+        return rc, err.value.decode()
+
+    one = torch.zeros((1, 1, 256), dtype=torch.float16)
+    for kw, msg in (
+        (dict(prefix=-1), "prefix_len must be"), (dict(prefix=table + 1), "prefix_len must be"), (dict(prefix=1 << 31), "prefix_len must be"),
+        (dict(nseg=3), "at least 4 segments"), (dict(qmax=9), "[1, 48]"), (dict(qmax=0), "[1, 48]"), (dict(num_seqs=3), "too small"),
+        (dict(num_seqs=0), "too small"), (dict(lse=torch.zeros((4, 11))), "lse must be"),
+        (dict(at=0, t=None), "null tensor descriptor"), (dict(at=0, t=case.q.float()), "q must be fp16"),
+        (dict(at=2, t=c.key_cache), "KV cache views"), (dict(at=5, t=case.block_table.long()), "must be int32"),
+        (dict(at=8, t=one.expand(4, 12, 256).transpose(0, 1)), "out must be"),
+    ):
+        rc, text = run(**kw)
+        assert rc == 1 and msg in text, (list(kw), rc, text)
+    # a table wide enough for more key tiles than 32 bits number (described, never read)
+    wide = pth_dec.describe(case.block_table)
+    wide.sizes[1] = 1 << 30
+    err = ctypes.create_string_buffer(256)
+    descs = [pth_dec.describe(x) for x in front]
+    descs[5] = wide
+    assert lib.pth_dec_decode_shared(*[ctypes.byref(x) for x in descs], ctypes.c_double(0.1),
+                                     *[ctypes.byref(pth_dec.describe(x)) for x in kvc.partial_buffers(4, 12, 4, "cpu")], None, 2, 3, 32, None,
+                                     err, len(err)) == 1 and b"at most 2^25" in err.value
+    assert lib.pth_dec_decode_shared(*[ctypes.byref(pth_dec.describe(x[:0] if i in (0, 8) else x)) for i, x in enumerate(front)],
+                                     ctypes.c_double(0.1), *[ctypes.byref(pth_dec.describe(x)) for x in kvc.partial_buffers(4, 12, 4, "cpu")],
+                                     None, 2, 3, 32, None, None, 0) == 0
+
+
 def test_python_face_refuses_host_tensors():
     case = make()
     c = case.cache
@@ -196,6 +238,9 @@ def test_python_face_refuses_host_tensors():
     i32 = lambda *s: torch.zeros(s, dtype=torch.int32)  # noqa: E731
     with pytest.raises(RuntimeError, match="one GPU"):
         pth_dec.rotary_cache_write(x[:, :12], x[:, 12:14], x[:, 14:], n64, torch.zeros((9, 64)), *views, n64)
+    with pytest.raises(RuntimeError, match="one GPU"):
+        pth_dec.decode_shared(case.q, *views, case.block_table, case.seq_lens, case.query_start_loc, torch.empty_like(case.q), 0.1,
+                              *kvc.partial_buffers(4, 12, 4, "cpu"), 2, 3, 16)
     with pytest.raises(RuntimeError, match="one GPU"):
         pth_dec.key_weights(case.q, *views, case.block_table, case.seq_lens, case.query_start_loc, torch.zeros((4, 12)),
                             torch.zeros((2, 2, 50)), 0.1, 2, 3)
