@@ -40,50 +40,60 @@ __global__ void __launch_bounds__(64 * kKwWaves) pd_key_weights_kernel(const Key
     const int first = blockIdx.x * kKwWaves + w;
     if (first >= nblk) return;
 
-    // ---- Q^T: lane (lg, li) holds row 16 rb + li, dims 64 (st / 2) + 16 lg + 8 (st % 2) + [0, 8) ----
-    half8_t qop[NRB][8];
-    float nlse[NRB];  // -lse in log2 units; -inf for a row that counts for nothing
-    int rpos[NRB];
-#pragma unroll
-    for (int rb = 0; rb < NRB; ++rb) {
-        const int r = 16 * rb + li;
-        const bool valid = r < R;
-        const int qi = valid ? r / G : 0, qh = valid ? r - qi * G : 0;
-        const _Float16* qrow = a.q + (int64_t)(q0 + qi) * a.q_st + (int64_t)(g * G + qh) * kDim;
-#pragma unroll
-        for (int st = 0; st < 8; ++st) {
-            half8_t v;
-            __builtin_memcpy(&v, __builtin_assume_aligned(qrow + 64 * (st >> 1) + 16 * lg + 8 * (st & 1), 4), 16);
-            qop[rb][st] = valid ? v : (half8_t)(_Float16)0.0f;
-        }
-        const float lse = a.lse[(int64_t)(q0 + qi) * a.Hq + g * G + qh];
-        // a row whose sum was 0 (lse -inf) weighs nothing, and neither does a row past the last
-        nlse[rb] = valid && lse != kNegInf ? -lse * 1.4426950408889634f : kNegInf;
-        rpos[rb] = valid ? ctx0 + qi : -1;
-    }
-
     const int8_t* gbase = a.kc + (int64_t)g * a.k_sh;
     const int* bt = a.block_table + (int64_t)b * a.bt_stride;
     float* wrow = a.weights + (int64_t)b * a.w_sb + (int64_t)g * a.w_sh;
+    // Three stages of a block, each a memory round trip, run one behind the other: the page of this lane's key, the operand
+    // bytes of its row (keys past the last are the last), the products.
+    auto key_of = [&](int n) __attribute__((always_inline)) { return min(n * kKwKeys + li, seq_len - 1); };
+    auto slot_of = [&](int key) __attribute__((always_inline)) { return a.bs_shift >= 0 ? key >> a.bs_shift : key / a.block_size; };
+    auto page_of = [&](int n) __attribute__((always_inline)) { return n < nblk ? bt[slot_of(key_of(n))] : 0; };
     struct Block {
         uint4_t k[4];
         float ks;
     };
-    // this lane's operand bytes of key 16 n + li, and that key's scale; keys past the last are the last
-    auto fetch = [&](int n) __attribute__((always_inline)) {
-        const int key = min(n * kKwKeys + li, seq_len - 1);
-        const int lb = a.bs_shift >= 0 ? key >> a.bs_shift : key / a.block_size;
-        const int8_t* row = gbase + (int64_t)bt[lb] * a.k_sb + (int64_t)(key - lb * a.block_size) * a.k_ss;
+    auto fetch = [&](int n, int page) __attribute__((always_inline)) {
+        const int key = key_of(n);
+        const int8_t* row = gbase + (int64_t)page * a.k_sb + (int64_t)(key - slot_of(key) * a.block_size) * a.k_ss;
         Block x;
 #pragma unroll
         for (int c = 0; c < 4; ++c) __builtin_memcpy(&x.k[c], __builtin_assume_aligned(row + 64 * c + 16 * lg, 8), 16);
         x.ks = *reinterpret_cast<const float*>(row + kDim);
         return x;
     };
-    Block cur = fetch(first);
+    const int page0 = page_of(first), page1 = page_of(first + stride);
+    int page2 = page_of(first + 2 * stride);
+
+    // ---- Q^T: lane (lg, li) holds row 16 rb + li, dims 64 (st / 2) + 16 lg + 8 (st % 2) + [0, 8) ----
+    half8_t qop[NRB][8];
+    float nlse[NRB];  // -lse in log2 units; -inf for a row that counts for nothing
+    int rpos[NRB];
+    bool valid[NRB];
+#pragma unroll
+    for (int rb = 0; rb < NRB; ++rb) {
+        const int r = 16 * rb + li;
+        valid[rb] = r < R;
+        const int qi = valid[rb] ? r / G : 0, qh = valid[rb] ? r - qi * G : 0;
+        const _Float16* qrow = a.q + (int64_t)(q0 + qi) * a.q_st + (int64_t)(g * G + qh) * kDim;
+#pragma unroll
+        for (int st = 0; st < 8; ++st)
+            __builtin_memcpy(&qop[rb][st], __builtin_assume_aligned(qrow + 64 * (st >> 1) + 16 * lg + 8 * (st & 1), 4), 16);
+        nlse[rb] = a.lse[(int64_t)(q0 + qi) * a.Hq + g * G + qh];
+        rpos[rb] = valid[rb] ? ctx0 + qi : -1;
+    }
+    Block cur = fetch(first, page0), next = cur;
+    if (first + stride < nblk) next = fetch(first + stride, page1);
+#pragma unroll
+    for (int rb = 0; rb < NRB; ++rb) {
+#pragma unroll
+        for (int st = 0; st < 8; ++st) qop[rb][st] = valid[rb] ? qop[rb][st] : (half8_t)(_Float16)0.0f;
+        // a row whose sum was 0 (lse -inf) weighs nothing, and neither does a row past the last
+        nlse[rb] = valid[rb] && nlse[rb] != kNegInf ? -nlse[rb] * 1.4426950408889634f : kNegInf;
+    }
     for (int n = first; n < nblk; n += stride) {
-        Block next;
-        if (n + stride < nblk) next = fetch(n + stride);
+        Block later = next;
+        if (n + 2 * stride < nblk) later = fetch(n + 2 * stride, page2);
+        page2 = page_of(n + 3 * stride);
         float4_t s[NRB];
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
@@ -111,6 +121,7 @@ __global__ void __launch_bounds__(64 * kKwWaves) pd_key_weights_kernel(const Key
         const float mine = li == 0 ? sum[0] : li == 1 ? sum[1] : li == 2 ? sum[2] : sum[3];
         if (li < 4 && key0 + li < min(seq_len, a.max_keys)) wrow[key0 + li] += mine;
         cur = next;
+        next = later;
     }
 }
 
@@ -121,7 +132,8 @@ hipError_t launch_key_weights(const KeyWeightsParams& p, int num_seqs, int heads
     const int rows = p.qmax * p.G, nrb = (rows + 15) / 16;
     const int known = compute_units(stream);
     const int64_t cus = known > 0 ? known : 256;
-    int64_t splits = 4 * cus / ((int64_t)num_seqs * heads_kv);
+    // as many workgroups as run at once: 4, 3 or 2 per CU by the registers of 1 to 3 row blocks
+    int64_t splits = (5 - nrb) * cus / ((int64_t)num_seqs * heads_kv);
     const int64_t most = (p.table_keys + kKwKeys * kKwWaves - 1) / (kKwKeys * kKwWaves);
     splits = splits < 1 ? 1 : splits;
     if (most >= 1 && splits > most) splits = most;
