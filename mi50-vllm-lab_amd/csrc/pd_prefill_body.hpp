@@ -82,8 +82,7 @@ struct FaWork {
     int part;                  // segment of the partials (kParts 1: split; 2: slot, or -1 for the output itself)
 };
 
-// kParts: 0 the rows are finished and stored; 1 partials of split wk.part; 2 either, as wk.part says; 3 partials
-// in segment wk.part of the decode's buffers (a.nsplit segments per row), in its units.
+// kParts: 0 the rows are finished and stored; 1 partials of split wk.part; 2 either, as wk.part says.
 template <bool kFast, bool kExact, int kParts, class T>
 __device__ __forceinline__ void prefill_body(const FaParams& a, const FaWork& wk, unsigned char* lds) {
     constexpr int kLdsRaw = 0, kLdsH = kFaLdsH, kLdsBt = kFaLdsBt;
@@ -94,10 +93,10 @@ __device__ __forceinline__ void prefill_body(const FaParams& a, const FaWork& wk
     // a multiply and a conversion for P'.
     constexpr bool kPinned = !kExact && kParts == 0;
     // K and V carry the widening bias (see the head of the file), whose rounding grows with the run of key tiles
-    // that one accumulator sums. The dealt instances' runs are as long as the deal makes them, so they widen exactly:
+    // that one accumulator sums. The dealt instance's runs are as long as the deal makes them, so it widens exactly:
     // error of four chunks of 70 to 900 tokens over 1,500 to 6,000 keys 4.4e-4 -> 2.9e-4 of the result (302 us
     // with 9 decoded sequences, 297 biased), of chunks over 30,000 to 60,000 keys on 10 workgroups 5.2e-3 -> 2.9e-4.
-    constexpr bool kBias = !kExact && kParts < 2;
+    constexpr bool kBias = !kExact && kParts != 2;
     const int b = wk.b, g = wk.g, tq0 = wk.tq0, ntok = wk.ntok, seq_len = wk.seq_len, qabs = wk.qabs;
     const int t0 = wk.t0, t1 = wk.t1;
     const int tid = threadIdx.x, l = tid & 63, lg = l >> 4, li = l & 15;
@@ -558,10 +557,9 @@ __device__ __forceinline__ void prefill_body(const FaParams& a, const FaWork& wk
         if (rvalid[rb]) {
             const int r = 48 * w + 16 * rb + li;
             const int tok = r / G, hh = r - (r / G) * G;
-            if (kParts == 1 || kParts == 3 || (kParts == 2 && wk.part >= 0)) {
-                const int64_t pr = kParts == 1   ? (((int64_t)b * a.Sq + tq0 + tok) * a.Hq + g * G + hh) * a.nsplit + wk.part
-                                   : kParts == 3 ? ((int64_t)(tq0 + tok) * a.Hq + g * G + hh) * a.nsplit + wk.part
-                                                 : (int64_t)wk.part * kFaRows + r;
+            if (kParts == 1 || (kParts == 2 && wk.part >= 0)) {
+                const int64_t pr = kParts == 1 ? (((int64_t)b * a.Sq + tq0 + tok) * a.Hq + g * G + hh) * a.nsplit + wk.part
+                                               : (int64_t)wk.part * kFaRows + r;
                 float* prow = a.part_o + pr * kDim;
 #pragma unroll
                 for (int m = 0; m < 17; ++m) {
@@ -569,8 +567,7 @@ __device__ __forceinline__ void prefill_body(const FaParams& a, const FaWork& wk
                     if (d0 >= 0 && d0 < kDim) *reinterpret_cast<float4_t*>(prow + d0) = oacc[rb][m] - corr;
                 }
                 if (lg == 0) {
-                    // (O and l carry 2^kPLog2, which the decode's segments do not)
-                    a.part_m[pr] = kParts == 3 ? m_run[rb] - kPLog2 : m_run[rb];
+                    a.part_m[pr] = m_run[rb];
                     a.part_l[pr] = l_row;
                 }
             } else {

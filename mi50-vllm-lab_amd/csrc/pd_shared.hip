@@ -6,43 +6,47 @@
 // pieces of the prefix, the others deal the own key tiles of all (sequence, kv head) among them as pd_balanced_kernel does.
 // wp and the number of pieces are worked out on the device from the lengths (every workgroup, the same numbers), by rating
 // each number of pieces: one lane, one number.
-//   prefix   up to 32 rows of a kv head (tokens of the batch x its query heads) are one group of the decode's workgroup
-//            (pd_partial.hpp) over a sequence made of the whole batch; more are tiles of 192 rows in the
-//            prefill's (pd_prefill_body.hpp), where all of the workgroup's waves share one widening of each tile. A piece
-//            is a run of the prefix's key tiles; it fills one segment of its rows.
-//   own      the decode's workgroup over keys [prefix, seq_len) of one sequence; segments behind the prefix's. More than 32
-//            rows of a sequence and kv head are two slices, which read the keys twice (three row blocks do not fit the
-//            registers beside the deal).
-// Segments of a row: [0, ns) the prefix's pieces, [ns, ..) the own ones, the rest up to the last marked empty; the last one's
-// place holds ns, which the join needs: a sequence that does not hold the prefix and its query tokens behind it
-// (seq_len - q_len < prefix) takes all of its keys as its own and leaves the prefix's segments out.
+//   prefix   tiles of up to 128 or 256 (token of the batch, query head of a kv head) rows. A piece is a run of the prefix's key
+//            tiles; it fills one segment of its rows.
+//   own      the rows of one sequence and kv head over its keys [prefix, seq_len); segments behind the prefix's.
+// Both in the same workgroup form (pd_shared_body.hpp).
+// Segments of a row: [0, ns) the prefix's pieces, [ns, ns + n) the own ones; the last one's place holds both numbers, a note that
+// spares marking the others empty and tells the join which to leave out: a sequence that does not hold the prefix and its
+// query tokens behind it (seq_len - q_len < prefix) takes all of its keys as its own.
 // The prefix's blocks are those of the first sequence that holds it.
 //
-// The 192-row tiles round P' = p v_scale once to fp16 as the default prefill does (11 bits: an error of about the final
-// fp16 rounding's size; hi + lo would double their P.V products), the decode's workgroups carry hi + lo.
-#include "pd_partial.hpp"
-#include "pd_prefill_body.hpp"
+// P' = p v_scale is rounded once to fp16 as in the default prefill (11 bits: an error of about the final fp16 rounding's
+// size; hi + lo would double the P.V products).
+//
+// What bounds it (gfx950, both launches, us; 24 / 4 heads unless said): 128 sequences of 64 to 2,048 keys behind 61,440 shared ones 233 to
+// 257, of which the prefix, bound by MFMA and the 32-bit arithmetic beside it, takes 207 alone (half of the MFMA rate of a large
+// matrix product), and the own keys 60 (4.7 TB/s: bound by memory); a CU streams at most 20 bytes a ns, so the deal counts
+// 1 us for an own tile and both kinds of work finish together. 32 sequences over 8,192: 38, 12 of them set-up of the pieces, their
+// partials (25 MB) and the join. 4 over 2,048: 13.7, five dependent trips to memory and a second launch.
+#include "pd_shared_body.hpp"
 #include "pth_dec.h"
 
 namespace pd {
 
-// Costs that the deal weighs, in 0.1 us: a workgroup's key tile and its set-up and merge.
-constexpr unsigned kShTile = 8, kShSegment = 100;        // decode workgroup
-constexpr unsigned kShWideTile = 18, kShWideSegment = 160;  // 192-row workgroup
-constexpr unsigned kShMergeRows = 190;                    // (token, head) rows whose segments cost 0.1 us to write and read again
-constexpr unsigned kShOwnUnits = 12;                      // set-up and merge of an own segment, in tiles (pd_balanced_kernel's line)
-constexpr unsigned kShSnap = 6;
+// Costs that the deal weighs, in 0.1 us, as stamps in the kernel showed them: a key tile of an own workgroup (20 bytes a ns), of a
+// prefix workgroup with one or two row blocks per wave, a prefix piece's set-up and end. The deal is flat around them: 9 to 11,
+// 12 to 13, 60 to 100 and 250 to 400 rows below change no measured batch by more than 4 % (an own tile of 4.5: 17 %).
+constexpr unsigned kShTile = 10;
+constexpr unsigned kShPrefixTile1 = 13, kShPrefixTile2 = 20;
+constexpr unsigned kShPrefixSegment = 80;
+constexpr unsigned kShMergeRows = 400;  // (token, head) rows whose segments cost 0.1 us to write and read again
+constexpr unsigned kShOwnUnits = 12;    // set-up and merge of an own segment, in tiles (pd_balanced_kernel's line)
+constexpr unsigned kShSnap = 6;         // a share's end moves to an item's that is this many units away (pd_balanced_kernel's too)
 
-// kWide: the prefix in 192-row tiles; NRB: row blocks of the decode workgroups (both parts without kWide).
-template <int NRB, bool kFast, bool kWide>
-__global__ void __launch_bounds__(kThreads, 1) pd_shared_kernel(const SharedParams sp) {
-    constexpr int kOwnLds = PartialLds<NRB, kFast>::kBytes;
-    __shared__ __attribute__((aligned(16))) unsigned char lds[kWide && kFaLdsBytes > kOwnLds ? kFaLdsBytes : kOwnLds];
+// OW: waves in rows of the own keys' workgroups (one row block each); PB: row blocks of the prefix's waves.
+template <int OW, bool kFast, int PB>
+__global__ void __launch_bounds__(kSwThreads, 1) pd_shared_kernel(const SharedParams sp) {
+    __shared__ __attribute__((aligned(16))) unsigned char lds[kSwLds];
+    constexpr int NB = 8 * PB;  // row blocks of a prefix tile
     const PartialParams& a = sp.p;
     const int lane = threadIdx.x & 63;
     const unsigned Hkv = (unsigned)(a.Hq / a.G), nwg = gridDim.x, wg = blockIdx.x;
     const int segs = a.nsplit - 1;  // and the note
-    const unsigned slices = NRB == 2 && a.qmax * a.G > 32 ? 2u : 1u, groups = Hkv * slices;  // own items of a sequence
 
     // ---- the batch: own tiles of each sequence, the first that holds the prefix ----
     auto own_lo = [&](int q_len, int len) __attribute__((always_inline)) { return len - q_len >= sp.prefix ? sp.prefix : 0; };
@@ -70,10 +74,11 @@ __global__ void __launch_bounds__(kThreads, 1) pd_shared_kernel(const SharedPara
             if (who) first_holder = c + __builtin_ctzll(who);
         }
     }
-    total *= groups;
+    total *= Hkv;
     const int T = max(0, min(sp.num_tokens, a.qsl[a.num_seqs]));
-    const int tok_tile = kWide ? kFaRows / a.G : T;                   // query tokens of a prefix item
-    const unsigned nrt = T > 0 ? (unsigned)((T + tok_tile - 1) / tok_tile) : 0u;
+    // rows of a kv head, their tiles, and the rows of a tile: equal shares in whole waves
+    const unsigned prows = (unsigned)(T * a.G), nrt = (prows + 16 * NB - 1) / (16 * NB);
+    const unsigned trows = nrt ? ((prows + nrt - 1) / nrt + 16 * PB - 1) / (16 * PB) * (16 * PB) : 0u;
     const unsigned ptiles = first_holder >= 0 && sp.prefix > 0 ? (unsigned)((sp.prefix - 1) / kTile + 1) : 0u;
     const unsigned items = ptiles ? nrt * Hkv : 0u;
 
@@ -82,8 +87,7 @@ __global__ void __launch_bounds__(kThreads, 1) pd_shared_kernel(const SharedPara
     unsigned wp = 0, ns = 0;
     if (items) {
         constexpr unsigned kLanes = 48;
-        const unsigned tile = kWide ? kShWideTile : kShTile;
-        const unsigned seg = kWide ? kShWideSegment : kShSegment;
+        constexpr unsigned tile = PB == 1 ? kShPrefixTile1 : kShPrefixTile2, seg = kShPrefixSegment;
         const unsigned rounds = (unsigned)lane < kLanes ? 1u : (unsigned)lane - kLanes + 2u;
         const unsigned pieces = rounds == 1 ? (unsigned)lane + 1u : 1u;
         const unsigned w = (items * pieces + rounds - 1) / rounds;
@@ -91,7 +95,7 @@ __global__ void __launch_bounds__(kThreads, 1) pd_shared_kernel(const SharedPara
         const bool can = w + (own ? 1u : 0u) <= nwg && pieces <= (unsigned)(segs - 2) && pieces <= ptiles;
         const unsigned prefix_us = rounds * (seg + (ptiles + pieces - 1) / pieces * tile) + (unsigned)(T * a.Hq) * pieces / kShMergeRows;
         const unsigned share = own && can ? max((total + nwg - w - 1) / (nwg - w), longest / (unsigned)(segs - (int)pieces - 1)) : 0u;
-        const unsigned own_us = share * (kShTile) * 9 / 8;
+        const unsigned own_us = share * kShTile;
         const unsigned cost = can ? min(max(prefix_us, own_us), 0x3ffffffu) : 0x3ffffffu;
         // the cheapest (the lowest lane of equal ones); more items than 17 rounds take: as many rounds as it needs
         const unsigned best = ~wave_umax(~((cost << 6) | (unsigned)lane)) & 63u;
@@ -111,68 +115,26 @@ __global__ void __launch_bounds__(kThreads, 1) pd_shared_kernel(const SharedPara
             if (x != wg) __syncthreads();  // the blocks of the piece before have been read
             const unsigned rt = x % nrt, gp = x / nrt, piece = gp % ns, g = gp / ns;
             const unsigned first = piece * ptiles / ns, last = (piece + 1) * ptiles / ns;
-            if constexpr (kWide) {
-                FaParams f = {};
-                f.q = a.q;
-                f.q_sh = kDim;
-                f.q_st = a.q_st;
-                f.kc = a.kc;
-                f.k_sb = a.k_sb;
-                f.k_ss = a.k_ss;
-                f.k_sh = a.k_sh;
-                f.block_table = a.block_table;
-                f.bt_stride = a.bt_stride;
-                f.Hq = a.Hq;
-                f.G = a.G;
-                f.tok_per_wg = tok_tile;
-                f.block_size = a.block_size;
-                f.bs_shift = a.bs_shift;
-                f.bt32 = sp.bt32;
-                f.scale_log2 = a.scale_log2;
-                f.nsplit = a.nseg;
-                f.part_o = a.part_o;
-                f.part_m = a.part_m;
-                f.part_l = a.part_l;
-                FaWork wk;
-                wk.b = first_holder;
-                wk.g = (int)g;
-                wk.tq0 = (int)rt * tok_tile;
-                wk.ntok = min(tok_tile, T - wk.tq0);
-                wk.seq_len = sp.prefix;
-                wk.qabs = 1 << 30;  // every key of the prefix is before every query token
-                wk.qrow0 = 0;
-                wk.orow0 = 0;
-                wk.t0 = (int)first;
-                wk.t1 = (int)last;
-                wk.part = (int)piece;
-                prefill_body<kFast, false, 3, _Float16>(f, wk, lds);
-            } else {
-                Work wk;
-                wk.g = (int)g;
-                wk.b = first_holder;
-                wk.row0 = 0;
-                wk.q0 = 0;
-                wk.q_len = T;
-                wk.ql = T;
-                wk.seq_len = sp.prefix;
-                wk.ctx0 = 1 << 30;
-                wk.lo = 0;
-                wk.seg = (int)piece;
-                wk.tb = (int)first;
-                wk.te = (int)last;
-                wk.t_first = 0;
-                wk.ntiles = (int)ptiles;
-                wk.W = 0;
-                wk.interleave = false;
-                partial_body<NRB, kFast, true>(a, wk, lds);
-            }
+            SharedWork wk;
+            wk.g = (int)g;
+            wk.b = first_holder;
+            wk.q0 = 0;
+            wk.pos0 = 1 << 30;  // every key of the prefix comes before every query token
+            wk.lo = 0;
+            wk.hi = sp.prefix;
+            wk.row0 = (int)(rt * trows);
+            wk.nrow = min((int)trows, (int)prows - wk.row0);
+            wk.t0 = (int)first;
+            wk.t1 = (int)last;
+            wk.seg = (int)piece;
+            shared_body<PB, 8, kFast>(sp, wk, lds);
         }
         return;
     }
 
     // ---- the own keys: pd_balanced_kernel's deal over the other workgroups ----
     if (total == 0) return;
-    const unsigned ow = wg - wp, on = nwg - wp, oitems = (unsigned)a.num_seqs * groups, cap = (unsigned)(segs - (int)ns);
+    const unsigned ow = wg - wp, on = nwg - wp, oitems = (unsigned)a.num_seqs * Hkv, cap = (unsigned)(segs - (int)ns);
     const unsigned share = max(max((total + on - 1) / on, (longest + cap - 2) / (cap - 1)), 2u);
     const unsigned nso = min(on / oitems, cap);
     const bool aligned = nso >= 1 && (longest + nso - 1) / nso <= share;
@@ -181,13 +143,13 @@ __global__ void __launch_bounds__(kThreads, 1) pd_shared_kernel(const SharedPara
     auto locate = [&](unsigned pos) __attribute__((always_inline)) {
         unsigned before = 0;
         for (int c = 0;; c += 64) {
-            const unsigned t = c == 0 ? t0 : tiles_of(c + lane);
-            const unsigned incl = c == 0 ? incl0 : wave_scan(units_of(t));
-            const int k = __popcll(__ballot(groups * (before + incl) <= pos));
+            const unsigned t = tiles_of(c + lane);
+            const unsigned incl = wave_scan(units_of(t));
+            const int k = __popcll(__ballot(Hkv * (before + incl) <= pos));
             if (k < 64) {
                 at_seq = (unsigned)(c + k);
                 at_tiles = (unsigned)__builtin_amdgcn_readlane((int)t, k);
-                at_start = groups * (before + (unsigned)__builtin_amdgcn_readlane((int)incl, k) - units_of(at_tiles));
+                at_start = Hkv * (before + (unsigned)__builtin_amdgcn_readlane((int)incl, k) - units_of(at_tiles));
                 return;
             }
             before += (unsigned)__builtin_amdgcn_readlane((int)incl, 63);
@@ -211,12 +173,12 @@ __global__ void __launch_bounds__(kThreads, 1) pd_shared_kernel(const SharedPara
     }
     while (true) {
         unsigned first, last, seg;
-        Work wk;
+        SharedWork wk;
         if (aligned) {
             const unsigned item = ow / nso;
             seg = ow - item * nso;
-            wk.b = (int)(item / groups);
-            wk.g = (int)(item - (unsigned)wk.b * groups);
+            wk.b = (int)(item / Hkv);
+            wk.g = (int)(item - (unsigned)wk.b * Hkv);
         } else {
             locate(pos);
             const unsigned units = units_of(at_tiles), g = (pos - at_start) / units, item = at_start + g * units;
@@ -228,41 +190,32 @@ __global__ void __launch_bounds__(kThreads, 1) pd_shared_kernel(const SharedPara
         }
         wk.q0 = ((const_int_ptr)(uintptr_t)a.qsl)[wk.b];
         const int q_end = ((const_int_ptr)(uintptr_t)a.qsl)[wk.b + 1];
-        wk.seq_len = ((const_int_ptr)(uintptr_t)a.seq_lens)[wk.b];
-        asm volatile("" ::"s"(wk.q0), "s"(q_end), "s"(wk.seq_len));
-        wk.q_len = q_end - wk.q0;
-        wk.lo = own_lo(wk.q_len, wk.seq_len);
-        wk.ctx0 = wk.seq_len - wk.q_len;
-        wk.ql = min(wk.q_len, a.qmax);
-        wk.t_first = wk.lo / kTile;
-        wk.ntiles = (wk.seq_len - 1) / kTile - wk.t_first + 1;
+        wk.hi = ((const_int_ptr)(uintptr_t)a.seq_lens)[wk.b];
+        asm volatile("" ::"s"(wk.q0), "s"(q_end), "s"(wk.hi));
+        const int q_len = q_end - wk.q0;
+        wk.lo = own_lo(q_len, wk.hi);
+        wk.pos0 = wk.hi - q_len;
+        wk.row0 = 0;
+        wk.nrow = min(q_len, a.qmax) * a.G;
+        const int t_first = wk.lo / kTile;
+        const unsigned ntiles = (unsigned)((wk.hi - 1) / kTile - t_first + 1);
         if (aligned) {
-            if (wk.q_len <= 0 || wk.seq_len <= 0) return;
-            const unsigned per = ((unsigned)wk.ntiles + nso - 1) / nso;
+            if (q_len <= 0 || wk.hi <= 0) return;
+            const unsigned per = (ntiles + nso - 1) / nso;
             first = seg * per;
-            last = min((unsigned)wk.ntiles, first + per);
+            last = min(ntiles, first + per);
             if (first >= last) return;
         }
-        wk.row0 = slices > 1 ? 32 * (wk.g & 1) : 0;
-        wk.g = slices > 1 ? wk.g >> 1 : wk.g;
         wk.seg = (int)(ns + seg);
-        wk.tb = wk.t_first + (int)first;
-        wk.te = wk.t_first + (int)last;
-        wk.W = 0;
-        wk.interleave = false;
-        const int R = min(16 * NRB, wk.ql * a.G - wk.row0);
-        if (R > 0) partial_body<NRB, kFast, true>(a, wk, lds);  // (a slice past the sequence's rows has none)
-        if (last == (unsigned)wk.ntiles) {  // the item's last workgroup: no other segments, and the note
-            const int spare = segs - wk.seg;
-            for (int k = threadIdx.x; k < R * spare; k += kThreads) {
-                const int r = k / spare, i = (wk.row0 + r) / a.G, hh = wk.row0 + r - i * a.G, s = wk.seg + 1 + (k - r * spare);
-                const int64_t pr = ((int64_t)(wk.q0 + i) * a.Hq + (wk.g * a.G + hh)) * a.nseg + s;
-                a.part_m[pr] = s == segs ? __builtin_bit_cast(float, ns) : kNegInf;
-                a.part_l[pr] = 0.f;
-            }
+        wk.t0 = t_first + (int)first;
+        wk.t1 = t_first + (int)last;
+        shared_body<1, OW, kFast>(sp, wk, lds);
+        if (last == ntiles && (int)threadIdx.x < wk.nrow) {  // the item's last workgroup knows how many there are: the note
+            const int r = (int)threadIdx.x, i = r / a.G, hh = r - i * a.G;
+            a.part_m[((int64_t)(wk.q0 + i) * a.Hq + (wk.g * a.G + hh)) * a.nseg + segs] = __builtin_bit_cast(float, ns | (ns + seg + 1) << 8);
         }
-        if (aligned || last < (unsigned)wk.ntiles) return;
-        pos = (first ? pos - first - kShOwnUnits : pos) + units_of((unsigned)wk.ntiles);
+        if (aligned || last < ntiles) return;
+        pos = (first ? pos - first - kShOwnUnits : pos) + units_of(ntiles);
         if (pos >= end) return;
         __syncthreads();
     }
@@ -292,9 +245,9 @@ __global__ void __launch_bounds__(256) pd_shared_combine_kernel(const SharedPara
     const int q_b = ((const_int_ptr)(uintptr_t)a.qsl)[bq], q_end = ((const_int_ptr)(uintptr_t)a.qsl)[bq + 1];
     const int len = ((const_int_ptr)(uintptr_t)a.seq_lens)[bq];
     if (!(b < a.num_seqs && tok >= q_b && len > 0 && tok - q_b < a.qmax)) return;  // (uniform over the row's waves)
-    const int ns = __builtin_amdgcn_readlane(__builtin_bit_cast(int, m_ld), segs);
-    const int from = len - (q_end - q_b) >= sp.prefix ? 0 : ns;
-    const bool live = lane >= from && lane < segs && m_ld != kNegInf;
+    const int note = __builtin_amdgcn_readlane(__builtin_bit_cast(int, m_ld), segs);
+    const int from = len - (q_end - q_b) >= sp.prefix ? 0 : note & 0xff;
+    const bool live = lane >= from && lane < note >> 8 && m_ld != kNegInf;
     uint64_t mask = __ballot(live);
     float M = live ? m_ld : kNegInf;
 #pragma unroll
@@ -338,12 +291,19 @@ __global__ void __launch_bounds__(256) pd_shared_combine_kernel(const SharedPara
 // ---------------------------------------------------------------------------------------
 // host side
 
-template <bool kFast, bool kWide>
+template <bool kFast, int PB>
 static void launch_shared_rows(const SharedParams& s, int rows, int wgs, hipStream_t stream) {
     if (rows <= 16)
-        hipLaunchKernelGGL((pd_shared_kernel<1, kFast, kWide>), dim3(wgs), dim3(kThreads), 0, stream, s);
+        hipLaunchKernelGGL((pd_shared_kernel<1, kFast, PB>), dim3(wgs), dim3(kSwThreads), 0, stream, s);
     else
-        hipLaunchKernelGGL((pd_shared_kernel<2, kFast, kWide>), dim3(wgs), dim3(kThreads), 0, stream, s);
+        hipLaunchKernelGGL((pd_shared_kernel<4, kFast, PB>), dim3(wgs), dim3(kSwThreads), 0, stream, s);
+}
+
+// Whether the prefix's waves take two row blocks, for `rows` rows of a kv head. A tile of 128 rows costs 1.25 us with one, of 256 1.95
+// with two, and a wave that has no row no time: 24 rows over 2,048 keys 13.5 us with one and 14.7 with two, 126 over 1,111 20.0 and
+// 20.9; 192 over 8,192 37.8 and 38.7, over 61,440 107 and 94; 384 over 15,840 51 and 47; 768 over 61,440 330 and 240.
+static bool two_row_blocks(int64_t rows) {
+    return rows > 128;
 }
 
 hipError_t launch_shared(const LaunchArgs& x, int prefix, int bt32, hipStream_t stream) {
@@ -382,12 +342,10 @@ hipError_t launch_shared(const LaunchArgs& x, int prefix, int bt32, hipStream_t 
     s.lse = x.lse;
     const int known = compute_units(stream), cus = known > 1 ? known : 256;
     const bool fast = fast_block_table(x.block_size, x.k_ss);
-    const int64_t all = (int64_t)x.num_tokens * p.G;  // rows of a kv head
-    const int own = x.qmax * p.G;
-    if (all <= 32)
-        fast ? launch_shared_rows<true, false>(s, (int)all, cus, stream) : launch_shared_rows<false, false>(s, (int)all, cus, stream);
-    else
-        fast ? launch_shared_rows<true, true>(s, own, cus, stream) : launch_shared_rows<false, true>(s, own, cus, stream);
+    const int rows_own = x.qmax * p.G;
+    const bool two = fast && two_row_blocks((int64_t)x.num_tokens * p.G);
+    two ? launch_shared_rows<true, 2>(s, rows_own, cus, stream)
+        : fast ? launch_shared_rows<true, 1>(s, rows_own, cus, stream) : launch_shared_rows<false, 1>(s, rows_own, cus, stream);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
     const int64_t rows = (int64_t)x.num_tokens * x.heads_q;

@@ -1,12 +1,12 @@
 """decode_shared on the GPU against float64: batches from 1 to 300 sequences, prefixes of 0, 1, 31 to 33 keys to thousands, ends
-inside blocks, own parts of the query tokens alone to long ones, every kernel form (64-, 128- and 256-row tiles of the prefix; one
-and two row blocks, two slices; 16-key row blocks or not), GQA groups of 1 to 48, both layouts, 4 to 128 segments,
+inside blocks, own parts of the query tokens alone to long ones, every kernel form (one and two row blocks of the prefix's
+waves; own rows of one wave and of four; 16-key row blocks or not), GQA groups of 1 to 48, both layouts, 4 to 128 segments,
 sequences that do not hold the prefix, padded sequences and tokens, NaN in masked places, outlier rows, strided
 tensors; the rows' logarithms; streams and a captured graph; and a decode step through all of the operators.
 
 Bounds. Scores in fp32 are off by U (256 A + 4 |s| + 8), U = 2^-24, A = sum_d |q_d k_d| scaled (256 partial sums), which is a relative
-error of each weight, of the sum of weights as well. P' = p v_scale of a shared key is rounded once to fp16: half a step, 2^-11 of it,
-below 2^-14 / 16 half a subnormal step (an own key's is hi + lo: 2^-21). The weighted sums of n keys add (n / 16 + 100) U of sum p |v|. With W = sum p |v| / sum p
+error of each weight, of the sum of weights as well. P' = p v_scale is rounded once to fp16: half a step, 2^-11 of it,
+below 2^-14 / 16 half a subnormal step. The weighted sums of n keys add (n / 16 + 100) U of sum p |v|. With W = sum p |v| / sum p
 an output is off by (2^-11 + 2 e + ..) W, and by half an fp16 step at the end.
 """
 import numpy as np
@@ -64,12 +64,12 @@ def reference(case, prefix):
             tot = p.sum(-1, keepdims=True)
             val = v * vs[:, None]
             e = U * (256 * a.max(-1) + 8 * np.abs(np.where(see, s, 0)).max(-1) + 8)[:, None]
-            w, shared = (p / tot) @ np.abs(val), (p / tot)[:, :prefix] @ np.abs(val[:prefix])
+            w = (p / tot) @ np.abs(val)
             o = (p / tot) @ val
             n = (seq / 16 + 100) * U
             # P' is formed as 16 p v_scale: below 2^-14 its half step is 2^-25
             small = 2.0 ** -25 / 16 * np.abs(v).sum(0)[None] / tot
-            err = 2.0 ** -11 * shared + (2.0 ** -21 + 2 * e + 2 * n) * w + small
+            err = (2.0 ** -11 + 2 * e + 2 * n) * w + small
             rows = (slice(at, at + ql), slice(h * g, (h + 1) * g))
             out[rows], tol[rows] = (x.reshape(ql, g, 256) for x in (o, err))
             lse[rows] = (m + np.log(tot))[:, 0].reshape(ql, g)

@@ -16,18 +16,18 @@ def const(name):
     return int(re.search(r"\b%s = (\d+)[;,]" % name, SRC).group(1))
 
 
-TILE, SEG, WTILE, WSEG, MERGE, OWN, SNAP = (const("kSh" + n) for n in (
-    "Tile", "Segment", "WideTile", "WideSegment", "MergeRows", "OwnUnits", "Snap"))
+TILE, PTILE1, PTILE2, PSEG, MERGE, OWN, SNAP = (const("kSh" + n) for n in (
+    "Tile", "PrefixTile1", "PrefixTile2", "PrefixSegment", "MergeRows", "OwnUnits", "Snap"))
 BIG = 0x3ffffff
 
 
-def plan(own, tokens, ptiles, hkv, hq, slices, nwg, nseg, wide):
-    """(workgroups of the prefix, pieces, row tiles): own: own key tiles of each sequence (0: no work)."""
+def plan(own, tokens, ptiles, hkv, hq, nwg, nseg, blocks):
+    """(workgroups of the prefix, pieces, row tiles): own: own key tiles of each sequence (0: no work); blocks: row blocks
+    of a prefix wave."""
     segs = min(nseg, 64) - 1
-    total = hkv * slices * sum(t + OWN if t else 0 for t in own)
+    total = hkv * sum(t + OWN if t else 0 for t in own)
     longest = max(own)
-    tok = 192 // (hq // hkv) if wide else tokens
-    nrt = -(-tokens // tok) if tokens > 0 else 0
+    nrt = -(-tokens * (hq // hkv) // (128 * blocks))
     items = nrt * hkv if ptiles else 0
     if not items:
         return 0, 0, nrt
@@ -39,9 +39,9 @@ def plan(own, tokens, ptiles, hkv, hq, slices, nwg, nseg, wide):
         if not (w + (total > 0) <= nwg and pieces <= segs - 2 and pieces <= ptiles):
             costs.append((BIG, lane, pieces, w))
             continue
-        us = rounds * ((WSEG if wide else SEG) + -(-ptiles // pieces) * (WTILE if wide else TILE)) + tokens * hq * pieces // MERGE
+        us = rounds * (PSEG + -(-ptiles // pieces) * (PTILE1 if blocks == 1 else PTILE2)) + tokens * hq * pieces // MERGE
         share = max(-(-total // (nwg - w)), longest // (segs - pieces - 1)) if total else 0
-        costs.append((min(max(us, share * TILE * 9 // 8), BIG), lane, pieces, w))
+        costs.append((min(max(us, share * TILE), BIG), lane, pieces, w))
     cost, _, pieces, w = min(costs)
     if cost == BIG:
         wp = max(1, nwg - nwg // 8) if total else nwg
@@ -109,8 +109,10 @@ def test_every_tile_once(seed):
         if not tokens:
             continue
         ptiles = r.choice([0, 1, r.randint(1, 60), r.randint(1, 4000)])
-        wide, slices = tokens * g > 32, 2 if qmax * g > 32 else 1
-        wp, ns, nrt = plan(tiles, tokens, ptiles, hkv, hkv * g, slices, nwg, nseg, wide)
+        blocks, rows = 1 + (tokens * g > 128), tokens * g
+        wp, ns, nrt = plan(tiles, tokens, ptiles, hkv, hkv * g, nwg, nseg, blocks)
+        share = -(-(-(-rows // nrt)) // (16 * blocks)) * 16 * blocks     # rows of a tile
+        assert share <= 128 * blocks and (nrt - 1) * share < rows <= nrt * share
         segs = min(nseg, 64) - 1
         assert 0 <= wp < nwg and ns <= segs - 2 and (ns >= 1) == (wp >= 1) == (ptiles > 0)
         seen = set()
@@ -123,9 +125,9 @@ def test_every_tile_once(seed):
                 seen.add((rt, head, piece))
         assert len(seen) == nrt * hkv * ns
         cap = segs - ns
-        got = own_deal(tiles, hkv * slices, nwg - wp, cap)
+        got = own_deal(tiles, hkv, nwg - wp, cap)
         for b, t in enumerate(tiles):
-            for head in range(hkv * slices):
+            for head in range(hkv):
                 pieces = sorted(got.get((b, head), []))
                 if not t:
                     assert not pieces
@@ -136,7 +138,7 @@ def test_every_tile_once(seed):
 
 
 def test_more_items_than_workgroups_run_in_rounds():
-    wp, ns, nrt = plan([4] * 512, 2048, 100, 4, 24, 1, 40, 64, True)
+    wp, ns, nrt = plan([4] * 512, 2048, 100, 4, 24, 40, 64, 2)
     assert ns == 1 and wp < 40 and nrt * 4 > 40
-    wp, ns, nrt = plan([4] * 4096, 16384, 100, 4, 24, 1, 40, 64, True)     # more than 17 rounds
+    wp, ns, nrt = plan([4] * 4096, 16384, 100, 4, 24, 40, 64, 2)     # more than 17 rounds
     assert ns == 1 and 1 <= wp < 40
