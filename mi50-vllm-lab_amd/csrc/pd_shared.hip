@@ -141,6 +141,9 @@ __global__ void __launch_bounds__(kSwThreads, 1) pd_shared_kernel(const SharedPa
     const unsigned snap = min(kShSnap, share / 8), lead = kShOwnUnits + snap;
     unsigned at_seq, at_start, at_tiles;
     auto locate = [&](unsigned pos) __attribute__((always_inline)) {
+        int lane = threadIdx.x;
+        asm volatile("" : "+v"(lane));  // (keeps the compiler from holding addresses in registers through the workgroups' bodies)
+        lane &= 63;
         unsigned before = 0;
         for (int c = 0;; c += 64) {
             const unsigned t = tiles_of(c + lane);

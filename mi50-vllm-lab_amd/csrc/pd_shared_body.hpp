@@ -142,6 +142,10 @@ __device__ __forceinline__ void shared_body(const SharedParams& sp, const Shared
     const int sro = kSwImgS + 16 * lg;  // k_scale of keys 4 lg + j of key block 0; block 1 64, v_scale 128 bytes on
 
     float4_t s[2][RB];
+    auto max8 = [&](int j) __attribute__((always_inline)) {
+        return fmaxf(fmaxf(fmaxf(s[0][j][0], s[0][j][1]), fmaxf(s[0][j][2], s[0][j][3])),
+                     fmaxf(fmaxf(s[1][j][0], s[1][j][1]), fmaxf(s[1][j][2], s[1][j][3])));
+    };
     // S: the tile's slot; F (RW = 8): this lane's place in its fragments
     auto scores = [&](int kb, const lds_u8* S, const lds_u8* F, const uint4_t* kc) __attribute__((always_inline)) {
         if constexpr (RW == 8) {
@@ -189,8 +193,9 @@ __device__ __forceinline__ void shared_body(const SharedParams& sp, const Shared
             }
         }
         if (kb < wk.lo || kb + kTile > min(hi, wk.pos0 + 1)) {  // some row does not see all of the tile
-            int lim[RB], lr = l;  // last key that the row sees
+            int lim[RB], lr = threadIdx.x;  // last key that the row sees
             asm volatile("" : "+v"(lr));
+            const int lg = lr >> 4 & 3;
 #pragma unroll
             for (int j = 0; j < RB; ++j) {
                 int tok, hd;
@@ -210,8 +215,7 @@ __device__ __forceinline__ void shared_body(const SharedParams& sp, const Shared
         bool need = false;
 #pragma unroll
         for (int j = 0; j < RB; ++j) {
-            mloc[j] = fmaxf(fmaxf(fmaxf(s[0][j][0], s[0][j][1]), fmaxf(s[0][j][2], s[0][j][3])),
-                            fmaxf(fmaxf(s[1][j][0], s[1][j][1]), fmaxf(s[1][j][2], s[1][j][3])));
+            mloc[j] = max8(j);
             need |= mloc[j] > thr_run[j];
         }
         if (__builtin_amdgcn_ballot_w64(need) != 0) {  // rare: raise the running max of the rows that need it
@@ -237,7 +241,10 @@ __device__ __forceinline__ void shared_body(const SharedParams& sp, const Shared
     auto value_scales = [&](int kb, const lds_u8* S, float4_t (&vs)[2]) __attribute__((always_inline)) {
 #pragma unroll
         for (int u = 0; u < 2; ++u) vs[u] = *(const lds_float4*)(S + sro + 64 * u + 128);
-        if (kb < wk.lo || kb + kTile > hi)  // a scale outside may be garbage, even NaN
+        if (kb < wk.lo || kb + kTile > hi) {  // a scale outside may be garbage, even NaN
+            int lr = threadIdx.x;
+            asm volatile("" : "+v"(lr));
+            const int lg = lr >> 4 & 3;
 #pragma unroll
             for (int u = 0; u < 2; ++u)
 #pragma unroll
@@ -245,40 +252,88 @@ __device__ __forceinline__ void shared_body(const SharedParams& sp, const Shared
                     const int t = kb + 16 * u + 4 * lg + i;
                     vs[u][i] = t >= wk.lo && t < hi ? vs[u][i] : 0.f;
                 }
+        }
     };
-    // ---- p' = 2^s, P' = p' * v_scale in fp16; O += V^T P'^T ----
-    auto values = [&](const float4_t (&vs)[2], const lds_u8* S, const lds_u8* F) __attribute__((always_inline)) {
-        half8_t pf[RB];
+    // ---- p' = 2^s, P' = p' * v_scale in fp16, hi and what hi leaves in lo; O += V^T P'^T ----
+    auto weights = [&](int j, float (&p)[8]) __attribute__((always_inline)) {
 #pragma unroll
-        for (int j = 0; j < RB; ++j) {
-            float p[8];
+        for (int i = 0; i < 8; ++i) p[i] = __builtin_amdgcn_exp2f(s[i >> 2][j][i & 3]);
+    };
+    auto split = [&](const float (&p)[8], const float4_t (&vs)[2], half8_t& hi8, half8_t& lo8) __attribute__((always_inline)) {
+        half2_t x[4], y[4];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) p[i] = __builtin_amdgcn_exp2f(s[i >> 2][j][i & 3]);
-            l_run[j] += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
-            half2_t x[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-                x[i] = __builtin_convertvector((float2_t){p[2 * i] * vs[i >> 1][2 * (i & 1)], p[2 * i + 1] * vs[i >> 1][2 * (i & 1) + 1]}, half2_t);
-            __builtin_memcpy(&pf[j], x, 16);
+        for (int i = 0; i < 4; ++i) {
+            const float a0 = p[2 * i] * vs[i >> 1][2 * (i & 1)], a1 = p[2 * i + 1] * vs[i >> 1][2 * (i & 1) + 1];
+            x[i] = __builtin_convertvector((float2_t){a0, a1}, half2_t);
+            y[i] = __builtin_convertvector((float2_t){a0 - (float)x[i].x, a1 - (float)x[i].y}, half2_t);
         }
-        half8_t vb[4];
-        if constexpr (RW == 8) {
-#pragma unroll
-            for (int m = 0; m < 3; ++m) vb[m] = *(const lds_half8*)(F + (16 + m) * 1024);
-        }
-#pragma unroll
-        for (int m = 0; m < 16; ++m) {
-            half8_t vf;
+        __builtin_memcpy(&hi8, x, 16);
+        __builtin_memcpy(&lo8, y, 16);
+    };
+    auto sum8 = [](const float (&p)[8]) __attribute__((always_inline)) { return ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7])); };
+    // (vs: with one row block)
+    auto values = [&](int kb, const float4_t (&vs)[2], const lds_u8* S, const lds_u8* F) __attribute__((always_inline)) {
+        half8_t pf[RB], pl[RB];
+        // O += V^T times each of the terms
+        auto products = [&](auto both) __attribute__((always_inline)) {
+            constexpr int kAhead = 3;
+            half8_t vb[kAhead + 1];
             if constexpr (RW == 8) {
-                if (m < 13) vb[(m + 3) & 3] = *(const lds_half8*)(F + (16 + m + 3) * 1024);
-                __builtin_amdgcn_sched_barrier(0);
-                vf = vb[m & 3];
-            } else {
-                const int2_t vr = __builtin_amdgcn_ds_read_tr8_b64_v2i32((lds_int2*)(S + vro[m >> 3] + 16 * m));
-                vf = widen_i8x8_exact((unsigned)vr.x, (unsigned)vr.y);
+#pragma unroll
+                for (int m = 0; m < kAhead; ++m) vb[m] = *(const lds_half8*)(F + (16 + m) * 1024);
             }
 #pragma unroll
-            for (int j = 0; j < RB; ++j) oacc[m][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, pf[j], oacc[m][j], 0, 0, 0);
+            for (int m = 0; m < 16; ++m) {
+                half8_t vf;
+                if constexpr (RW == 8) {
+                    if (m + kAhead < 16) vb[(m + kAhead) % (kAhead + 1)] = *(const lds_half8*)(F + (16 + m + kAhead) * 1024);
+                    __builtin_amdgcn_sched_barrier(0);
+                    vf = vb[m % (kAhead + 1)];
+                } else {
+                    const int2_t vr = __builtin_amdgcn_ds_read_tr8_b64_v2i32((lds_int2*)(S + vro[m >> 3] + 16 * m));
+                    vf = widen_i8x8_exact((unsigned)vr.x, (unsigned)vr.y);
+                }
+#pragma unroll
+                for (int j = 0; j < RB; ++j) {
+                    oacc[m][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, pf[j], oacc[m][j], 0, 0, 0);
+                    if constexpr (decltype(both)::value) oacc[m][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, pl[j], oacc[m][j], 0, 0, 0);
+                }
+            }
+        };
+        if constexpr (RB == 1) {
+            float p[8];
+            weights(0, p);
+            l_run[0] += sum8(p);
+            split(p, vs, pf[0], pl[0]);
+            products(std::true_type{});
+        } else {
+            // A pass for hi and, where some key is heavy, one for lo (in a loop: registers are short). Heavy: a weight above
+            // the lane's sum before, which is about a quarter of the row's.
+            bool heavy = false;
+#pragma unroll
+            for (int j = 0; j < RB; ++j) heavy |= __builtin_amdgcn_exp2f(max8(j)) > l_run[j];
+            int passes = __builtin_amdgcn_ballot_w64(heavy) != 0 ? 2 : 1;
+            float4_t vp[2];
+            value_scales(kb, S, vp);
+#pragma unroll
+            for (int j = 0; j < RB; ++j) {
+                float p[8];
+                weights(j, p);
+                l_run[j] += sum8(p);
+                if (passes == 2) {
+                    split(p, vp, pf[j], pl[j]);
+                } else {
+                    half8_t unused;
+                    split(p, vp, pf[j], unused);
+                }
+            }
+#pragma unroll 1
+            while (true) {
+                products(std::false_type{});
+                if (--passes == 0) break;
+#pragma unroll
+                for (int j = 0; j < RB; ++j) pf[j] = pl[j];
+            }
         }
     };
 
@@ -313,8 +368,9 @@ __device__ __forceinline__ void shared_body(const SharedParams& sp, const Shared
         unsigned kvo, vvo;
         int sco, lc;
         auto locate = [&](int n) __attribute__((always_inline)) {
-            lc = l;
+            lc = threadIdx.x;
             asm volatile("" : "+v"(lc));
+            lc &= 63;
             const int lg = lc >> 4, li = lc & 15;
             kvo = (unsigned)(kFast ? (lg + 4 * r) * a.k_ss : 0) + 16u * (unsigned)(li ^ (4 * lg));
             vvo = (unsigned)(kFast ? (4 * lg + r) * a.k_ss : 0) + 260u + 16u * (unsigned)(li ^ (8 * (lg & 1)));
@@ -372,8 +428,9 @@ __device__ __forceinline__ void shared_body(const SharedParams& sp, const Shared
             };
             // This wave's share of a tile's conversion: steps 2 c, 2 c + 1 of key block u and dim blocks 2 w, 2 w + 1
             const int u = w & 1, c = w >> 1;
-            const int ko = kImgK + (4 * u + (li >> 2)) * kBlk + 256 * (l & 3) + 64 * (c ^ (l & 3)) + 16 * lg;
-            const int vo = vro[0] + 32 * w - (w >= 4 && (lg & 1) ? 256 : 0);
+            int ko = kImgK + (4 * u + (li >> 2)) * kBlk + 256 * (l & 3) + 64 * (c ^ (l & 3)) + 16 * lg;
+            int vo = vro[0] + 32 * w - (w >= 4 && (lg & 1) ? 256 : 0);
+            asm volatile("" : "+v"(ko), "+v"(vo));  // (or it keeps their terms)
             lds_u8* const fr = L + kSwWide * kSwSlot + 16 * l;
             auto convert = [&](int n, const lds_u8* S) __attribute__((always_inline)) {
                 lds_u8* F = fr + (n & 1) * kSwFrag;
@@ -418,8 +475,8 @@ __device__ __forceinline__ void shared_body(const SharedParams& sp, const Shared
                     const lds_u8* F = fr + (n & 1) * kSwFrag;
                     float4_t vs[2];
                     scores(kb, S0, F, nullptr);
-                    value_scales(kb, S0, vs);
-                    values(vs, S0, F);
+                    if constexpr (RB == 1) value_scales(kb, S0, vs);
+                    values(kb, vs, S0, F);
                 }
                 if (w >= 4) prepare();
                 S0 = S1;
@@ -453,7 +510,7 @@ __device__ __forceinline__ void shared_body(const SharedParams& sp, const Shared
                     float4_t vs[2];
                     scores(kb, S, nullptr, nullptr);
                     value_scales(kb, S, vs);
-                    values(vs, S, nullptr);
+                    values(kb, vs, S, nullptr);
                 }
                 S += kSwSlot;
                 if (--left == 0) {
@@ -493,7 +550,7 @@ __device__ __forceinline__ void shared_body(const SharedParams& sp, const Shared
                 float4_t vs[2];
                 scores(kb, S, nullptr, kc);
                 value_scales(kb, S, vs);
-                values(vs, S, nullptr);
+                values(kb, vs, S, nullptr);
                 wait_lds();  // the slot has been read
             }
         }
@@ -546,8 +603,9 @@ __device__ __forceinline__ void shared_body(const SharedParams& sp, const Shared
     }
 
     // ---- the rows' unnormalised O, running max and sum, in the decode's units (O and l carry 2^kPLog2, which m takes off) ----
-    int le = l;
+    int le = threadIdx.x;
     asm volatile("" : "+v"(le));  // (nor its end's around its tile loop)
+    le &= 63;
 #pragma unroll
     for (int j = 0; j < RB; ++j) {
         const int x = 16 * (RB * r + j) + (le & 15);
