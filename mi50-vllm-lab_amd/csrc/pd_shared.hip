@@ -15,14 +15,16 @@
 // query tokens behind it (seq_len - q_len < prefix) takes all of its keys as its own.
 // The prefix's blocks are those of the first sequence that holds it.
 //
-// P' = p v_scale is rounded once to fp16 as in the default prefill (11 bits: an error of about the final fp16 rounding's
-// size; hi + lo would double the P.V products).
+// P' = p v_scale enters P.V as fp16. Rounded once, as in the default prefill, it costs an error of about the final fp16 rounding's
+// size where many keys share a row, and more where a few carry it. Workgroups with one row block per wave add what it leaves
+// (hi + lo as in the decode: 16 MFMAs of 48 a tile, while memory or set-up bounds them); with two, a tile with a heavy key does. Error
+// against 64 bits, 2-norm, of 2.1e-4 that the final rounding alone makes: 2.1e-4, and 2.9e-4 with two row blocks over 61,440 keys.
 //
-// What bounds it (gfx950, both launches, us; 24 / 4 heads unless said): 128 sequences of 64 to 2,048 keys behind 61,440 shared ones 233 to
-// 257, of which the prefix, bound by MFMA and the 32-bit arithmetic beside it, takes 207 alone (half of the MFMA rate of a large
+// What bounds it (gfx950, both launches, us; 24 / 4 heads unless said): 128 sequences of 64 to 2,048 keys behind 61,440 shared ones 254,
+// of which the prefix, bound by MFMA and the 32-bit arithmetic beside it, takes 225 alone (45 % of the MFMA rate of a large
 // matrix product), and the own keys 60 (4.7 TB/s: bound by memory); a CU streams at most 20 bytes a ns, so the deal counts
 // 1 us for an own tile and both kinds of work finish together. 32 sequences over 8,192: 38, 12 of them set-up of the pieces, their
-// partials (25 MB) and the join. 4 over 2,048: 13.7, five dependent trips to memory and a second launch.
+// partials (12 MB) and the join. 4 over 2,048: 13.5, five dependent trips to memory and a second launch.
 #include "pd_shared_body.hpp"
 #include "pth_dec.h"
 
@@ -302,11 +304,13 @@ static void launch_shared_rows(const SharedParams& s, int rows, int wgs, hipStre
         hipLaunchKernelGGL((pd_shared_kernel<4, kFast, PB>), dim3(wgs), dim3(kSwThreads), 0, stream, s);
 }
 
-// Whether the prefix's waves take two row blocks, for `rows` rows of a kv head. A tile of 128 rows costs 1.25 us with one, of 256 1.95
-// with two, and a wave that has no row no time: 24 rows over 2,048 keys 13.5 us with one and 14.7 with two, 126 over 1,111 20.0 and
-// 20.9; 192 over 8,192 37.8 and 38.7, over 61,440 107 and 94; 384 over 15,840 51 and 47; 768 over 61,440 330 and 240.
-static bool two_row_blocks(int64_t rows) {
-    return rows > 128;
+// Whether the prefix's waves take two row blocks, for `rows` rows of a kv head. Two read and widen every key half as often; one
+// makes smaller pieces and always adds lo. us with one and two, 24 / 4 heads: 24 rows over 2,048 keys 13.7 and 14.7, 126 over 1,111 20.0 and
+// 20.9; 192 over 8,192 38 and 41, over 16,384 52.5 and 51, over 32,768 78 and 66; 252 over 8,192 45 and 48, over 16,384 60 and 60; 384 over
+// 2,048 45.6 and 44.8, over 32,768 130 and 115; 768 over 61,440 388 and 266. (For up to 64 rows the own keys' form, tiles in LDS that
+// four waves share, gains 6 % over 32,768 keys and nothing below; it is not here.)
+static bool two_row_blocks(int64_t rows, int prefix) {
+    return rows > 256 || (rows > 128 && prefix > 12288);
 }
 
 hipError_t launch_shared(const LaunchArgs& x, int prefix, int bt32, hipStream_t stream) {
@@ -346,7 +350,7 @@ hipError_t launch_shared(const LaunchArgs& x, int prefix, int bt32, hipStream_t 
     const int known = compute_units(stream), cus = known > 1 ? known : 256;
     const bool fast = fast_block_table(x.block_size, x.k_ss);
     const int rows_own = x.qmax * p.G;
-    const bool two = fast && two_row_blocks((int64_t)x.num_tokens * p.G);
+    const bool two = fast && two_row_blocks((int64_t)x.num_tokens * p.G, prefix);
     two ? launch_shared_rows<true, 2>(s, rows_own, cus, stream)
         : fast ? launch_shared_rows<true, 1>(s, rows_own, cus, stream) : launch_shared_rows<false, 1>(s, rows_own, cus, stream);
     hipError_t e = hipGetLastError();

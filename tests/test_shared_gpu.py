@@ -108,6 +108,7 @@ def compare(case, prefix, out, lse=None):
 CASES = [
     # own keys, query tokens, prefix, and what differs from 24 / 4 heads, block size 16, 64 segments
     ([20, 5], [1, 1], 64, {}),
+    ([5] * 25 + [300], [1] * 26, 12321, dict(hq=6, hkv=1)),        # 156 rows behind a long prefix: two row blocks per wave
     ([0], [1], 0, {}),                                            # one sequence, nothing shared, one key
     ([0, 0, 0], [1, 1, 1], 1, {}),                                # one shared key
     ([3, 40, 0], [1, 2, 1], 31, {}),
