@@ -109,6 +109,10 @@ CASES = [
     # own keys, query tokens, prefix, and what differs from 24 / 4 heads, block size 16, 64 segments
     ([20, 5], [1, 1], 64, {}),
     ([5] * 25 + [300], [1] * 26, 12321, dict(hq=6, hkv=1)),        # 156 rows behind a long prefix: two row blocks per wave
+    # few segments over long runs: block tables that do not fit the workgroup's LDS, of the prefix and of own keys
+    ([40000, 3], [1, 1], 40000, dict(hq=6, hkv=1, nseg=4)),
+    ([40000, 3], [3, 1], 40000, dict(hq=6, hkv=1, nseg=4)),
+    ([20000, 3], [1, 3], 20000, dict(hq=6, hkv=1, nseg=4, bs=8, layout="NHD")),
     ([0], [1], 0, {}),                                            # one sequence, nothing shared, one key
     ([0, 0, 0], [1, 1, 1], 1, {}),                                # one shared key
     ([3, 40, 0], [1, 2, 1], 31, {}),
