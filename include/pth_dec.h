@@ -289,7 +289,7 @@ int pth_cache_write(const pd_tensor* key, const pd_tensor* value, const pd_tenso
  * engine runs its own rotary kernel before the cache update.
  *   query        fp16, bf16 or fp32 [T, Hq, 256], unit dim stride; rotated into query_out
  *   query_out    [T, Hq, 256] of the query's dtype or fp16: the query itself (same data, dtype and strides: in place) or
- *                a tensor that does not overlap it
+ *                a tensor that does not overlap it; its rows apart
  *   key, value   [T, Hkv, 256] of the query's dtype, left as they are; the rotated key and the value are
  *                quantised into the cache rows as pth_cache_write does
  *   positions    int64 [>= T]; a token whose position lies outside cos_sin is skipped (query_out and cache row stay)
@@ -313,7 +313,7 @@ int pth_cache_write_rotary(const pd_tensor* query, const pd_tensor* query_out, c
  *   q, key_cache .. query_start_loc, scale, num_seqs, qmax   as for pth_dec_decode (causal, no window)
  *   lse          fp32, contiguous [>= T, Hq], of pth_dec_decode_lse or _shared on the same rows; a row of
  *                -inf adds nothing
- *   weights      fp32 [>= num_seqs, Hkv, keys], unit key stride; only keys below seq_len and below `keys` are touched
+ *   weights      fp32 [>= num_seqs, Hkv, keys], unit key stride, its rows apart; only keys below seq_len and below `keys` are touched
  * Every weight is formed in a fixed order (no atomics). Returns 0, 1 or 2 as above.
  */
 int pth_cache_key_weights(const pd_tensor* q, const pd_tensor* key_cache, const pd_tensor* value_cache,

@@ -673,6 +673,14 @@ static bool heads_of_4(const pd_tensor* t, int64_t esz) {
     return reinterpret_cast<uintptr_t>(t->data) % (uintptr_t)(4 * esz) == 0 && t->strides[0] % 4 == 0 && t->strides[1] % 4 == 0;
 }
 
+// Whether the rows of `len` elements of an output's first n0 x sizes[1] (dims 0 and 1) are apart: no element has two writers.
+static bool rows_apart(const pd_tensor* t, int64_t n0, int64_t len) {
+    int64_t n[2] = {n0, t->sizes[1]}, st[2] = {t->strides[0], t->strides[1]};
+    if (n[1] <= 1 || (n[0] > 1 && st[0] < st[1])) std::swap(n[0], n[1]), std::swap(st[0], st[1]);  // the smaller stride second
+    if (n[1] <= 1 || len == 0) return true;
+    return st[1] >= len && (n[0] <= 1 || (st[0] - len) / st[1] >= n[1] - 1);
+}
+
 int pth_cache_write_rotary(const pd_tensor* query, const pd_tensor* query_out, const pd_tensor* key, const pd_tensor* value,
                            const pd_tensor* positions, const pd_tensor* cos_sin, const pd_tensor* key_cache,
                            const pd_tensor* value_cache, const pd_tensor* k_scale, const pd_tensor* v_scale,
@@ -701,6 +709,7 @@ int pth_cache_write_rotary(const pd_tensor* query, const pd_tensor* query_out, c
     const int64_t esz = dt == PD_DTYPE_FP32 ? 4 : 2, osz = out_dt == PD_DTYPE_FP32 ? 4 : 2;
     if (!(heads_of_4(query, esz) && heads_of_4(key, esz) && heads_of_4(value, esz) && heads_of_4(query_out, osz)))
         return fail(err, errlen, "query, query_out, key and value rows must be aligned to 4 elements");
+    if (!rows_apart(query_out, T, kDim)) return fail(err, errlen, "query_out rows must not overlap");
     const bool in_place = query_out->data == query->data;
     if (in_place && !(out_dt == dt && query_out->strides[0] == query->strides[0] && query_out->strides[1] == query->strides[1]))
         return fail(err, errlen, "query_out must be the query itself or not overlap it");
@@ -780,7 +789,8 @@ int pth_cache_key_weights(const pd_tensor* q, const pd_tensor* key_cache, const 
           int_rows(query_start_loc, num_seqs + 1)))
         return fail(err, errlen, "block_table / seq_lens / query_start_loc must be int32 with a row for each of 1 to 65535 sequences");
     if (const char* why = lse_refused(lse, T, Hq)) return fail(err, errlen, why);
-    if (!weight_rows(weights, num_seqs, Hkv)) return fail(err, errlen, "weights must be fp32 [num_seqs, Hkv, keys] with unit key stride");
+    if (!(weight_rows(weights, num_seqs, Hkv) && rows_apart(weights, num_seqs, weights->sizes[2])))
+        return fail(err, errlen, "weights must be fp32 [num_seqs, Hkv, keys] with unit key stride, its rows apart");
     if (T == 0 || weights->sizes[2] == 0) return 0;
     KeyWeightsParams p = {};
     p.q = static_cast<const _Float16*>(q->data);
@@ -824,8 +834,9 @@ int pth_cache_evict(const pd_tensor* weights, const pd_tensor* key_cache, const 
           int_rows(seq_lens, num_seqs) && int_table(new_block_table, num_seqs) && int_rows(new_seq_lens, num_seqs)))
         return fail(err, errlen, "block tables and sequence lengths must be int32 with a row for each of 1 to 65535 sequences");
     if (new_block_table->sizes[1] * bs < keep) return fail(err, errlen, "new_block_table must hold keep keys");
-    if (!(weight_rows(weights, num_seqs, Hkv) && weight_rows(new_weights, num_seqs, Hkv) && new_weights->sizes[2] >= keep))
-        return fail(err, errlen, "weights and new_weights must be fp32 [num_seqs, Hkv, keys] with unit key stride, new_weights of at least keep keys");
+    if (!(weight_rows(weights, num_seqs, Hkv) && weight_rows(new_weights, num_seqs, Hkv) && new_weights->sizes[2] >= keep &&
+          rows_apart(new_weights, num_seqs, new_weights->sizes[2])))
+        return fail(err, errlen, "weights and new_weights must be fp32 [num_seqs, Hkv, keys] with unit key stride, new_weights of at least keep keys, its rows apart");
     if (!(kept->dtype == PD_DTYPE_INT32 && kept->ndim == 3 && kept->sizes[0] >= num_seqs && kept->sizes[1] == Hkv &&
           kept->sizes[2] == keep && is_contig(kept)))
         return fail(err, errlen, "kept must be contiguous int32 [num_seqs, Hkv, keep]");

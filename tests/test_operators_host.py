@@ -64,6 +64,11 @@ def test_rotary_write_refusals(lib):
         (dict(query_out=x[:2, :12]), "query's dtype or fp16"),
         (dict(query_out=x.view(3, 8, 512)[:, :, :256]), "query's dtype or fp16"),
         (dict(query_out=x.as_strided((3, 12, 256), (16 * 256, 256 + 4, 1))), "itself or not overlap"),
+        (dict(query=x[:1, :12].expand(3, 12, 256), query_out=x[:1, :12].expand(3, 12, 256)), "rows must not overlap"),
+        (dict(query_out=x[:, :1].expand(3, 12, 256)), "rows must not overlap"),
+        (dict(query_out=x.as_strided((3, 12, 256), (256, 256, 1))), "rows must not overlap"),
+        (dict(query_out=x.as_strided((3, 12, 256), (11 * 256 + 4, 256, 1))), "rows must not overlap"),
+        (dict(query_out=x.as_strided((3, 12, 256), (256, 3 * 256 - 4, 1))), "rows must not overlap"),
         (dict(positions=torch.zeros(3, dtype=torch.int32)), "positions must be"),
         (dict(positions=torch.zeros(2, dtype=torch.int64)), "positions must be"),
         (dict(positions=torch.zeros(6, dtype=torch.int64)[::2]), "positions must be"),
@@ -123,10 +128,14 @@ def test_key_weights_refusals(lib):
         (dict(weights=torch.zeros((1, 2, 50))), "weights must be"),
         (dict(weights=torch.zeros((2, 2, 50)).double()), "weights must be"),
         (dict(weights=torch.zeros((2, 2, 100))[..., ::2]), "weights must be"),
+        (dict(weights=torch.zeros((1, 2, 50)).expand(2, 2, 50)), "its rows apart"),
+        (dict(weights=torch.zeros((2, 1, 50)).expand(2, 2, 50)), "its rows apart"),
+        (dict(weights=torch.zeros(200).as_strided((2, 2, 50), (99, 50, 1))), "its rows apart"),
     ]
     scalars = dict(scale=ctypes.c_double(0.1), num_seqs=2, qmax=3)
     refusals(lib.pth_cache_key_weights, names, good, scalars, cases)
-    for empty in (dict(q=case.q[:0], lse=torch.zeros((0, 12))), dict(weights=torch.zeros((2, 2, 0)))):
+    for empty in (dict(q=case.q[:0], lse=torch.zeros((0, 12))), dict(weights=torch.zeros((2, 2, 0))),
+                  dict(weights=torch.zeros((1, 1, 0)).expand(2, 2, 0))):
         t = {**good, **empty}
         assert call(lib.pth_cache_key_weights, [t[n] for n in names], *scalars.values()) == (0, "")
 
@@ -155,6 +164,8 @@ def test_evict_refusals(lib):
         (dict(weights=torch.zeros((2, 2, 100))[..., ::2]), "weights and new_weights"),
         (dict(nweights=torch.zeros((2, 2, 19))), "weights and new_weights"),
         (dict(nweights=torch.zeros((2, 2, 20)).half()), "weights and new_weights"),
+        (dict(nweights=torch.zeros((1, 2, 20)).expand(2, 2, 20)), "its rows apart"),
+        (dict(nweights=torch.zeros((2, 1, 20)).expand(2, 2, 20)), "its rows apart"),
         (dict(kept=i32(2, 2, 21)), "kept must be"),
         (dict(kept=i32(2, 2, 20).long()), "kept must be"),
         (dict(kept=i32(2, 2, 40)[..., ::2]), "kept must be"),
