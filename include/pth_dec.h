@@ -170,8 +170,7 @@ int pth_dec_decode_lse(const pd_tensor* q, const pd_tensor* key_cache, const pd_
  *                the prefix ends in, blocks that agree on its keys): the table of the first such sequence is
  *                read. Sequences that do not are computed from their own table alone.
  * At most 2^25 (token, head) rows and 2^30 / heads_kv key tiles that the block table can hold. The weights
- * enter P.V as the decode's hi + lo, but for batches of more than 128 rows per kv head over a long prefix (or more than
- * 256), where a shared key that carries little of its row enters as one fp16 (as pth_fa_forward's). Returns 0, 1 or 2 as above.
+ * enter P.V as the decode's hi + lo. Returns 0, 1 or 2 as above.
  */
 int pth_dec_decode_shared(const pd_tensor* q, const pd_tensor* key_cache, const pd_tensor* value_cache,
                           const pd_tensor* k_scale, const pd_tensor* v_scale, const pd_tensor* block_table,

@@ -15,10 +15,9 @@
 // query tokens behind it (seq_len - q_len < prefix) takes all of its keys as its own.
 // The prefix's blocks are those of the first sequence that holds it.
 //
-// P' = p v_scale enters P.V as fp16. Rounded once, as in the default prefill, it costs an error of about the final fp16 rounding's
-// size where many keys share a row, and more where a few carry it. Workgroups with one row block per wave add what it leaves
-// (hi + lo as in the decode: 16 MFMAs of 48 a tile, while memory or set-up bounds them); with two, a tile with a heavy key does. Error
-// against 64 bits, 2-norm, of 2.1e-4 that the final rounding alone makes: 2.1e-4, and 2.9e-4 with two row blocks over 61,440 keys.
+// P' = p v_scale enters P.V as fp16 hi + lo, as in the decode: rounded once it would cost an error of about the final fp16 rounding's
+// size (2.9e-4 against 64 bits, 2-norm, where that rounding alone makes 2.1e-4). The 16 more MFMAs per row block, of 48 a
+// tile, cost 19 % of the largest batch (128 sequences over 61,440 keys 254 us without, 303 with) and nothing where memory or set-up bounds.
 //
 // What bounds it (gfx950, both launches, us; 24 / 4 heads unless said): 128 sequences of 64 to 2,048 keys behind 61,440 shared ones 254,
 // of which the prefix, bound by MFMA and the 32-bit arithmetic beside it, takes 225 alone (45 % of the MFMA rate of a large
@@ -30,11 +29,12 @@
 
 namespace pd {
 
-// Costs that the deal weighs, in 0.1 us, as stamps in the kernel showed them: a key tile of an own workgroup (20 bytes a ns), of a
-// prefix workgroup with one or two row blocks per wave, a prefix piece's set-up and end. The deal is flat around them: 9 to 11,
-// 12 to 13, 60 to 100 and 250 to 400 rows below change no measured batch by more than 4 % (an own tile of 4.5: 17 %).
-constexpr unsigned kShTile = 10;
-constexpr unsigned kShPrefixTile1 = 13, kShPrefixTile2 = 20;
+// Costs that the deal weighs, in 0.1 us: a key tile of an own workgroup with one wave in rows (20 bytes a ns) or four, of a prefix
+// workgroup with one or two row blocks per wave, a prefix piece's set-up and end. Fitted to 46 batches of 10 to 86 sequences
+// (13 instead of 15 for the prefix 2 % slower on average and up to 10, 10 instead of 13 for four waves up to 25); set-up
+// of 60 to 100 and 250 to 400 rows below change no batch by more than 4 %.
+constexpr unsigned kShTile = 10, kShTileFour = 13;
+constexpr unsigned kShPrefixTile1 = 15, kShPrefixTile2 = 25;
 constexpr unsigned kShPrefixSegment = 80;
 constexpr unsigned kShMergeRows = 400;  // (token, head) rows whose segments cost 0.1 us to write and read again
 constexpr unsigned kShOwnUnits = 12;    // set-up and merge of an own segment, in tiles (pd_balanced_kernel's line)
@@ -97,7 +97,7 @@ __global__ void __launch_bounds__(kSwThreads, 1) pd_shared_kernel(const SharedPa
         const bool can = w + (own ? 1u : 0u) <= nwg && pieces <= (unsigned)(segs - 2) && pieces <= ptiles;
         const unsigned prefix_us = rounds * (seg + (ptiles + pieces - 1) / pieces * tile) + (unsigned)(T * a.Hq) * pieces / kShMergeRows;
         const unsigned share = own && can ? max((total + nwg - w - 1) / (nwg - w), longest / (unsigned)(segs - (int)pieces - 1)) : 0u;
-        const unsigned own_us = share * kShTile;
+        const unsigned own_us = share * (OW == 1 ? kShTile : kShTileFour);
         const unsigned cost = can ? min(max(prefix_us, own_us), 0x3ffffffu) : 0x3ffffffu;
         // the cheapest (the lowest lane of equal ones); more items than 17 rounds take: as many rounds as it needs
         const unsigned best = ~wave_umax(~((cost << 6) | (unsigned)lane)) & 63u;
@@ -305,12 +305,13 @@ static void launch_shared_rows(const SharedParams& s, int rows, int wgs, hipStre
 }
 
 // Whether the prefix's waves take two row blocks, for `rows` rows of a kv head. Two read and widen every key half as often; one
-// makes smaller pieces and always adds lo. us with one and two, 24 / 4 heads: 24 rows over 2,048 keys 13.7 and 14.7, 126 over 1,111 20.0 and
-// 20.9; 192 over 8,192 38 and 41, over 16,384 52.5 and 51, over 32,768 78 and 66; 252 over 8,192 45 and 48, over 16,384 60 and 60; 384 over
-// 2,048 45.6 and 44.8, over 32,768 130 and 115; 768 over 61,440 388 and 266. (For up to 64 rows the own keys' form, tiles in LDS that
-// four waves share, gains 6 % over 32,768 keys and nothing below; it is not here.)
+// makes smaller pieces and tiles. us with one and two, 24 / 4 heads: 192 rows over 8,192 keys 37.6 and 39.0, over 61,440 109.6 and 111;
+// 258 over 32,768 93.7 and 104; 384 over 16,384 69.8 and 75.8, over 61,440 169 and 179; 510 over 16,384 89.5 and 89.6, over 32,768
+// 136 and 132, over 61,440 224 and 200; 768 over 8,192 66.9 and 72.5, over 16,384 99.2 and 99.3, over 32,768 181 and 161, over 61,440
+// 309 and 275; 1,020 over 8,192 108 and 115, over 32,768 256 and 232. (For up to 64 rows the own keys' form, tiles in LDS that four waves
+// share, gains 6 % over 32,768 keys and nothing below; it is not here.)
 static bool two_row_blocks(int64_t rows, int prefix) {
-    return rows > 256 || (rows > 128 && prefix > 12288);
+    return rows > 384 && prefix > 16384;
 }
 
 hipError_t launch_shared(const LaunchArgs& x, int prefix, int bt32, hipStream_t stream) {

@@ -15,7 +15,7 @@
 //   RW = 4  (own keys, up to 48 rows) as RW = 1 on tiles in LDS that four waves share; 7 sequences of 3 x 6 rows 20.0 us, with two row
 //           blocks per wave and four key groups 21.9.
 // Tiles come by DMA into rings of kRing slots per key group, copied by the group's own waves; RW > 1: one barrier per tile.
-// P' = p v_scale enters P.V as fp16, hi and, always with one row block, lo (see pd_shared.hip).
+// P' = p v_scale enters P.V as fp16 hi + lo (see pd_shared.hip).
 #pragma once
 
 #include "pd_tile.hpp"
@@ -277,69 +277,38 @@ __device__ __forceinline__ void shared_body(const SharedParams& sp, const Shared
         __builtin_memcpy(&lo8, y, 16);
     };
     auto sum8 = [](const float (&p)[8]) __attribute__((always_inline)) { return ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7])); };
-    // (vs: with one row block)
-    auto values = [&](int kb, const float4_t (&vs)[2], const lds_u8* S, const lds_u8* F) __attribute__((always_inline)) {
+    auto values = [&](int kb, const lds_u8* S, const lds_u8* F) __attribute__((always_inline)) {
         half8_t pf[RB], pl[RB];
-        // O += V^T times each of the terms
-        auto products = [&](auto both) __attribute__((always_inline)) {
-            constexpr int kAhead = 3;
-            half8_t vb[kAhead + 1];
-            if constexpr (RW == 8) {
+        float4_t vs[2];
+        value_scales(kb, S, vs);
 #pragma unroll
-                for (int m = 0; m < kAhead; ++m) vb[m] = *(const lds_half8*)(F + (16 + m) * 1024);
-            }
-#pragma unroll
-            for (int m = 0; m < 16; ++m) {
-                half8_t vf;
-                if constexpr (RW == 8) {
-                    if (m + kAhead < 16) vb[(m + kAhead) % (kAhead + 1)] = *(const lds_half8*)(F + (16 + m + kAhead) * 1024);
-                    __builtin_amdgcn_sched_barrier(0);
-                    vf = vb[m % (kAhead + 1)];
-                } else {
-                    const int2_t vr = __builtin_amdgcn_ds_read_tr8_b64_v2i32((lds_int2*)(S + vro[m >> 3] + 16 * m));
-                    vf = widen_i8x8_exact((unsigned)vr.x, (unsigned)vr.y);
-                }
-#pragma unroll
-                for (int j = 0; j < RB; ++j) {
-                    oacc[m][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, pf[j], oacc[m][j], 0, 0, 0);
-                    if constexpr (decltype(both)::value) oacc[m][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, pl[j], oacc[m][j], 0, 0, 0);
-                }
-            }
-        };
-        if constexpr (RB == 1) {
+        for (int j = 0; j < RB; ++j) {
             float p[8];
-            weights(0, p);
-            l_run[0] += sum8(p);
-            split(p, vs, pf[0], pl[0]);
-            products(std::true_type{});
-        } else {
-            // A pass for hi and, where some key is heavy, one for lo (in a loop: registers are short). Heavy: a weight above
-            // the lane's sum before, which is about a quarter of the row's.
-            bool heavy = false;
+            weights(j, p);
+            l_run[j] += sum8(p);
+            split(p, vs, pf[j], pl[j]);
+        }
+        constexpr int kAhead = 3;
+        half8_t vb[kAhead + 1];
+        if constexpr (RW == 8) {
 #pragma unroll
-            for (int j = 0; j < RB; ++j) heavy |= __builtin_amdgcn_exp2f(max8(j)) > l_run[j];
-            int passes = __builtin_amdgcn_ballot_w64(heavy) != 0 ? 2 : 1;
-            float4_t vp[2];
-            value_scales(kb, S, vp);
+            for (int m = 0; m < kAhead; ++m) vb[m] = *(const lds_half8*)(F + (16 + m) * 1024);
+        }
 #pragma unroll
-            for (int j = 0; j < RB; ++j) {
-                float p[8];
-                weights(j, p);
-                l_run[j] += sum8(p);
-                if (passes == 2) {
-                    split(p, vp, pf[j], pl[j]);
-                } else {
-                    half8_t unused;
-                    split(p, vp, pf[j], unused);
-                }
+        for (int m = 0; m < 16; ++m) {
+            half8_t vf;
+            if constexpr (RW == 8) {
+                if (m + kAhead < 16) vb[(m + kAhead) % (kAhead + 1)] = *(const lds_half8*)(F + (16 + m + kAhead) * 1024);
+                __builtin_amdgcn_sched_barrier(0);
+                vf = vb[m % (kAhead + 1)];
+            } else {
+                const int2_t vr = __builtin_amdgcn_ds_read_tr8_b64_v2i32((lds_int2*)(S + vro[m >> 3] + 16 * m));
+                vf = widen_i8x8_exact((unsigned)vr.x, (unsigned)vr.y);
             }
-#pragma unroll 1
-            while (true) {
-                products(std::false_type{});
-                if (--passes == 0) break;
 #pragma unroll
-                for (int j = 0; j < RB; ++j) pf[j] = pl[j];
-            }
+            for (int j = 0; j < RB; ++j) oacc[m][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, pf[j], oacc[m][j], 0, 0, 0);
+#pragma unroll
+            for (int j = 0; j < RB; ++j) oacc[m][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, pl[j], oacc[m][j], 0, 0, 0);
         }
     };
 
@@ -479,10 +448,8 @@ __device__ __forceinline__ void shared_body(const SharedParams& sp, const Shared
                 if (rows) {
                     const int kb = (t0 + n) * kTile;
                     const lds_u8* F = fr + (n & 1) * kSwFrag;
-                    float4_t vs[2];
                     scores(kb, S0, F, nullptr);
-                    if constexpr (RB == 1) value_scales(kb, S0, vs);
-                    values(kb, vs, S0, F);
+                    values(kb, S0, F);
                 }
                 if (w >= 4) prepare();
                 S0 = S1;
@@ -513,10 +480,8 @@ __device__ __forceinline__ void shared_body(const SharedParams& sp, const Shared
                 if (n + kRing - 1 < mine) issue(n + kRing - 1);  // into tile n - 1's slot, which every wave is done with
                 if (rows && n < mine) {
                     const int kb = (t0 + KW * n + k) * kTile;
-                    float4_t vs[2];
                     scores(kb, S, nullptr, nullptr);
-                    value_scales(kb, S, vs);
-                    values(kb, vs, S, nullptr);
+                    values(kb, S, nullptr);
                 }
                 S += kSwSlot;
                 if (--left == 0) {
@@ -553,10 +518,8 @@ __device__ __forceinline__ void shared_body(const SharedParams& sp, const Shared
                 if (n + 1 < mine) request(n + 1);
                 const int kb = (t0 + KW * n + k) * kTile;
                 const lds_u8* S = L + (k * 2 + (n & 1)) * kSwOwn - kImgV;  // (as if a K image came first)
-                float4_t vs[2];
                 scores(kb, S, nullptr, kc);
-                value_scales(kb, S, vs);
-                values(kb, vs, S, nullptr);
+                values(kb, S, nullptr);
                 wait_lds();  // the slot has been read
             }
         }

@@ -234,8 +234,7 @@ def decode_shared(q: torch.Tensor, key_cache: torch.Tensor, value_cache: torch.T
     partial buffers need NSEG >= 4. prefix_len keys, within the block table's width: the tables of all sequences that hold them
     before their query tokens name the same blocks for them (a block that the prefix ends in may be each sequence's own
     copy). A sequence that does not hold them, seq_len - q_len < prefix_len, is computed from its own table alone, and a padded
-    one (seq_len 0 or no query tokens) is left alone. Weights enter P.V as decode's hi + lo, but for large batches, where a
-    shared key that carries little of its row enters as one fp16. lse: as decode's.
+    one (seq_len 0 or no query tokens) is left alone. Weights enter P.V as decode's hi + lo. lse: as decode's.
     """
     native().decode_shared(_entry("pth_dec_decode_shared"), q, key_cache, value_cache, k_scale, v_scale, block_table, seq_lens,
                            query_start_loc, out, part_o, part_m, part_l, lse, scale, int(num_seqs), int(qmax), int(prefix_len))
