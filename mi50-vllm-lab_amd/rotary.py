@@ -7,8 +7,8 @@ scaled (`scaling`):
           highest stays.
   yarn    Peng et al., "YaRN: Efficient Context Window Extension of Large Language Models" (2023): pairs that turn more than
           beta_fast times over the original context keep their frequency, those that turn less than
-          beta_slow times are divided by factor, linearly blended in between over the pair number; the cosines and sines
-          are multiplied by 0.1 ln(factor) + 1 (or by attention_factor).
+          beta_slow times are divided by factor, linearly blended in between over the pair number (whose ends, rounded outwards,
+          are kept within 0 and rotary_dim - 1); the cosines and sines are multiplied by 0.1 ln(factor) + 1 (or by attention_factor).
 """
 from __future__ import annotations
 
@@ -41,7 +41,8 @@ def rotary_frequencies(rotary_dim: int, base: float = 10000.0, scaling: dict | N
         def pair_of(turns: float) -> float:  # the pair number that turns so often over the original context
             return rotary_dim * math.log(original / (turns * 2.0 * math.pi)) / (2.0 * math.log(base))
 
-        lo, hi = max(0, math.floor(pair_of(fast))), min(rotary_dim // 2 - 1, math.ceil(pair_of(slow)))
+        # (hi may lie beyond the last pair: if that still turns more than beta_slow times, the ramp ends behind it)
+        lo, hi = max(0, math.floor(pair_of(fast))), min(rotary_dim - 1, math.ceil(pair_of(slow)))
         number = torch.arange(rotary_dim // 2, dtype=torch.float64)
         slowed = ((number - lo) / max(hi - lo, 1e-3)).clamp(0.0, 1.0)
         mult = scaling.get("attention_factor")
