@@ -710,7 +710,7 @@ int pth_cache_write_rotary(const pd_tensor* query, const pd_tensor* query_out, c
     if (!(heads_of_4(query, esz) && heads_of_4(key, esz) && heads_of_4(value, esz) && heads_of_4(query_out, osz)))
         return fail(err, errlen, "query, query_out, key and value rows must be aligned to 4 elements");
     if (!rows_apart(query_out, T, kDim)) return fail(err, errlen, "query_out rows must not overlap");
-    const bool in_place = query_out->data == query->data;
+    const bool in_place = T > 0 && query_out->data == query->data;  // (all empty tensors are at null)
     if (in_place && !(out_dt == dt && query_out->strides[0] == query->strides[0] && query_out->strides[1] == query->strides[1]))
         return fail(err, errlen, "query_out must be the query itself or not overlap it");
     if (!(positions->dtype == PD_DTYPE_INT64 && positions->ndim == 1 && positions->sizes[0] >= T &&
