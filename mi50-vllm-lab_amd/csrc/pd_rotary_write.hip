@@ -122,12 +122,24 @@ __global__ void __launch_bounds__(256) pd_rotary_write_kernel(const RotaryWriteP
 // ---------------------------------------------------------------------------------------
 // host side
 
+// A launch has fewer than 2^32 threads, 2^24 workgroups: longer batches go a run of tokens at a time.
 template <class In, class Out, int kLanes>
 static void launch_groups(RotaryWriteParams p, hipStream_t stream) {
-    const int64_t kv = ((int64_t)p.T * p.Hkv + 7) / 8, groups = (p.Hq + kHeads - 1) / kHeads;
-    const int64_t q = ((int64_t)p.T * groups + 256 / kLanes - 1) / (256 / kLanes);
-    p.kv_groups = (int)kv;
-    hipLaunchKernelGGL((pd_rotary_write_kernel<In, Out, kLanes>), dim3((unsigned)(kv + q)), dim3(256), 0, stream, p);
+    const int64_t tokens = p.T, groups = (p.Hq + kHeads - 1) / kHeads;
+    const int64_t most = (((int64_t)1 << 24) - 2) * 256 / (32 * (int64_t)p.Hkv + kLanes * groups);
+    const RotaryWriteParams all = p;
+    for (int64_t t = 0; t < tokens; t += most) {
+        p.T = (int)(tokens - t < most ? tokens - t : most);
+        p.query = static_cast<const In*>(all.query) + t * p.q_st;
+        p.query_out = static_cast<Out*>(all.query_out) + t * p.o_st;
+        p.key = static_cast<const In*>(all.key) + t * p.k_st;
+        p.value = static_cast<const In*>(all.value) + t * p.v_st;
+        p.positions = all.positions + t;
+        p.slots = all.slots + t;
+        const int64_t kv = ((int64_t)p.T * p.Hkv + 7) / 8, q = (p.T * groups + 256 / kLanes - 1) / (256 / kLanes);
+        p.kv_groups = (int)kv;
+        hipLaunchKernelGGL((pd_rotary_write_kernel<In, Out, kLanes>), dim3((unsigned)(kv + q)), dim3(256), 0, stream, p);
+    }
 }
 
 template <class In, class Out>

@@ -1,0 +1,41 @@
+"""The operators around a decode step at sizes beyond what one launch numbers, and on inputs at the edges of their contracts, on
+the GPU.
+"""
+import pytest
+import torch
+
+import workload as kvc
+from mi50_vllm_lab_amd import pth_dec, rotary
+
+pytestmark = pytest.mark.gpu
+
+
+def test_rotary_write_of_more_tokens_than_one_launch_takes():
+    # 8.1 million tokens of 16 kv heads and one query head are 17.2 million workgroups; a launch has fewer than 2^24
+    T, hq, hkv, rd = 8_100_001, 1, 16, 64
+    g = torch.Generator(device="cuda").manual_seed(1)
+    table = rotary.rotary_table(rd, 600, device="cuda")
+    one = torch.randn((1, hq + 2 * hkv, 256), device="cuda", generator=g).half()
+    x = one.expand(T, -1, -1)
+    pos = torch.arange(T, device="cuda") % 600
+    slots = torch.full((T,), -1, device="cuda")
+    at = torch.tensor([0, 1, 4_000_000, 7_895_158, 7_895_159, 7_895_160, 7_895_161, T - 2, T - 1], device="cuda")
+    slots[at] = torch.arange(len(at), device="cuda") * 3
+    caches = [kvc.allocate_cache(2, 16, hkv, "HND", "cuda") for _ in range(2)]
+    out = torch.empty((T, hq, 256), dtype=torch.float16, device="cuda")
+    c = caches[0]
+    pth_dec.rotary_cache_write(x[:, :hq], x[:, hq:hq + hkv], x[:, hq + hkv:], pos, table, c.key_cache, c.value_cache, c.k_scale,
+                               c.v_scale, slots, query_out=out)
+    # the 600 positions, in one launch
+    small = torch.empty((600, hq, 256), dtype=torch.float16, device="cuda")
+    c, n = caches[1], torch.full((600,), -1, device="cuda")
+    y = one.expand(600, -1, -1)
+    pth_dec.rotary_cache_write(y[:, :hq], y[:, hq:hq + hkv], y[:, hq + hkv:], pos[:600].clone(), table, c.key_cache, c.value_cache,
+                               c.k_scale, c.v_scale, n, query_out=small)
+    for t in range(0, T, 600_000):
+        part = out[t:t + 600_000]
+        assert torch.equal(part, small[pos[t:t + 600_000]]), t
+    z = one.expand(len(at), -1, -1)
+    pth_dec.rotary_cache_write(z[:, :hq], z[:, hq:hq + hkv], z[:, hq + hkv:], pos[at], table, c.key_cache, c.value_cache, c.k_scale,
+                               c.v_scale, slots[at], query_out=torch.empty((len(at), hq, 256), dtype=torch.float16, device="cuda"))
+    assert torch.equal(caches[0].kv, caches[1].kv)
