@@ -312,7 +312,8 @@ int pth_cache_write_rotary(const pd_tensor* query, const pd_tensor* query_out, c
  *   q, key_cache .. query_start_loc, scale, num_seqs, qmax   as for pth_dec_decode (causal, no window)
  *   lse          fp32, contiguous [>= T, Hq], of pth_dec_decode_lse or _shared on the same rows; a row of
  *                -inf adds nothing
- *   weights      fp32 [>= num_seqs, Hkv, keys], unit key stride, its rows apart; only keys below seq_len and below `keys` are touched
+ *   weights      fp32 [>= num_seqs, Hkv, keys <= 2^28], unit key stride, its rows apart; only keys below seq_len and below `keys`
+ *                are touched
  * Every weight is formed in a fixed order (no atomics). Returns 0, 1 or 2 as above.
  */
 int pth_cache_key_weights(const pd_tensor* q, const pd_tensor* key_cache, const pd_tensor* value_cache,
@@ -325,14 +326,14 @@ int pth_cache_key_weights(const pd_tensor* q, const pd_tensor* key_cache, const 
  * Eviction by running weights: per sequence and kv head the last `recent` keys and the keep - recent others with the
  * largest weights stay (equal weights: the lowest key; NaN counts as the largest), in the order of their positions. Their
  * rows are copied into the blocks of new_block_table; the old blocks are left as they are. No counterpart in the reference.
- *   weights      fp32 [>= num_seqs, Hkv, keys]; keys of a sequence past `keys` or past its block table are dropped
+ *   weights      fp32 [>= num_seqs, Hkv, keys <= 2^28]; keys of a sequence past `keys` or past its block table are dropped
  *   block_table, seq_lens   int32, the batch before; sequences of at most keep keys are copied whole
  *   new_block_table         int32 [>= num_seqs, columns for keep keys]: blocks that no table row of the call reads
  *                           and no two of its rows share, in the part that holds a sequence's min(seq_len, keep) keys
  *   new_seq_lens            int32 [>= num_seqs], written: min(seq_len, keep)
  *   new_weights             fp32 [>= num_seqs, Hkv, >= keep], written: the kept keys' weights, then zeros
  *   kept                    int32, contiguous [>= num_seqs, Hkv, keep], written: the kept keys' numbers, then -1
- *   keep, recent            keep >= 1, 0 <= recent <= keep
+ *   keep, recent            1 <= keep <= 2^28, 0 <= recent <= keep
  * The new tensors must not be the old ones. Rotated keys keep the positions they were rotated by; rows written later take
  * positions (pth_cache_write_rotary) that count the evicted keys too. Returns 0, 1 or 2 as above.
  */

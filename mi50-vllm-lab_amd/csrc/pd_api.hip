@@ -762,9 +762,11 @@ static bool int_rows(const pd_tensor* t, int64_t n) { return t->dtype == PD_DTYP
 static bool int_table(const pd_tensor* t, int64_t n) {
     return t->dtype == PD_DTYPE_INT32 && t->ndim == 2 && t->strides[1] == 1 && t->sizes[0] >= n && t->sizes[1] <= INT32_MAX;
 }
+// Keys of a row of weights, and that stay: the kernels step over them in 32 bits, and a launch copies 32 to a workgroup.
+constexpr int64_t kMaxWeightKeys = (int64_t)1 << 28;
 // fp32 [>= num_seqs, Hkv, keys] with its keys side by side
 static bool weight_rows(const pd_tensor* t, int64_t n, int64_t hkv) {
-    return t->dtype == PD_DTYPE_FP32 && t->ndim == 3 && t->sizes[0] >= n && t->sizes[1] == hkv && t->sizes[2] <= INT32_MAX &&
+    return t->dtype == PD_DTYPE_FP32 && t->ndim == 3 && t->sizes[0] >= n && t->sizes[1] == hkv && t->sizes[2] <= kMaxWeightKeys &&
            (t->strides[2] == 1 || t->sizes[2] <= 1);
 }
 
@@ -790,7 +792,7 @@ int pth_cache_key_weights(const pd_tensor* q, const pd_tensor* key_cache, const 
         return fail(err, errlen, "block_table / seq_lens / query_start_loc must be int32 with a row for each of 1 to 65535 sequences");
     if (const char* why = lse_refused(lse, T, Hq)) return fail(err, errlen, why);
     if (!(weight_rows(weights, num_seqs, Hkv) && rows_apart(weights, num_seqs, weights->sizes[2])))
-        return fail(err, errlen, "weights must be fp32 [num_seqs, Hkv, keys] with unit key stride, its rows apart");
+        return fail(err, errlen, "weights must be fp32 [num_seqs, Hkv, keys] of at most 2^28 keys with unit key stride, its rows apart");
     if (T == 0 || weights->sizes[2] == 0) return 0;
     KeyWeightsParams p = {};
     p.q = static_cast<const _Float16*>(q->data);
@@ -828,15 +830,15 @@ int pth_cache_evict(const pd_tensor* weights, const pd_tensor* key_cache, const 
     if (!layout_ok(key_cache, value_cache, k_scale, v_scale))
         return fail(err, errlen, "KV cache views do not have the int8 per-token-head row layout");
     const int64_t Hkv = key_cache->sizes[2], bs = key_cache->sizes[1];
-    if (!(keep >= 1 && keep <= INT32_MAX && recent >= 0 && recent <= keep))
-        return fail(err, errlen, "keep must be at least 1 and recent in [0, keep]");
+    if (!(keep >= 1 && keep <= kMaxWeightKeys && recent >= 0 && recent <= keep))
+        return fail(err, errlen, "keep must be in [1, 2^28] and recent in [0, keep]");
     if (!(num_seqs >= 1 && num_seqs <= 65535 && Hkv >= 1 && Hkv <= 65535 && int_table(block_table, num_seqs) &&
           int_rows(seq_lens, num_seqs) && int_table(new_block_table, num_seqs) && int_rows(new_seq_lens, num_seqs)))
         return fail(err, errlen, "block tables and sequence lengths must be int32 with a row for each of 1 to 65535 sequences");
     if (new_block_table->sizes[1] * bs < keep) return fail(err, errlen, "new_block_table must hold keep keys");
     if (!(weight_rows(weights, num_seqs, Hkv) && weight_rows(new_weights, num_seqs, Hkv) && new_weights->sizes[2] >= keep &&
           rows_apart(new_weights, num_seqs, new_weights->sizes[2])))
-        return fail(err, errlen, "weights and new_weights must be fp32 [num_seqs, Hkv, keys] with unit key stride, new_weights of at least keep keys, its rows apart");
+        return fail(err, errlen, "weights and new_weights must be fp32 [num_seqs, Hkv, keys] of at most 2^28 keys with unit key stride, new_weights of at least keep keys, its rows apart");
     if (!(kept->dtype == PD_DTYPE_INT32 && kept->ndim == 3 && kept->sizes[0] >= num_seqs && kept->sizes[1] == Hkv &&
           kept->sizes[2] == keep && is_contig(kept)))
         return fail(err, errlen, "kept must be contiguous int32 [num_seqs, Hkv, keep]");

@@ -234,7 +234,7 @@ __global__ void __launch_bounds__(256) pd_evict_copy_kernel(const EvictParams a)
     const int g = blockIdx.y, b = blockIdx.z, j0 = blockIdx.x * kEvCopyRows, tid = threadIdx.x;
     const int n = max(0, min(min(a.seq_lens[b], a.max_keys), a.keep));
     float* wdst = a.new_weights + (int64_t)b * a.n_sb + (int64_t)g * a.n_sh;
-    for (int j = n + blockIdx.x * 256 + tid; j < a.new_keys; j += 256 * gridDim.x) wdst[j] = 0.f;
+    for (int64_t j = n + (int64_t)blockIdx.x * 256 + tid; j < a.new_keys; j += (int64_t)256 * gridDim.x) wdst[j] = 0.f;
     const int rows = min(kEvCopyRows, n - j0);
     if (rows <= 0) return;
     if (tid < rows) {

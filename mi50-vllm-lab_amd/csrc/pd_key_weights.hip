@@ -39,7 +39,7 @@ __global__ void __launch_bounds__(64 * kKwWaves) pd_key_weights_kernel(const Key
     const int seq_len = a.seq_lens[b];
     if (q_len <= 0 || seq_len <= 0) return;
     const int G = a.G, R = min(16 * NRB, min(q_len, a.qmax) * G), ctx0 = seq_len - q_len;
-    const int nblk = (seq_len + kKwKeys - 1) / kKwKeys, stride = gridDim.x * kKwWaves;
+    const int nblk = (min(seq_len, a.max_keys) + kKwKeys - 1) / kKwKeys, stride = gridDim.x * kKwWaves;
     const int first = blockIdx.x * kKwWaves + w;
     if (first >= nblk) return;
 

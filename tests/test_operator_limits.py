@@ -48,3 +48,36 @@ def test_rotary_write_of_no_tokens_into_another_tensor(lib, dtype, out):
     # (the data of all empty tensors is the null pointer: that does not make query_out the query)
     assert call(lib.pth_cache_write_rotary, describe(x[:, :12], out(12), x[:, 12:14], x[:, 14:], n, torch.zeros((9, 64)), *views(c), n),
                 0) == (0, "")
+
+
+# ---- sizes that 32-bit steps or a launch would not do ----
+
+def weights_args(change):
+    c = case()
+    i32 = lambda *s: torch.zeros(s, dtype=torch.int32)  # noqa: E731
+    d = dict(zip(("q", "kc", "vc", "ks", "vs", "bt", "lens", "qsl", "lse", "weights"), describe(
+        c.q, *views(c.cache), c.block_table, c.seq_lens, c.query_start_loc, torch.zeros((4, 12)), torch.zeros((2, 2, 50)))))
+    e = dict(zip(("weights", "kc", "vc", "ks", "vs", "bt", "lens", "nbt", "nlens", "nweights", "kept"), describe(
+        torch.zeros((2, 2, 50)), *views(c.cache), c.block_table, c.seq_lens, i32(2, 2), i32(2), torch.zeros((2, 2, 20)), i32(2, 2, 20))))
+    for t in (d, e):
+        for name, (dim, size) in change.items():
+            if name in t:
+                rows = 1
+                t[name].sizes[dim] = size
+                for i in (2, 1, 0) if t[name].ndim == 3 else (1, 0):
+                    t[name].strides[i], rows = rows, rows * t[name].sizes[i]
+    return d, e
+
+
+@pytest.mark.parametrize("keys", [(1 << 28) + 1, (1 << 31) - 1])
+def test_rows_of_more_keys_than_2_to_the_28(lib, keys):
+    d, e = weights_args({"weights": (2, keys)})
+    rc, text = call(lib.pth_cache_key_weights, d.values(), ctypes.c_double(0.1), 2, 3)
+    assert rc == 1 and "at most 2^28 keys" in text
+    rc, text = call(lib.pth_cache_evict, e.values(), 2, 20, 4)
+    assert rc == 1 and "at most 2^28 keys" in text
+    rc, text = call(lib.pth_cache_evict, weights_args({"nweights": (2, keys)})[1].values(), 2, 20, 4)
+    assert rc == 1 and "at most 2^28 keys" in text
+    e = weights_args({"nweights": (2, keys), "kept": (2, keys), "nbt": (1, keys)})[1]
+    rc, text = call(lib.pth_cache_evict, e.values(), 2, keys, 4)
+    assert rc == 1 and "keep must be in [1, 2^28]" in text

@@ -39,3 +39,20 @@ def test_rotary_write_of_more_tokens_than_one_launch_takes():
     pth_dec.rotary_cache_write(z[:, :hq], z[:, hq:hq + hkv], z[:, hq + hkv:], pos[at], table, c.key_cache, c.value_cache, c.k_scale,
                                c.v_scale, slots[at], query_out=torch.empty((len(at), hq, 256), dtype=torch.float16, device="cuda"))
     assert torch.equal(caches[0].kv, caches[1].kv)
+
+
+def test_evict_with_the_largest_budget():
+    # a short sequence; behind it 2^28 places to clear, a workgroup per 32 of them
+    keep, bs, n = 1 << 28, 1584, 100
+    c = kvc.allocate_cache(3, bs, 1, "HND", "cuda")
+    c.kv.random_(-128, 128, generator=torch.Generator(device="cuda").manual_seed(2))
+    before = c.kv.clone()
+    old, new = torch.tensor([[0]], dtype=torch.int32, device="cuda"), torch.full((1, -(-keep // bs)), 2, dtype=torch.int32, device="cuda")
+    lens, new_lens = torch.tensor([n], dtype=torch.int32, device="cuda"), torch.zeros(1, dtype=torch.int32, device="cuda")
+    w = torch.rand((1, 1, 200), device="cuda")
+    new_w, kept = torch.full((1, 1, keep), 9.0, device="cuda"), torch.full((1, 1, keep), 9, dtype=torch.int32, device="cuda")
+    pth_dec.evict(w, c.key_cache, c.value_cache, c.k_scale, c.v_scale, old, lens, new, new_lens, new_w, kept, 1, keep, 5)
+    torch.cuda.synchronize()
+    assert new_lens.tolist() == [n] and kept[0, 0, :n].tolist() == list(range(n)) and torch.equal(new_w[0, 0, :n], w[0, 0, :n])
+    assert int(kept[0, 0, n:].max()) == -1 and int(kept[0, 0, n:].min()) == -1 and not bool(new_w[0, 0, n:].any())
+    assert torch.equal(c.kv[2, 0, :n], before[0, 0, :n]) and torch.equal(c.kv[:2], before[:2]) and torch.equal(c.kv[2, 0, n:], before[2, 0, n:])
