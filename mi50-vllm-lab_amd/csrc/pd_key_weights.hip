@@ -69,8 +69,8 @@ __global__ void __launch_bounds__(64 * kKwWaves) pd_key_weights_kernel(const Key
 
     // ---- Q^T: lane (lg, li) holds row 16 rb + li, dims 64 (st / 2) + 16 lg + 8 (st % 2) + [0, 8) ----
     half8_t qop[NRB][8];
-    float nlse[NRB];  // -lse in log2 units; -inf for a row that counts for nothing
-    int rpos[NRB];
+    float nlse[NRB];  // -lse in log2 units
+    int rpos[NRB];    // the last key that counts for the row: none where its sum was 0 or it is past the last row
     bool valid[NRB];
 #pragma unroll
     for (int rb = 0; rb < NRB; ++rb) {
@@ -82,7 +82,7 @@ __global__ void __launch_bounds__(64 * kKwWaves) pd_key_weights_kernel(const Key
         for (int st = 0; st < 8; ++st)
             __builtin_memcpy(&qop[rb][st], __builtin_assume_aligned(qrow + 64 * (st >> 1) + 16 * lg + 8 * (st & 1), 4), 16);
         nlse[rb] = a.lse[(int64_t)(q0 + qi) * a.Hq + g * G + qh];
-        rpos[rb] = valid[rb] ? ctx0 + qi : -1;
+        rpos[rb] = ctx0 + qi;
     }
     Block cur = fetch(first, page0), next = cur;
     if (first + stride < nblk) next = fetch(first + stride, page1);
@@ -90,8 +90,8 @@ __global__ void __launch_bounds__(64 * kKwWaves) pd_key_weights_kernel(const Key
     for (int rb = 0; rb < NRB; ++rb) {
 #pragma unroll
         for (int st = 0; st < 8; ++st) qop[rb][st] = valid[rb] ? qop[rb][st] : (half8_t)(_Float16)0.0f;
-        // a row whose sum was 0 (lse -inf) weighs nothing, and neither does a row past the last
-        nlse[rb] = valid[rb] && nlse[rb] != kNegInf ? -nlse[rb] * 1.4426950408889634f : kNegInf;
+        rpos[rb] = valid[rb] && nlse[rb] != kNegInf ? rpos[rb] : -1;
+        nlse[rb] *= -1.4426950408889634f;
     }
     for (int n = first; n < nblk; n += stride) {
         Block later = next;

@@ -56,3 +56,21 @@ def test_evict_with_the_largest_budget():
     assert new_lens.tolist() == [n] and kept[0, 0, :n].tolist() == list(range(n)) and torch.equal(new_w[0, 0, :n], w[0, 0, :n])
     assert int(kept[0, 0, n:].max()) == -1 and int(kept[0, 0, n:].min()) == -1 and not bool(new_w[0, 0, n:].any())
     assert torch.equal(c.kv[2, 0, :n], before[0, 0, :n]) and torch.equal(c.kv[:2], before[:2]) and torch.equal(c.kv[2, 0, n:], before[2, 0, n:])
+
+
+def test_key_weights_of_rows_without_a_sum_where_scores_are_not_finite():
+    # e^(score - lse) of a row with lse -inf is no weight, whatever its scores are: with infinite or NaN key scales too
+    case = kvc.make_case([50, 20], [2, 1], num_q_heads=12, num_kv_heads=2, block_size=16, seed=8)
+    d = case.to("cuda")
+    page = case.block_table[0].long()
+    d.cache.k_scale[int(page[0]), 3] = float("inf")
+    d.cache.k_scale[int(page[1]), 2] = float("nan")
+    d.cache.k_scale[int(page[2]), 5] = float("-inf")
+    lse = torch.zeros((3, 12), device="cuda")
+    lse[:2] = float("-inf")
+    w = torch.rand((2, 2, 60), device="cuda")
+    before = w.clone()
+    pth_dec.key_weights(d.q, d.cache.key_cache, d.cache.value_cache, d.cache.k_scale, d.cache.v_scale, d.block_table, d.seq_lens,
+                        d.query_start_loc, lse, w, d.scale, 2, 2)
+    assert torch.equal(w[0], before[0])
+    assert bool(torch.isfinite(w[1]).all()) and bool((w[1, :, :21] > before[1, :, :21]).all())
