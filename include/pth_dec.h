@@ -288,7 +288,8 @@ int pth_cache_write(const pd_tensor* key, const pd_tensor* value, const pd_tenso
  * engine runs its own rotary kernel before the cache update.
  *   query        fp16, bf16 or fp32 [T, Hq, 256], unit dim stride; rotated into query_out
  *   query_out    [T, Hq, 256] of the query's dtype or fp16: the query itself (same data, dtype and strides: in place) or
- *                a tensor that does not overlap it; its rows apart
+ *                a tensor that does not overlap it; its rows apart, and no part of key or value. (Views of one buffer are
+ *                known to be apart by their extents, or by a stride that both have.)
  *   key, value   [T, Hkv, 256] of the query's dtype, left as they are; the rotated key and the value are
  *                quantised into the cache rows as pth_cache_write does
  *   positions    int64 [>= T]; a token whose position lies outside cos_sin is skipped (query_out and cache row stay)
@@ -334,7 +335,8 @@ int pth_cache_key_weights(const pd_tensor* q, const pd_tensor* key_cache, const 
  *   new_weights             fp32 [>= num_seqs, Hkv, >= keep], written: the kept keys' weights, then zeros
  *   kept                    int32, contiguous [>= num_seqs, Hkv, keep], written: the kept keys' numbers, then -1
  *   keep, recent            1 <= keep <= 2^28, 0 <= recent <= keep
- * The new tensors must not be the old ones. Rotated keys keep the positions they were rotated by; rows written later take
+ * The new tensors must not be the old ones, and those written (new_seq_lens, new_weights, kept) overlap neither what is
+ * read nor each other. Rotated keys keep the positions they were rotated by; rows written later take
  * positions (pth_cache_write_rotary) that count the evicted keys too. Returns 0, 1 or 2 as above.
  */
 int pth_cache_evict(const pd_tensor* weights, const pd_tensor* key_cache, const pd_tensor* value_cache,

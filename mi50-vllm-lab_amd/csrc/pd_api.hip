@@ -681,6 +681,39 @@ static bool rows_apart(const pd_tensor* t, int64_t n0, int64_t len) {
     return st[1] >= len && (n[0] <= 1 || (st[0] - len) / st[1] >= n[1] - 1);
 }
 
+// Rows of `len` bytes that a call reads or writes: n[0] x n[1] of them, st bytes apart.
+struct ByteRows {
+    uintptr_t at;
+    int64_t n[2], st[2], len;
+};
+static ByteRows byte_rows(const pd_tensor* t, int64_t n0, int64_t len, int64_t esz) {
+    const bool two = t->ndim == 3;
+    return {reinterpret_cast<uintptr_t>(t->data), {n0, two ? t->sizes[1] : 1}, {t->strides[0] * esz, two ? t->strides[1] * esz : 0}, len * esz};
+}
+// The first n0 elements or rows of a tensor of one or two dims, its last dim contiguous.
+static ByteRows byte_span(const pd_tensor* t, int64_t n0, int64_t esz) {
+    if (t->ndim == 1) return {reinterpret_cast<uintptr_t>(t->data), {1, 1}, {0, 0}, n0 * esz};
+    return byte_rows(t, n0, t->sizes[1], esz);
+}
+
+// Whether two tensors' rows surely share no byte: their extents are apart, or both repeat with one stride and lie apart in a period
+// of it (heads of one fused buffer, say). Rows of other strides within one another's extent count as overlapping.
+static bool apart(const ByteRows& a, const ByteRows& b) {
+    if (a.n[0] <= 0 || a.n[1] <= 0 || a.len <= 0 || b.n[0] <= 0 || b.n[1] <= 0 || b.len <= 0) return true;
+    auto extent = [](const ByteRows& r) { return (uint64_t)((r.n[0] - 1) * r.st[0] + (r.n[1] - 1) * r.st[1] + r.len); };
+    if (a.at + extent(a) <= b.at || b.at + extent(b) <= a.at) return true;
+    for (int d = 0; d < 2; ++d) {
+        const int o = 1 - d;
+        const int64_t s = a.n[d] > 1 ? a.st[d] : b.st[d];
+        if (s <= 0 || (a.n[d] <= 1 && b.n[d] <= 1) || (a.n[d] > 1 && b.n[d] > 1 && a.st[d] != b.st[d])) continue;
+        // bytes of a period that the rows of the other dim take (those a whole number of periods on fall together)
+        auto width = [&](const ByteRows& r) { return r.n[o] <= 1 || r.st[o] % s == 0 ? r.len : (r.n[o] - 1) * r.st[o] + r.len; };
+        const uint64_t gap = b.at >= a.at ? (b.at - a.at) % (uint64_t)s : ((uint64_t)s - (a.at - b.at) % (uint64_t)s) % (uint64_t)s;
+        if (gap >= (uint64_t)width(a) && gap + (uint64_t)width(b) <= (uint64_t)s) return true;
+    }
+    return false;
+}
+
 int pth_cache_write_rotary(const pd_tensor* query, const pd_tensor* query_out, const pd_tensor* key, const pd_tensor* value,
                            const pd_tensor* positions, const pd_tensor* cos_sin, const pd_tensor* key_cache,
                            const pd_tensor* value_cache, const pd_tensor* k_scale, const pd_tensor* v_scale,
@@ -713,6 +746,11 @@ int pth_cache_write_rotary(const pd_tensor* query, const pd_tensor* query_out, c
     const bool in_place = T > 0 && query_out->data == query->data;  // (all empty tensors are at null)
     if (in_place && !(out_dt == dt && query_out->strides[0] == query->strides[0] && query_out->strides[1] == query->strides[1]))
         return fail(err, errlen, "query_out must be the query itself or not overlap it");
+    const ByteRows written = byte_rows(query_out, T, kDim, osz);
+    if (!in_place && !apart(written, byte_rows(query, T, kDim, esz)))
+        return fail(err, errlen, "query_out must be the query itself or not overlap it");
+    if (!apart(written, byte_rows(key, T, kDim, esz)) || !apart(written, byte_rows(value, T, kDim, esz)))
+        return fail(err, errlen, "query_out must not overlap key or value");
     if (!(positions->dtype == PD_DTYPE_INT64 && positions->ndim == 1 && positions->sizes[0] >= T &&
           (positions->strides[0] == 1 || positions->sizes[0] <= 1)))
         return fail(err, errlen, "positions must be a contiguous int64 [T]");
@@ -844,6 +882,16 @@ int pth_cache_evict(const pd_tensor* weights, const pd_tensor* key_cache, const 
         return fail(err, errlen, "kept must be contiguous int32 [num_seqs, Hkv, keep]");
     if (new_weights->data == weights->data || new_seq_lens->data == seq_lens->data || new_block_table->data == block_table->data)
         return fail(err, errlen, "the new tensors must not be the old ones: eviction copies to other blocks");
+    const ByteRows outs[] = {byte_rows(new_weights, num_seqs, new_weights->sizes[2], 4), byte_rows(kept, num_seqs, keep, 4),
+                             byte_span(new_seq_lens, num_seqs, 4)};
+    const ByteRows ins[] = {byte_rows(weights, num_seqs, weights->sizes[2], 4), byte_span(seq_lens, num_seqs, 4),
+                            byte_span(block_table, num_seqs, 4), byte_span(new_block_table, num_seqs, 4)};
+    for (const ByteRows& x : outs) {
+        for (const ByteRows& y : ins)
+            if (!apart(x, y)) return fail(err, errlen, "the tensors that eviction writes must not overlap those that it reads");
+        for (const ByteRows& y : outs)
+            if (&x != &y && !apart(x, y)) return fail(err, errlen, "the tensors that eviction writes must not overlap");
+    }
     EvictParams p = {};
     p.weights = static_cast<const float*>(weights->data);
     p.w_sb = weights->strides[0];

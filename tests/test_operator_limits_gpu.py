@@ -74,3 +74,30 @@ def test_key_weights_of_rows_without_a_sum_where_scores_are_not_finite():
                         d.query_start_loc, lse, w, d.scale, 2, 2)
     assert torch.equal(w[0], before[0])
     assert bool(torch.isfinite(w[1]).all()) and bool((w[1, :, :21] > before[1, :, :21]).all())
+
+
+def test_outputs_beside_the_inputs_in_one_buffer():
+    T, hq, hkv = 37, 24, 4
+    g = torch.Generator().manual_seed(3)
+    buf = torch.randn((T, 2 * hq + 2 * hkv, 256), generator=g).cuda().bfloat16()
+    before = buf.clone()
+    pos, table = torch.arange(T, device="cuda"), rotary.rotary_table(128, 64, device="cuda")
+    caches = [kvc.allocate_cache(4, 16, hkv, "HND", "cuda") for _ in range(2)]
+    want = torch.empty((T, hq, 256), dtype=torch.bfloat16, device="cuda")
+    for x, c, out in ((before, caches[0], want), (buf, caches[1], buf[:, hq:2 * hq])):
+        pth_dec.rotary_cache_write(x[:, :hq], x[:, 2 * hq:2 * hq + hkv], x[:, 2 * hq + hkv:], pos, table, c.key_cache, c.value_cache,
+                                   c.k_scale, c.v_scale, pos, query_out=out)
+    assert torch.equal(buf[:, hq:2 * hq], want) and torch.equal(buf[:, :hq], before[:, :hq])
+    assert torch.equal(buf[:, 2 * hq:], before[:, 2 * hq:]) and torch.equal(caches[0].kv, caches[1].kv)
+    # sums and kept sums as columns of one tensor
+    c = kvc.allocate_cache(40, 16, 2, "HND", "cuda")
+    lens = torch.tensor([200, 90], dtype=torch.int32, device="cuda")
+    bt = torch.arange(26, dtype=torch.int32, device="cuda").view(2, 13)
+    nbt = torch.arange(26, 34, dtype=torch.int32, device="cuda").view(2, 4)
+    sums = torch.rand((2, 2, 264), generator=g).cuda()
+    outs = []
+    for w, nw in ((sums[..., :200].clone(), torch.empty((2, 2, 64), device="cuda")), (sums[..., :200], sums[..., 200:])):
+        nl, kept = torch.zeros_like(lens), torch.zeros((2, 2, 64), dtype=torch.int32, device="cuda")
+        pth_dec.evict(w, c.key_cache, c.value_cache, c.k_scale, c.v_scale, bt, lens, nbt, nl, nw, kept, 2, 64, 8)
+        outs.append((nl, nw.clone(), kept))
+    assert all(torch.equal(x, y) for x, y in zip(*outs))
