@@ -164,12 +164,19 @@ def decode_splits(nseg: int, window: int, num_kv_heads: int, num_seqs: int, devi
                                     SPLIT_FIXED_US, SPLIT_EMPTY_US, COMBINE_US_PER_MB, PARTIAL_ROW_BYTES)
 
 
+def shared_tables_fit(num_seqs: int, num_kv_heads: int, max_blocks: int, block_size: int) -> bool:
+    """Whether the key tiles that the block tables can hold are as many as decode_shared numbers (pth_dec_decode_shared's limit)."""
+    tiles = max_blocks * block_size // 32 + 16
+    most = (1 << 31) - 1
+    return max_blocks <= most and tiles <= most // 2 and tiles * num_seqs <= most // (2 * num_kv_heads)
+
+
 def shared_prefix(meta, window: int, num_kv_heads: int, num_seqs: int, block_size: int, max_blocks: int, nseg: int) -> int:
     """Keys of the common prefix that a decode batch reads once for all of its sequences (decode_shared), 0: decode reads it for
     each. Where the reads that it spares come to PTH_SHARED_MIN_BYTES; never with a window. (Under graph capture the length
     would stay in the graph, so the routing does not ask then.)"""
     prefix = min(int(getattr(meta, "common_prefix_len", 0) or 0), max_blocks * block_size)
-    if prefix <= 0 or window > 0 or nseg < PTH_SHARED_MIN_NSEG:
+    if prefix <= 0 or window > 0 or nseg < PTH_SHARED_MIN_NSEG or not shared_tables_fit(num_seqs, num_kv_heads, max_blocks, block_size):
         return 0
     return prefix if (num_seqs - 1) * prefix * num_kv_heads * ROW_BYTES >= PTH_SHARED_MIN_BYTES else 0
 
