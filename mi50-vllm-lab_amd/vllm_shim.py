@@ -52,9 +52,11 @@ PTH_DEC_SPLITS = int(os.environ.get("VLLM_GFX950_PTH_DEC_SPLITS", "64"))
 PTH_DEC_CUS = int(os.environ.get("VLLM_GFX950_PTH_DEC_CUS", "0"))  # 0: the device's CU count
 PTH_FA_EXACT = os.environ.get("VLLM_GFX950_PTH_FA_EXACT", "0") == "1"  # prefill through pth_fa_forward_exact
 MAX_ROWS_PER_KV_HEAD = 48  # qmax * G the decode operator takes
-# decode_shared against decode, us, 24 / 4 heads, 50 to 600 own keys: sparing 64 MB of reads 21.3 against 19.9 (16 sequences over
-# 2,048 keys), 23.1 against 22.1 (32 over 1,024); 132 MB 25.2 against 28.3 (32 over 2,048), 34.4 against 32.8 (64 over 1,024); 528 MB (32 over
-# 8,192, 100 to 2,000 own) 37 against 76
+# decode_shared against decode over 461 batches (24 / 4, 12 / 2 and 32 / 8 heads, 1, 2 and 4 query tokens, 2 to 512 sequences, 64 to
+# 32,768 shared and 50 to 4,000 own keys, 40 to 1,200 MB of spared reads): it is taken where both hold, the bytes and the estimated gain (shared_gain_us).
+# It is then at most 8 % slower (256 sequences of 32 / 8 heads over 256 keys 155 us, decode 144) and by more than 2 % in 5 batches; by the
+# bytes alone 21 % (64 sequences x 4 tokens over 1,024 keys 58 and 49) and 30. us: 16 sequences over 4,096 keys, 128 MB spared, 23.0, decode
+# 25.4; 64 over 2,048, 268 MB, 33.8 and 43.9; 32 x 4 tokens over 8,192, 528 MB, 64.6 and 86.0; 128 over 4,096, 1,082 MB, 70.5 and 135.
 PTH_SHARED_MIN_BYTES = 128 << 20
 PTH_SHARED_MIN_NSEG = 4  # segments that decode_shared needs
 
@@ -171,14 +173,31 @@ def shared_tables_fit(num_seqs: int, num_kv_heads: int, max_blocks: int, block_s
     return max_blocks <= most and tiles <= most // 2 and tiles * num_seqs <= most // (2 * num_kv_heads)
 
 
-def shared_prefix(meta, window: int, num_kv_heads: int, num_seqs: int, block_size: int, max_blocks: int, nseg: int) -> int:
+def shared_gain_us(prefix: int, num_kv_heads: int, num_seqs: int, num_tokens: int, num_q_heads: int) -> float:
+    """What decode_shared is estimated to gain over decode, fitted to the batches above: 0.07 us per MB of spared reads, less the prefix's
+    own pass (14 us per 1,000 keys on one workgroup's share of the GPU; 48 workgroups at most take a kv head's 128 rows), less its
+    set-up and partials, and less the slower rows of more than 16 per sequence and kv head."""
+    group = num_q_heads // num_kv_heads
+    spared = (num_seqs - 1) * prefix * num_kv_heads * ROW_BYTES
+    row_tiles = -(-num_tokens * group // 128)
+    own_pass = 14e-3 * prefix * max(1 / 48, num_kv_heads * row_tiles / 256)
+    many = 5.0 if num_tokens * group > 16 * num_seqs else 0.0
+    return 0.07e-6 * spared - own_pass - 8.0 - 0.2e-3 * num_tokens * num_q_heads - many
+
+
+def shared_prefix(meta, window: int, num_kv_heads: int, num_seqs: int, block_size: int, max_blocks: int, nseg: int,
+                  num_tokens: Optional[int] = None, num_q_heads: Optional[int] = None) -> int:
     """Keys of the common prefix that a decode batch reads once for all of its sequences (decode_shared), 0: decode reads it for
-    each. Where the reads that it spares come to PTH_SHARED_MIN_BYTES; never with a window. (Under graph capture the length
-    would stay in the graph, so the routing does not ask then.)"""
+    each. Where the reads that it spares come to PTH_SHARED_MIN_BYTES and more than the batch's rows cost it (shared_gain_us; a token
+    per sequence and 6 q heads per kv head when not given); never with a window. (Under graph capture the length would stay
+    in the graph, so the routing does not ask then.)"""
     prefix = min(int(getattr(meta, "common_prefix_len", 0) or 0), max_blocks * block_size)
     if prefix <= 0 or window > 0 or nseg < PTH_SHARED_MIN_NSEG or not shared_tables_fit(num_seqs, num_kv_heads, max_blocks, block_size):
         return 0
-    return prefix if (num_seqs - 1) * prefix * num_kv_heads * ROW_BYTES >= PTH_SHARED_MIN_BYTES else 0
+    if (num_seqs - 1) * prefix * num_kv_heads * ROW_BYTES < PTH_SHARED_MIN_BYTES:
+        return 0
+    gain = shared_gain_us(prefix, num_kv_heads, num_seqs, num_tokens or num_seqs, num_q_heads or 6 * num_kv_heads)
+    return prefix if gain > 0 else 0
 
 
 def _capturing(device) -> bool:
@@ -305,7 +324,7 @@ class Gfx950Int8Attention:
         batch = (segm_o.shape[2], self.window, self.num_kv_heads, seq_lens.shape[0], query.device, seq_lens_host,
                  max(1, max_q), query.shape[1])
         prefix = shared_prefix(meta, self.window, self.num_kv_heads, seq_lens.shape[0], key_cache.shape[1],
-                               block_table.shape[1], segm_o.shape[2])
+                               block_table.shape[1], segm_o.shape[2], query.shape[0], query.shape[1])
         if prefix and not _capturing(query.device):
             self.pth_dec.decode_shared(query, key_cache, value_cache, k_scale_cache, v_scale_cache, block_table, seq_lens,
                                        query_start_loc, output, self.scale, segm_o, meta.softmax_segm_max,

@@ -33,3 +33,21 @@ def test_the_limit_is_the_entry_s(num_seqs, hkv, bs, blocks):
     rc = pth_dec.load_library().pth_dec_decode_shared(*map(ctypes.byref, d), ctypes.c_double(0.1), *map(ctypes.byref, tail), None, num_seqs, 3,
                                                       0, None, None, 0)
     assert rc in (0, 1) and (rc == 0) == shim.shared_tables_fit(num_seqs, hkv, blocks, bs)
+
+
+# batches measured on an MI355X (sequences, query tokens each, shared keys, q and kv heads)
+FASTER_SHARED = [(16, 1, 8192, 24, 4), (32, 1, 4096, 24, 4), (64, 1, 2048, 24, 4), (128, 1, 2048, 24, 4), (8, 1, 16384, 24, 4), (32, 2, 8192, 24, 4),
+                 (32, 4, 8192, 24, 4), (64, 1, 4096, 12, 2), (512, 1, 1024, 24, 4)]
+FASTER_DECODE = [(64, 4, 1024, 24, 4), (64, 4, 2048, 24, 4), (8, 2, 32768, 12, 2), (8, 4, 16384, 24, 4), (4, 1, 32768, 24, 4), (4, 2, 32768, 24, 4),
+                 (16, 1, 2048, 24, 4), (64, 2, 1024, 24, 4)]
+
+
+@pytest.mark.parametrize("seqs,ql,prefix,hq,hkv", FASTER_SHARED + FASTER_DECODE)
+def test_the_faster_operator_takes_the_batch(seqs, ql, prefix, hq, hkv):
+    got = shim.shared_prefix(Meta(prefix), -1, hkv, seqs, 16, 4096, 64, seqs * ql, hq)
+    assert got == (prefix if (seqs, ql, prefix, hq, hkv) in FASTER_SHARED else 0)
+
+
+def test_the_route_counts_the_batch_s_rows(monkeypatch):
+    # 268 MB are spared either way; four tokens per sequence cost more than that gains
+    assert run(monkeypatch, 2048, seqs=64)[0] == "shared" and run(monkeypatch, 2048, seqs=64, qlen=4)[0] == "decode"
