@@ -327,11 +327,13 @@ int pth_cache_key_weights(const pd_tensor* q, const pd_tensor* key_cache, const 
  * Eviction by running weights: per sequence and kv head the last `recent` keys and the keep - recent others with the
  * largest weights stay (equal weights: the lowest key; NaN counts as the largest), in the order of their positions. Their
  * rows are copied into the blocks of new_block_table; the old blocks are left as they are. No counterpart in the reference.
- *   weights      fp32 [>= num_seqs, Hkv, keys <= 2^28]; keys of a sequence past `keys` or past its block table are dropped
+ *   weights      fp32 [>= num_seqs, Hkv, keys <= 2^28]. A sequence is taken to end where its weights or its block table do: n =
+ *                min(seq_len, keys, keys of the table), and its keys behind n, the newest ones, are dropped. `keys` must hold
+ *                the longest sequence for `recent` to be its last keys
  *   block_table, seq_lens   int32, the batch before; sequences of at most keep keys are copied whole
  *   new_block_table         int32 [>= num_seqs, columns for keep keys]: blocks that no table row of the call reads
- *                           and no two of its rows share, in the part that holds a sequence's min(seq_len, keep) keys
- *   new_seq_lens            int32 [>= num_seqs], written: min(seq_len, keep)
+ *                           and no two of its rows share, in the part that holds a sequence's min(n, keep) keys
+ *   new_seq_lens            int32 [>= num_seqs], written: min(n, keep)
  *   new_weights             fp32 [>= num_seqs, Hkv, >= keep], written: the kept keys' weights, then zeros
  *   kept                    int32, contiguous [>= num_seqs, Hkv, keep], written: the kept keys' numbers, then -1
  *   keep, recent            1 <= keep <= 2^28, 0 <= recent <= keep

@@ -430,7 +430,7 @@ def key_weights(q: torch.Tensor, key_cache: torch.Tensor, value_cache: torch.Ten
 
     The arguments up to query_start_loc, scale, num_seqs and qmax are decode's, of a causal step without window; lse
     [>= T, Hq] is what decode(..., lse=) or decode_shared(..., lse=) stored for it. Keys past the last column of weights are
-    not counted. evict keeps the keys with the largest sums.
+    not counted (and evict would drop them). evict keeps the keys with the largest sums.
     """
     native().key_weights(_entry("pth_cache_key_weights"), q, key_cache, value_cache, k_scale, v_scale, block_table, seq_lens,
                          query_start_loc, lse, weights, scale, int(num_seqs), int(qmax))
@@ -444,7 +444,9 @@ def evict(weights: torch.Tensor, key_cache: torch.Tensor, value_cache: torch.Ten
 
     The kept rows are copied into the blocks of new_block_table (int32 [>= num_seqs, columns for keep keys]), which must not
     be among those that the call reads; the old blocks stay as they are, also where other sequences share
-    them, and are free once the call is done. Written: new_seq_lens (int32, min(seq_len, keep)), new_weights (fp32
+    them, and are free once the call is done. weights (fp32 [>= num_seqs, Hkv, keys]) must have a column for every key of the
+    longest sequence: one longer than `keys` (or than its block table) is cut to its first `keys` keys before the choice, so its
+    newest ones go. Written: new_seq_lens (int32, min(seq_len, keys, keep)), new_weights (fp32
     [>= num_seqs, Hkv, >= keep]: the kept keys' sums, then zeros, as key_weights goes on with them) and kept (int32 [>=
     num_seqs, Hkv, keep]: their numbers, then -1). Sequences of at most keep keys are copied whole. The keys stay rotated
     by their own positions; tokens written later go on counting from the sequence's full length.
