@@ -13,9 +13,9 @@
 // CU 4 waves x kPer x its instructions on each SIMD: keys of weight 0, which sums that no row has added to
 // share, and lanes that agree on a part do not queue for one counter.
 //
-// What bounds it, us: 8 sequences of up to 8,192 keys (4 kv heads, 2,048 kept) select 7.3 to 8.7, latency of its passes, and copy 9.6, 68 MB
-// at 7 TB/s from and to caches; one of 61,440 (2 heads, 8,192 kept) select 31, the instructions of the one CU that a row
-// has, and copy 5.5.
+// What bounds it, us: 8 sequences of 1,000 to 6,000 keys (4 kv heads, 2,048 kept) select 7.3 to 8.7, latency of its passes, and copy 9.6, 68 MB
+// at 7 TB/s from and to caches; one of 61,440 (2 heads, 8,000 kept) select 32, the instructions of the one CU that a row
+// has, and copy 6. One of 131,072, read again in every pass, 83 in all (16,000 kept: 87).
 #include "pd_tile.hpp"
 #include "pth_dec.h"
 
@@ -263,7 +263,7 @@ __global__ void __launch_bounds__(256) pd_evict_copy_kernel(const EvictParams a)
 // host side
 
 hipError_t launch_evict(const EvictParams& p, int num_seqs, hipStream_t stream) {
-    // registers for the longest row that the table and the weights can hold: sequences of up to 8,192 keys, both launches, 19.0 us with 8
+    // registers for the longest row that the table and the weights can hold: sequences of up to 6,000 keys, both launches, 19.0 us with 8
     // a lane, 20.6 with 24, 24.8 with 64; one of 61,440 keys 37.3 with 64 and 45.7 read again in every pass
     const dim3 rows(p.Hkv, num_seqs), block(kEvThreads);
     if (p.max_keys <= 8 * kEvThreads)

@@ -15,7 +15,8 @@
 // head in place touches only its rotated octets.
 //
 // What bounds it: small calls a trip to memory for positions and slots and one for the rows (2.8 us at 1 token, 3.8 at 129); large ones
-// memory, 32,768 fp16 tokens of 12 / 2 heads 115 us for 537 MB, 4.7 TB/s.
+// memory, 32,768 fp16 tokens of 12 / 2 heads 113 us for 537 MB, 4.7 TB/s; bf16 109, fp32 into fp32 190 for 1,008 MB, 5.3 TB/s (24 / 4 heads
+// 203, 201 and 364).
 #include "pd_quant.hpp"
 #include "pth_dec.h"
 

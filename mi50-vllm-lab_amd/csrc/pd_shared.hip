@@ -19,11 +19,11 @@
 // size (2.9e-4 against 64 bits, 2-norm, where that rounding alone makes 2.1e-4). The 16 more MFMAs per row block, of 48 a
 // tile, cost 19 % of the largest batch (128 sequences over 61,440 keys 254 us without, 303 with) and nothing where memory or set-up bounds.
 //
-// What bounds it (gfx950, both launches, us; 24 / 4 heads unless said): 128 sequences of 64 to 2,048 keys behind 61,440 shared ones 254,
-// of which the prefix, bound by MFMA and the 32-bit arithmetic beside it, takes 225 alone (45 % of the MFMA rate of a large
-// matrix product), and the own keys 60 (4.7 TB/s: bound by memory); a CU streams at most 20 bytes a ns, so the deal counts
-// 1 us for an own tile and both kinds of work finish together. 32 sequences over 8,192: 38, 12 of them set-up of the pieces, their
-// partials (12 MB) and the join. 4 over 2,048: 13.5, five dependent trips to memory and a second launch.
+// What bounds it (gfx950, both launches, us; 24 / 4 heads unless said): 128 sequences of 64 to 2,048 keys behind 61,440 shared ones 303.
+// The prefix alone takes 265 and its join 14: with both terms of P' 1,090 TFLOP/s of MFMAs, 94 % of the rate of a large matrix
+// product. The own keys alone take 65 (4.7 TB/s: bound by memory); a CU streams at most 20 bytes a ns, so the deal counts
+// 1 us for an own tile and both kinds of work finish together. 32 sequences over 8,192: 37, 12 of them set-up of the pieces, their
+// partials (12 MB) and the join. 4 over 2,048: 13.4, five dependent trips to memory and a second launch.
 #include "pd_shared_body.hpp"
 #include "pth_dec.h"
 

@@ -2,14 +2,14 @@
 // per SIMD, in KW key groups of RW row groups: wave (k, r) takes every KW-th tile of the run for RB blocks of 16 rows, and the
 // key groups' states are merged through LDS at the end. A wave holds Q and O of its rows in registers; S^T = K Q^T leaves a lane
 // the weights that it needs as an operand of O^T += V^T P^T, so nothing is exchanged between waves in a tile and a row's
-// running max belongs to one wave. Per tile a wave has 32 RB MFMAs for the scores, as many for each term of P', a softmax
+// running max belongs to one wave. Per tile a wave has 16 RB MFMAs for the scores, as many for each term of P', a softmax
 // of 8 RB scores per lane, and the widening of int8 to fp16 operands (256 conversions for all of a tile), which is what the three forms
 // treat differently:
 //   RW = 8  (the prefix) each wave widens an eighth of the tile into operands in LDS, a tile ahead, and all read them: 32 conversions
 //           and 32 reads of 1 KiB. The two waves of a SIMD do so before and behind their products, so that one converts while
-//           the other multiplies. With every wave widening all of it for itself a tile of 256 rows took 2.9 us instead
-//           of 1.95 (VALU busy 61 % and MFMA 31 % of the time, nothing of it at once); with the scores' keys and the values' dims
-//           split over the waves and P' exchanged through LDS, 2.9 for 256 rows too (two tiles of 128).
+//           the other multiplies. A tile of 256 rows takes 2.4 us (2.0 with one term of P'; then 2.9 with every wave widening all
+//           of it for itself, VALU busy 61 % and MFMA 31 % of the time, nothing of it at once, and 2.9, two tiles of 128, with the
+//           scores' keys and the values' dims split over the waves and P' exchanged through LDS).
 //   RW = 1  (own keys, <= 16 rows) a wave's tiles are its own: no barrier, every byte is widened once, K goes straight to
 //           registers, as its operands lie as the rows do.
 //   RW = 4  (own keys, up to 48 rows) as RW = 1 on tiles in LDS that four waves share; 7 sequences of 3 x 6 rows 20.0 us, with two row
