@@ -347,6 +347,63 @@ int pth_cache_evict(const pd_tensor* weights, const pd_tensor* key_cache, const 
               const pd_tensor* new_weights, const pd_tensor* kept, int64_t num_seqs, int64_t keep, int64_t recent,
               hipStream_t stream, char* err, int errlen);
 
+/*
+ * pth_cache_write_rotary with the norms that a model applies to its query and key heads before the rotation: every head x of
+ * query and key is x / sqrt(mean(x^2) + eps) * (weight + weight_offset) first, in fp32. No counterpart in the reference.
+ *   query_weight, key_weight   contiguous [256], both fp32 or both of the query's dtype, aligned to 4 elements
+ *   eps, weight_offset         eps >= 0
+ * The other arguments are pth_cache_write_rotary's; query_out must not overlap the weights either. In place the whole query
+ * is written. Returns 0, 1 or 2 as above.
+ */
+int pth_cache_write_norm_rotary(const pd_tensor* query, const pd_tensor* query_out, const pd_tensor* key,
+                                const pd_tensor* value, const pd_tensor* query_weight, const pd_tensor* key_weight,
+                                double eps, double weight_offset, const pd_tensor* positions, const pd_tensor* cos_sin,
+                                const pd_tensor* key_cache, const pd_tensor* value_cache, const pd_tensor* k_scale,
+                                const pd_tensor* v_scale, const pd_tensor* slot_mapping, int64_t interleaved,
+                                hipStream_t stream, char* err, int errlen);
+
+/*
+ * Block tables and reference counts on the device. No counterpart in the reference, whose engine keeps them on the host.
+ *   caches       `layers` (1..128) raw caches, int8 [pages <= 2^22, Hkv, block_size, 520], of the same sizes and strides, their rows
+ *                8-byte aligned and apart; page numbers are those of all of them
+ *   refs         int32 [pages], how many table entries name each page; 0 (or less): the page is free
+ *   block_table  int32 [B, columns], an entry outside [0, pages) names no page
+ *   workspace    int32, 16-byte aligned, of pth_cache_pages_workspace(pages, B, N) (0, 0 for compact); its contents need not be
+ *                kept between calls, and calls that may overlap in time need one each
+ *
+ * pth_cache_fork_pages: row i of the new tables goes on from row p = parents[i] (null: i) of n = seq_lens[p] keys. Of
+ * its columns below ceil((n + grow) / block_size), those of full pages keep p's entry, or become -1 if window > 0 and all keys of the
+ * page lie at or past `sinks` and before n + 1 - window; each other column keeps p's entry if the row is the first child
+ * of p and the page's count is 1, else it takes a free page (the lowest of those free before the call, in the order of row and
+ * column), and the keys below n that p has there are copied for all caches. All further columns become -1. The old rows'
+ * references are dropped, the new rows' counted.
+ *   seq_lens     int32 [B] (less than 0 counts as 0); parents int32 [N] or null; a parent outside [0, B): an empty row of length 0
+ *   new_refs     int32 [pages]: refs itself, or apart from it
+ *   new_block_table, new_seq_lens   int32 [N, columns] and [N]: apart from the old ones, without parents also the old ones
+ *                themselves
+ *   needed       int32 [1], written: the pages wanted. Where more than were free, the last columns that wanted one are -1
+ *   grow, sinks  >= 0; window <= 0: none
+ * At most 8,192 rows in either table.
+ *
+ * pth_cache_compact_pages: of n used pages, those numbered n or above move, in order, into the free ones below n, for all caches.
+ *   new_refs, new_block_table   as above, each the old one or apart from it; an entry that names no used page becomes -1
+ *   places       int32 [pages], written: where each page lies now, -1 for a free one
+ *   used         int32 [1], written: n
+ *
+ * The tensors that are written overlap neither each other nor those that are read, but for what is said above. No results depend
+ * on the order in which the device works. Both return 0, 1 or 2 as above.
+ */
+int pth_cache_fork_pages(const pd_tensor* caches, int64_t layers, const pd_tensor* refs, const pd_tensor* block_table,
+                         const pd_tensor* seq_lens, const pd_tensor* parents, const pd_tensor* new_refs,
+                         const pd_tensor* new_block_table, const pd_tensor* new_seq_lens, const pd_tensor* needed,
+                         const pd_tensor* workspace, int64_t grow, int64_t window, int64_t sinks, hipStream_t stream,
+                         char* err, int errlen);
+int pth_cache_compact_pages(const pd_tensor* caches, int64_t layers, const pd_tensor* refs, const pd_tensor* block_table,
+                            const pd_tensor* new_refs, const pd_tensor* new_block_table, const pd_tensor* places,
+                            const pd_tensor* used, const pd_tensor* workspace, hipStream_t stream, char* err, int errlen);
+/* Workspace int32s of the above for caches of `pages` pages and tables of `rows` old and `new_rows` new rows; 0 if out of range. */
+int64_t pth_cache_pages_workspace(int64_t pages, int64_t rows, int64_t new_rows);
+
 #ifdef __cplusplus
 }
 #endif

@@ -714,10 +714,17 @@ static bool apart(const ByteRows& a, const ByteRows& b) {
     return false;
 }
 
-int pth_cache_write_rotary(const pd_tensor* query, const pd_tensor* query_out, const pd_tensor* key, const pd_tensor* value,
-                           const pd_tensor* positions, const pd_tensor* cos_sin, const pd_tensor* key_cache,
-                           const pd_tensor* value_cache, const pd_tensor* k_scale, const pd_tensor* v_scale,
-                           const pd_tensor* slot_mapping, int64_t interleaved, hipStream_t stream, char* err, int errlen) {
+// The norms of a rotary write's query and key heads.
+struct HeadNorms {
+    const pd_tensor *q_weight, *k_weight;
+    double eps, offset;
+};
+
+static int rotary_entry(const pd_tensor* query, const pd_tensor* query_out, const pd_tensor* key, const pd_tensor* value,
+                        const pd_tensor* positions, const pd_tensor* cos_sin, const pd_tensor* key_cache,
+                        const pd_tensor* value_cache, const pd_tensor* k_scale, const pd_tensor* v_scale,
+                        const pd_tensor* slot_mapping, int64_t interleaved, hipStream_t stream, char* err, int errlen,
+                        const HeadNorms* norms = nullptr) {
     if (!query || !query_out || !key || !value || !positions || !cos_sin || !key_cache || !value_cache || !k_scale ||
         !v_scale || !slot_mapping)
         return fail(err, errlen, "null tensor descriptor");
@@ -757,6 +764,18 @@ int pth_cache_write_rotary(const pd_tensor* query, const pd_tensor* query_out, c
     if (!(slot_mapping->dtype == PD_DTYPE_INT64 && slot_mapping->ndim == 1 && slot_mapping->sizes[0] >= T &&
           (slot_mapping->strides[0] == 1 || slot_mapping->sizes[0] <= 1)))
         return fail(err, errlen, "slot_mapping must be a contiguous int64 [T]");
+    if (norms) {
+        for (const pd_tensor* w : {norms->q_weight, norms->k_weight}) {
+            if (!((w->dtype == dt || w->dtype == PD_DTYPE_FP32) && w->dtype == norms->q_weight->dtype && w->ndim == 1 &&
+                  w->sizes[0] == kDim && w->strides[0] == 1 &&
+                  reinterpret_cast<uintptr_t>(w->data) % (w->dtype == PD_DTYPE_FP32 ? 16 : 8) == 0))
+                return fail(err, errlen, "query_weight and key_weight must be contiguous [256] of one dtype, the query's or fp32, aligned to 4 elements");
+            if (!apart(written, byte_span(w, kDim, w->dtype == PD_DTYPE_FP32 ? 4 : 2)))
+                return fail(err, errlen, "query_out must not overlap the weights");
+        }
+        if (!(norms->eps >= 0 && norms->eps < 1e30 && norms->offset > -1e30 && norms->offset < 1e30))
+            return fail(err, errlen, "eps must be at least 0 and finite, weight_offset finite");
+    }
     const int64_t rd = cos_sin->ndim == 2 ? cos_sin->sizes[1] : 0;
     if (!(cos_sin->dtype == PD_DTYPE_FP32 && cos_sin->ndim == 2 && rd >= 8 && rd <= kDim && rd % 8 == 0 &&
           cos_sin->strides[1] == 1 && cos_sin->strides[0] % 4 == 0 && reinterpret_cast<uintptr_t>(cos_sin->data) % 16 == 0))
@@ -792,7 +811,33 @@ int pth_cache_write_rotary(const pd_tensor* query, const pd_tensor* query_out, c
     p.rotary_dim = (int)rd;
     p.interleaved = interleaved != 0;
     p.in_place = in_place;
+    if (norms) {
+        p.q_weight = norms->q_weight->data;
+        p.k_weight = norms->k_weight->data;
+        p.weight_fp32 = norms->q_weight->dtype == PD_DTYPE_FP32;
+        p.eps = (float)norms->eps;
+        p.weight_offset = (float)norms->offset;
+    }
     return op_result(launch_rotary_write(p, dt, out_dt, stream), "rotary cache write", err, errlen);
+}
+
+int pth_cache_write_rotary(const pd_tensor* query, const pd_tensor* query_out, const pd_tensor* key, const pd_tensor* value,
+                           const pd_tensor* positions, const pd_tensor* cos_sin, const pd_tensor* key_cache,
+                           const pd_tensor* value_cache, const pd_tensor* k_scale, const pd_tensor* v_scale,
+                           const pd_tensor* slot_mapping, int64_t interleaved, hipStream_t stream, char* err, int errlen) {
+    return rotary_entry(query, query_out, key, value, positions, cos_sin, key_cache, value_cache, k_scale, v_scale, slot_mapping,
+                        interleaved, stream, err, errlen);
+}
+
+int pth_cache_write_norm_rotary(const pd_tensor* query, const pd_tensor* query_out, const pd_tensor* key, const pd_tensor* value,
+                                const pd_tensor* query_weight, const pd_tensor* key_weight, double eps, double weight_offset,
+                                const pd_tensor* positions, const pd_tensor* cos_sin, const pd_tensor* key_cache,
+                                const pd_tensor* value_cache, const pd_tensor* k_scale, const pd_tensor* v_scale,
+                                const pd_tensor* slot_mapping, int64_t interleaved, hipStream_t stream, char* err, int errlen) {
+    if (!query_weight || !key_weight) return fail(err, errlen, "null tensor descriptor");
+    const HeadNorms norms = {query_weight, key_weight, eps, weight_offset};
+    return rotary_entry(query, query_out, key, value, positions, cos_sin, key_cache, value_cache, k_scale, v_scale, slot_mapping,
+                        interleaved, stream, err, errlen, &norms);
 }
 
 // The batch of a decode step as the weights and the eviction take it.
@@ -917,6 +962,197 @@ int pth_cache_evict(const pd_tensor* weights, const pd_tensor* key_cache, const 
     p.keep = (int)keep;
     p.recent = (int)recent;
     return op_result(launch_evict(p, (int)num_seqs, stream), "evict", err, errlen);
+}
+
+// Whether the rows of a raw cache [pages, Hkv, keys, 520] are apart: in the order of the strides, each spans the dims below it.
+static bool cache_rows_apart(const pd_tensor* kv) {
+    int order[3] = {0, 1, 2};
+    std::sort(order, order + 3, [&](int a, int b) {
+        return kv->strides[a] != kv->strides[b] ? kv->strides[a] < kv->strides[b] : kv->sizes[a] < kv->sizes[b];
+    });
+    int64_t span = kRowBytes;
+    for (int d : order) {
+        if (kv->sizes[d] <= 1) continue;
+        if (kv->strides[d] < span || kv->strides[d] > INT64_MAX / 4 / kv->sizes[d]) return false;
+        span = kv->strides[d] * (kv->sizes[d] - 1) + span;
+    }
+    return true;
+}
+
+// The caches and the table rows that a page operator takes; null, or why not.
+static const char* page_caches(const pd_tensor* caches, int64_t layers, PageCaches& k) {
+    if (!(layers >= 1 && layers <= kMaxPageLayers)) return "1 to 128 caches per call";
+    for (int64_t i = 0; i < layers; ++i) {
+        const pd_tensor& c = caches[i];
+        if (!(c.dtype == PD_DTYPE_INT8 && c.ndim == 4 && c.sizes[3] == kRowBytes && c.strides[3] == 1 &&
+              reinterpret_cast<uintptr_t>(c.data) % 8 == 0))
+            return "caches must be int8 [pages, Hkv, block_size, 520] with contiguous, 8-byte aligned rows";
+        for (int d = 0; d < 3; ++d) {
+            if (c.strides[d] % 8 != 0) return "caches must be int8 [pages, Hkv, block_size, 520] with contiguous, 8-byte aligned rows";
+            if (c.sizes[d] != caches[0].sizes[d] || c.strides[d] != caches[0].strides[d])
+                return "the caches of a call must have the same sizes and strides";
+        }
+        k.kv[i] = static_cast<int8_t*>(const_cast<void*>(c.data));
+    }
+    const pd_tensor& c = caches[0];
+    if (!(c.sizes[0] >= 1 && c.sizes[0] <= kMaxPages && c.sizes[1] >= 1 && c.sizes[1] <= (1 << 20) && c.sizes[2] >= 1 &&
+          c.sizes[2] <= (1 << 20) && c.sizes[1] * c.sizes[2] <= (1 << 20)))
+        return "caches of 1 to 2^22 pages of 1 to 2^20 rows";
+    if (!cache_rows_apart(&c)) return "cache rows must not overlap";
+    k.sb = c.strides[0];
+    k.sh = c.strides[1];
+    k.ss = c.strides[2];
+    k.layers = (int)layers;
+    k.Hkv = (int)c.sizes[1];
+    k.block_size = (int)c.sizes[2];
+    return nullptr;
+}
+static bool page_table_rows(const pd_tensor* t, int64_t most) {
+    return t->dtype == PD_DTYPE_INT32 && t->ndim == 2 && (t->strides[1] == 1 || t->sizes[1] <= 1) && t->sizes[0] <= most &&
+           t->sizes[1] <= INT32_MAX / 2;
+}
+static bool table_rows_apart(const pd_tensor* t) { return t->sizes[0] <= 1 || t->strides[0] >= t->sizes[1]; }
+// Workspace ints: both masks, the counts, and for a fork the rows' plans.
+static int64_t page_work_ints(int64_t pages, int64_t rows, int64_t new_rows) {
+    const int64_t chunks = (pages + 1023) / 1024;
+    return chunks * (2 * 32 + 1) + rows + 3 * new_rows + 1;
+}
+static const char* page_work(const pd_tensor* ws, int64_t pages, int64_t ints, PageWork& w) {
+    if (!(ws->dtype == PD_DTYPE_INT32 && ws->ndim == 1 && is_contig(ws) && ws->sizes[0] >= ints &&
+          reinterpret_cast<uintptr_t>(ws->data) % 16 == 0))
+        return "workspace must be contiguous 16-byte aligned int32 of pth_cache_pages_workspace";
+    w.pages = (int)pages;
+    w.chunks = (int)((pages + 1023) / 1024);
+    w.free_mask = static_cast<unsigned long long*>(const_cast<void*>(ws->data));
+    w.alone_mask = w.free_mask + 16 * w.chunks;
+    w.counts = reinterpret_cast<int*>(w.alone_mask + 16 * w.chunks);
+    return nullptr;
+}
+// Whether an output is the input itself (data and strides) or apart from it.
+static bool same_or_apart(const pd_tensor* out, const pd_tensor* in, int64_t n_out, int64_t n_in, bool may_be_same) {
+    const bool same = out->data == in->data && out->ndim == in->ndim && (out->ndim == 1 || (out->strides[0] == in->strides[0] &&
+                      out->sizes[1] == in->sizes[1]));
+    return (same && may_be_same) || apart(byte_span(out, n_out, 4), byte_span(in, n_in, 4));
+}
+
+int64_t pth_cache_pages_workspace(int64_t pages, int64_t rows, int64_t new_rows) {
+    if (pages < 1 || pages > kMaxPages || rows < 0 || rows > INT32_MAX || new_rows < 0 || new_rows > INT32_MAX) return 0;
+    return page_work_ints(pages, rows, new_rows);
+}
+
+int pth_cache_fork_pages(const pd_tensor* caches, int64_t layers, const pd_tensor* refs, const pd_tensor* block_table,
+                         const pd_tensor* seq_lens, const pd_tensor* parents, const pd_tensor* new_refs,
+                         const pd_tensor* new_block_table, const pd_tensor* new_seq_lens, const pd_tensor* needed,
+                         const pd_tensor* workspace, int64_t grow, int64_t window, int64_t sinks, hipStream_t stream, char* err,
+                         int errlen) {
+    if (!caches || !refs || !block_table || !seq_lens || !new_refs || !new_block_table || !new_seq_lens || !needed || !workspace)
+        return fail(err, errlen, "null tensor descriptor");
+    ForkParams p = {};
+    PageCaches k = {};
+    if (const char* why = page_caches(caches, layers, k)) return fail(err, errlen, why);
+    const int64_t pages = caches[0].sizes[0];
+    if (!(int_rows(refs, pages) && refs->sizes[0] == pages && int_rows(new_refs, pages) && new_refs->sizes[0] == pages))
+        return fail(err, errlen, "refs and new_refs must be contiguous int32 with an entry for each page");
+    if (!(page_table_rows(block_table, kMaxForkRows) && page_table_rows(new_block_table, kMaxForkRows) &&
+          new_block_table->sizes[1] == block_table->sizes[1]))
+        return fail(err, errlen, "block tables must be int32 of at most 8192 rows, with the same columns");
+    const int64_t B = block_table->sizes[0], N = new_block_table->sizes[0];
+    if (!(int_rows(seq_lens, B) && int_rows(new_seq_lens, N))) return fail(err, errlen, "sequence lengths must be contiguous int32 with an entry for each row");
+    if (parents ? !int_rows(parents, N) : N != B)
+        return fail(err, errlen, "parents must be contiguous int32 with an entry for each new row (none: as many new rows as old)");
+    if (!int_rows(needed, 1)) return fail(err, errlen, "needed must be int32 [1]");
+    if (!(grow >= 0 && grow <= INT32_MAX && window >= INT32_MIN && window <= INT32_MAX && sinks >= 0 && sinks <= INT32_MAX))
+        return fail(err, errlen, "grow and sinks must be at least 0 and, like window, fit in 32 bits");
+    if (!table_rows_apart(new_block_table)) return fail(err, errlen, "new_block_table rows must not overlap");
+    const bool keeps = parents == nullptr;  // a row's entry then depends on nothing but itself
+    if (!(same_or_apart(new_refs, refs, pages, pages, true) && same_or_apart(new_block_table, block_table, N, B, keeps) &&
+          same_or_apart(new_seq_lens, seq_lens, N, B, keeps)))
+        return fail(err, errlen, keeps ? "the new tensors must be the old ones or not overlap them"
+                                       : "new_refs must be refs or not overlap it; with parents the other new tensors must not overlap the old ones");
+    if (const char* why = page_work(workspace, pages, page_work_ints(pages, B, N), p.w)) return fail(err, errlen, why);
+    {
+        const ByteRows outs[] = {byte_span(new_refs, pages, 4), byte_span(new_block_table, N, 4), byte_span(new_seq_lens, N, 4),
+                                 byte_span(needed, 1, 4), byte_span(workspace, workspace->sizes[0], 4)};
+        const ByteRows ins[] = {byte_span(refs, pages, 4), byte_span(block_table, B, 4), byte_span(seq_lens, B, 4)};
+        for (int i = 0; i < 5; ++i) {
+            for (int j = 0; j < 5; ++j)
+                if (i != j && !apart(outs[i], outs[j])) return fail(err, errlen, "the tensors that are written must not overlap");
+            for (int j = 0; j < 3; ++j)
+                if (i != j && !apart(outs[i], ins[j])) return fail(err, errlen, "the tensors that are written must not overlap those that are read");
+            if (parents && !apart(outs[i], byte_span(parents, N, 4)))
+                return fail(err, errlen, "the tensors that are written must not overlap those that are read");
+        }
+    }
+    p.refs = static_cast<const int*>(refs->data);
+    p.new_refs = static_cast<int*>(const_cast<void*>(new_refs->data));
+    p.table = static_cast<const int*>(block_table->data);
+    p.t_st = block_table->strides[0];
+    p.new_table = static_cast<int*>(const_cast<void*>(new_block_table->data));
+    p.n_st = new_block_table->strides[0];
+    p.seq_lens = static_cast<const int*>(seq_lens->data);
+    p.new_lens = static_cast<int*>(const_cast<void*>(new_seq_lens->data));
+    // (no new rows: an empty tensor has no data, but that all old rows end is said by its not being null)
+    p.parents = parents ? static_cast<const int*>(N > 0 ? parents->data : refs->data) : nullptr;
+    p.needed = static_cast<int*>(const_cast<void*>(needed->data));
+    p.rows = (int)B;
+    p.new_rows = (int)N;
+    p.cols = (int)block_table->sizes[1];
+    p.block_size = k.block_size;
+    p.grow = grow;
+    p.window = window;
+    p.sinks = sinks;
+    p.eldest = p.w.counts + p.w.chunks;
+    p.first_taken = p.eldest + B;
+    p.copy_row = p.first_taken + N;
+    p.copy_from = p.copy_row + N;
+    p.copies = p.copy_from + N;
+    return op_result(launch_fork(p, k, stream), "fork pages", err, errlen);
+}
+
+int pth_cache_compact_pages(const pd_tensor* caches, int64_t layers, const pd_tensor* refs, const pd_tensor* block_table,
+                            const pd_tensor* new_refs, const pd_tensor* new_block_table, const pd_tensor* places,
+                            const pd_tensor* used, const pd_tensor* workspace, hipStream_t stream, char* err, int errlen) {
+    if (!caches || !refs || !block_table || !new_refs || !new_block_table || !places || !used || !workspace)
+        return fail(err, errlen, "null tensor descriptor");
+    CompactParams p = {};
+    PageCaches k = {};
+    if (const char* why = page_caches(caches, layers, k)) return fail(err, errlen, why);
+    const int64_t pages = caches[0].sizes[0];
+    if (!(int_rows(refs, pages) && refs->sizes[0] == pages && int_rows(new_refs, pages) && new_refs->sizes[0] == pages &&
+          int_rows(places, pages) && places->sizes[0] == pages))
+        return fail(err, errlen, "refs, new_refs and places must be contiguous int32 with an entry for each page");
+    const int64_t B = block_table->sizes[0];
+    if (!(page_table_rows(block_table, 1 << 20) && page_table_rows(new_block_table, 1 << 20) && new_block_table->sizes[0] == B &&
+          new_block_table->sizes[1] == block_table->sizes[1]))
+        return fail(err, errlen, "block tables must be int32 of at most 2^20 rows, with the same rows and columns");
+    if (!int_rows(used, 1)) return fail(err, errlen, "used must be int32 [1]");
+    if (!table_rows_apart(new_block_table)) return fail(err, errlen, "new_block_table rows must not overlap");
+    if (!(same_or_apart(new_refs, refs, pages, pages, true) && same_or_apart(new_block_table, block_table, B, B, true)))
+        return fail(err, errlen, "the new tensors must be the old ones or not overlap them");
+    if (const char* why = page_work(workspace, pages, page_work_ints(pages, 0, 0), p.w)) return fail(err, errlen, why);
+    {
+        const ByteRows outs[] = {byte_span(new_refs, pages, 4), byte_span(new_block_table, B, 4), byte_span(places, pages, 4),
+                                 byte_span(used, 1, 4), byte_span(workspace, workspace->sizes[0], 4)};
+        const ByteRows ins[] = {byte_span(refs, pages, 4), byte_span(block_table, B, 4)};
+        for (int i = 0; i < 5; ++i) {
+            for (int j = 0; j < 5; ++j)
+                if (i != j && !apart(outs[i], outs[j])) return fail(err, errlen, "the tensors that are written must not overlap");
+            for (int j = 0; j < 2; ++j)
+                if (i != j && !apart(outs[i], ins[j])) return fail(err, errlen, "the tensors that are written must not overlap those that are read");
+        }
+    }
+    p.refs = static_cast<const int*>(refs->data);
+    p.new_refs = static_cast<int*>(const_cast<void*>(new_refs->data));
+    p.table = static_cast<const int*>(block_table->data);
+    p.t_st = block_table->strides[0];
+    p.new_table = static_cast<int*>(const_cast<void*>(new_block_table->data));
+    p.n_st = new_block_table->strides[0];
+    p.places = static_cast<int*>(const_cast<void*>(places->data));
+    p.used = static_cast<int*>(const_cast<void*>(used->data));
+    p.rows = (int)B;
+    p.cols = (int)block_table->sizes[1];
+    p.block_size = k.block_size;
+    return op_result(launch_compact(p, k, stream), "compact pages", err, errlen);
 }
 
 const char* pth_dec_version(void) { return "pth_dec-gfx950 0.2"; }

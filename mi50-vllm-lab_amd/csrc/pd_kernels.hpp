@@ -1,6 +1,6 @@
 // Internal interface of libpthdec.so between the C ABI (pd_api.hip) and the kernel files
 // (pd_decode.hip, pd_prefill.hip, pd_prefill_wide.hip, pd_cache_write.hip, pd_rotary_write.hip, pd_key_weights.hip,
-// pd_evict.hip, pd_shared.hip): the parameter block each kernel takes and
+// pd_evict.hip, pd_shared.hip, pd_pages.hip): the parameter block each kernel takes and
 // the host functions that launch them. The public interface is include/pth_dec.h; nothing here
 // is exported from the library.
 #pragma once
@@ -142,6 +142,10 @@ struct RotaryWriteParams {
     int T, Hq, Hkv, block_size, rotary_dim, interleaved;
     int in_place;                    // query_out is query: its other dims are there already
     int kv_groups;                   // workgroups that take key/value rows (set by the launch)
+    const void* q_weight;            // [256] norm weights of query and key heads, fp32 or the query's dtype; null: no norms
+    const void* k_weight;
+    int weight_fp32;
+    float eps, weight_offset;
 };
 
 // Running attention weights (pd_key_weights_kernel).
@@ -179,6 +183,57 @@ struct EvictParams {
     const int* new_table;
     int64_t nt_stride;
     int block_size, Hkv, keep, recent;
+};
+
+// Page tables (pd_pages.hip).
+constexpr int64_t kRowBytes = 520;
+constexpr int64_t kMaxPages = (int64_t)1 << 22;  // 4,096 counts of 1,024 pages fit the prefix in LDS
+constexpr int kMaxForkRows = 8192;               // old rows' first children in LDS
+constexpr int kMaxPageLayers = 128;              // caches of a call: kernel arguments
+constexpr int kPageCopyGroups = 2048;            // workgroups that copy: 8 per CU
+constexpr int64_t kPagePiece = 16384;            // bytes of a copied piece, at the most
+enum PageForm { kPageWhole, kPageHeads, kPageRows };
+// The counts before the call as bit masks and counts of free pages, in the caller's workspace.
+struct PageWork {
+    unsigned long long* free_mask;   // count 0 (or below): chunks x 16 words
+    unsigned long long* alone_mask;  // count 1
+    int* counts;                     // free pages of each 1,024
+    int pages, chunks;
+};
+struct PageCaches {
+    int8_t* kv[kMaxPageLayers];
+    int64_t sb, sh, ss;              // bytes between pages / kv heads / keys
+    int64_t key_bytes;
+    int layers, Hkv, block_size;
+    int form, runs, cuts;            // runs of adjacent bytes in a page, pieces of a run (set by the launch)
+};
+struct ForkParams {
+    PageWork w;
+    const int* refs;
+    int* new_refs;
+    const int* table;
+    int64_t t_st;
+    int* new_table;
+    int64_t n_st;
+    const int* seq_lens;
+    int* new_lens;
+    const int* parents;              // null: row i goes on from row i
+    int* needed;
+    int rows, new_rows, cols, block_size;
+    int64_t grow, window, sinks;     // window <= 0: none
+    int *eldest, *first_taken, *copy_row, *copy_from, *copies;  // workspace: first child of each old row; per new row; the copies
+};
+struct CompactParams {
+    PageWork w;
+    const int* refs;
+    int* new_refs;
+    const int* table;
+    int64_t t_st;
+    int* new_table;
+    int64_t n_st;
+    int* places;
+    int* used;
+    int rows, cols, block_size;
 };
 
 // The decode launch as the C ABI describes it (pointers, strides in bytes or elements as the
@@ -249,6 +304,10 @@ hipError_t launch_rotary_write(const RotaryWriteParams& p, int dtype, int out_dt
 // running attention weights (pd_key_weights.hip) and eviction by them (pd_evict.hip)
 hipError_t launch_key_weights(const KeyWeightsParams& p, int num_seqs, int heads_kv, hipStream_t stream);
 hipError_t launch_evict(const EvictParams& p, int num_seqs, hipStream_t stream);
+
+// page tables (pd_pages.hip)
+hipError_t launch_fork(ForkParams p, PageCaches k, hipStream_t stream);
+hipError_t launch_compact(const CompactParams& p, PageCaches k, hipStream_t stream);
 
 // cache writer (pd_cache_write.hip); dtype is a PD_DTYPE_* code of key and value
 hipError_t launch_cache_write(const CacheWriteParams& p, int dtype, hipStream_t stream);

@@ -388,6 +388,108 @@ PyObject* evict(PyObject*, PyObject* const* a, Py_ssize_t n) {
     });
 }
 
+// norm_rotary_cache_write(entry, query, query_out, key, value, query_weight, key_weight, positions, cos_sin, key_cache, value_cache,
+//                         k_scale, v_scale, slot_mapping, eps, weight_offset, interleaved)
+PyObject* norm_rotary_cache_write(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    return guarded([&]() -> PyObject* {
+        decltype(&pth_cache_write_norm_rotary) fn;
+        pd_tensor t[13];
+        double eps, offset;
+        int64_t interleaved;
+        if (!count_is(n, 17) || !entry(a[0], fn) || !describe_all(a + 1, t, 13) || !same_gpu(a + 1, 13) || !as_double(a[14], eps) ||
+            !as_double(a[15], offset) || !as_int64(a[16], interleaved))
+            return nullptr;
+        char err[256] = "";
+        OnDevice dev(a[1]);
+        int rc;
+        Py_BEGIN_ALLOW_THREADS;
+        rc = fn(&t[0], &t[1], &t[2], &t[3], &t[4], &t[5], eps, offset, &t[6], &t[7], &t[8], &t[9], &t[10], &t[11], &t[12], interleaved,
+                dev.stream, err, (int)sizeof err);
+        Py_END_ALLOW_THREADS;
+        return done(rc, err);
+    });
+}
+
+// Raw caches from a list or tuple, all on the GPU of `on`; false with a Python error set.
+bool take_caches(PyObject* o, PyObject* on, std::vector<pd_tensor>& caches) {
+    if (!PyList_Check(o) && !PyTuple_Check(o)) {
+        PyErr_SetString(PyExc_TypeError, "caches must be a list or tuple of tensors");
+        return false;
+    }
+    const Py_ssize_t count = PySequence_Fast_GET_SIZE(o);
+    if (count > 128) {  // (the entry's limit)
+        PyErr_SetString(PyExc_RuntimeError, "1 to 128 caches per call");
+        return false;
+    }
+    caches.resize((size_t)std::max<Py_ssize_t>(1, count));
+    for (Py_ssize_t i = 0; i < count; ++i) {
+        PyObject* both[2] = {on, PySequence_Fast_GET_ITEM(o, i)};
+        if (!describe(both[1], caches[(size_t)i]) || !same_gpu(both, 2)) return false;
+    }
+    return true;
+}
+// int32 workspace of a page operator on the GPU of `on`.
+at::Tensor page_workspace(int64_t ints, PyObject* on, pd_tensor& d) {
+    at::Tensor ws = at::empty({std::max<int64_t>(4, ints)}, THPVariable_Unpack(on).options().dtype(at::kInt));
+    d = pd_tensor{};
+    d.data = ws.data_ptr();
+    d.dtype = PD_DTYPE_INT32;
+    d.ndim = 1;
+    d.sizes[0] = ws.numel();
+    d.strides[0] = 1;
+    return ws;
+}
+
+// fork_pages(entry, workspace entry, caches, refs, block_table, seq_lens, new_refs, new_block_table, new_seq_lens, needed,
+//            parents or None, grow, window, sinks)
+PyObject* fork_pages(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    return guarded([&]() -> PyObject* {
+        decltype(&pth_cache_fork_pages) fn;
+        decltype(&pth_cache_pages_workspace) need;
+        pd_tensor t[8], wd;
+        std::vector<pd_tensor> caches;
+        int64_t v[3];
+        if (!count_is(n, 14) || !entry(a[0], fn) || !entry(a[1], need)) return nullptr;
+        const bool parents = a[10] != Py_None;
+        const int tensors = parents ? 8 : 7;
+        if (!describe_all(a + 3, t, tensors) || !same_gpu(a + 3, tensors) || !take_caches(a[2], a[3], caches)) return nullptr;
+        for (int i = 0; i < 3; ++i)
+            if (!as_int64(a[11 + i], v[i])) return nullptr;
+        const int64_t layers = PySequence_Fast_GET_SIZE(a[2]);
+        OnDevice dev(a[3]);
+        const at::Tensor ws = page_workspace(need(caches[0].sizes[0], t[1].sizes[0], t[4].sizes[0]), a[3], wd);
+        char err[256] = "";
+        int rc;
+        Py_BEGIN_ALLOW_THREADS;
+        rc = fn(caches.data(), layers, &t[0], &t[1], &t[2], parents ? &t[7] : nullptr, &t[3], &t[4], &t[5], &t[6], &wd, v[0], v[1],
+                v[2], dev.stream, err, (int)sizeof err);
+        Py_END_ALLOW_THREADS;
+        return done(rc, err);
+    });
+}
+
+// compact_pages(entry, workspace entry, caches, refs, block_table, new_refs, new_block_table, places, used)
+PyObject* compact_pages(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    return guarded([&]() -> PyObject* {
+        decltype(&pth_cache_compact_pages) fn;
+        decltype(&pth_cache_pages_workspace) need;
+        pd_tensor t[6], wd;
+        std::vector<pd_tensor> caches;
+        if (!count_is(n, 9) || !entry(a[0], fn) || !entry(a[1], need) || !describe_all(a + 3, t, 6) || !same_gpu(a + 3, 6) ||
+            !take_caches(a[2], a[3], caches))
+            return nullptr;
+        const int64_t layers = PySequence_Fast_GET_SIZE(a[2]);
+        OnDevice dev(a[3]);
+        const at::Tensor ws = page_workspace(need(caches[0].sizes[0], 0, 0), a[3], wd);
+        char err[256] = "";
+        int rc;
+        Py_BEGIN_ALLOW_THREADS;
+        rc = fn(caches.data(), layers, &t[0], &t[1], &t[2], &t[3], &t[4], &t[5], &wd, dev.stream, err, (int)sizeof err);
+        Py_END_ALLOW_THREADS;
+        return done(rc, err);
+    });
+}
+
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 // The lengths of a batch on the host: a contiguous int32 or int64 CPU tensor.
@@ -589,6 +691,9 @@ PyMethodDef methods[] = {
     PD_METHOD(rotary_cache_write, "pth_cache_write_rotary on torch tensors"),
     PD_METHOD(key_weights, "pth_cache_key_weights on torch tensors"),
     PD_METHOD(evict, "pth_cache_evict on torch tensors"),
+    PD_METHOD(norm_rotary_cache_write, "pth_cache_write_norm_rotary on torch tensors"),
+    PD_METHOD(fork_pages, "pth_cache_fork_pages on torch tensors"),
+    PD_METHOD(compact_pages, "pth_cache_compact_pages on torch tensors"),
     PD_METHOD(plan_decode, "split count of a decode batch"),
     PD_METHOD(deal_pays, "whether a batch of unsplit sequences is dealt instead"),
     PD_METHOD(plan_prefill, "key splits of a prefill launch"),

@@ -62,6 +62,10 @@ EXPORTED_SYMBOLS = (
     "pth_cache_write_rotary",
     "pth_cache_key_weights",
     "pth_cache_evict",
+    "pth_cache_write_norm_rotary",
+    "pth_cache_fork_pages",
+    "pth_cache_compact_pages",
+    "pth_cache_pages_workspace",
 )
 
 
@@ -155,12 +159,22 @@ def load_library(path: str | None = None) -> ctypes.CDLL:
     lib.pth_cache_key_weights.restype = c_int
     lib.pth_cache_evict.argtypes = [tp] * 11 + [ctypes.c_int64] * 3 + [vp, ctypes.c_char_p, c_int]
     lib.pth_cache_evict.restype = c_int
+    lib.pth_cache_write_norm_rotary.argtypes = [tp] * 6 + [c_double, c_double] + [tp] * 7 + [ctypes.c_int64, vp, ctypes.c_char_p, c_int]
+    lib.pth_cache_write_norm_rotary.restype = c_int
+    lib.pth_cache_fork_pages.argtypes = [tp, ctypes.c_int64] + [tp] * 9 + [ctypes.c_int64] * 3 + [vp, ctypes.c_char_p, c_int]
+    lib.pth_cache_fork_pages.restype = c_int
+    lib.pth_cache_compact_pages.argtypes = [tp, ctypes.c_int64] + [tp] * 7 + [vp, ctypes.c_char_p, c_int]
+    lib.pth_cache_compact_pages.restype = c_int
+    lib.pth_cache_pages_workspace.argtypes = [ctypes.c_int64] * 3
+    lib.pth_cache_pages_workspace.restype = ctypes.c_int64
     lib.pth_dec_version.argtypes = []
     lib.pth_dec_version.restype = ctypes.c_char_p
     _entries.update({name: ctypes.cast(getattr(lib, name), vp).value
                      for name in ("pth_dec_decode", "pth_fa_forward", "pth_fa_forward_exact", "pth_fa_forward_split",
                                   "pth_fa_forward_balanced", "pth_fa_balanced_workspace", "pth_cache_write", "pth_dec_decode_lse",
-                                  "pth_dec_decode_shared", "pth_cache_write_rotary", "pth_cache_key_weights", "pth_cache_evict")})
+                                  "pth_dec_decode_shared", "pth_cache_write_rotary", "pth_cache_key_weights", "pth_cache_evict",
+                                  "pth_cache_write_norm_rotary", "pth_cache_fork_pages", "pth_cache_compact_pages",
+                                  "pth_cache_pages_workspace")})
     _lib, _lib_path = lib, os.path.realpath(p)
     return lib
 
@@ -420,6 +434,65 @@ def rotary_cache_write(query: torch.Tensor, key: torch.Tensor, value: torch.Tens
     """
     native().rotary_cache_write(_entry("pth_cache_write_rotary"), query, query if query_out is None else query_out, key, value,
                                 positions, cos_sin, key_cache, value_cache, k_scale, v_scale, slot_mapping, 1 if interleaved else 0)
+
+
+def norm_rotary_cache_write(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor, query_weight: torch.Tensor,
+                            key_weight: torch.Tensor, positions: torch.Tensor, cos_sin: torch.Tensor, key_cache: torch.Tensor,
+                            value_cache: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor, slot_mapping: torch.Tensor,
+                            eps: float = 1e-6, weight_offset: float = 0.0, interleaved: bool = False,
+                            query_out: torch.Tensor | None = None) -> None:
+    """rotary_cache_write for models that norm each query and key head first, all in one launch (no counterpart in the
+    reference).
+
+    Every head x of query and key becomes x / sqrt(mean(x^2) + eps) * (weight + weight_offset) before its rotation, in fp32 and
+    not rounded in between. query_weight and key_weight: [256], of the query's dtype or fp32, which all heads share;
+    weight_offset 1 for models that store their weights less 1. The other arguments are rotary_cache_write's; in place (no query_out)
+    the whole query is written.
+    """
+    native().norm_rotary_cache_write(_entry("pth_cache_write_norm_rotary"), query, query if query_out is None else query_out, key, value,
+                                     query_weight, key_weight, positions, cos_sin, key_cache, value_cache, k_scale, v_scale,
+                                     slot_mapping, eps, weight_offset, 1 if interleaved else 0)
+
+
+def _raw_caches(caches) -> list:
+    return [getattr(c, "kv", c) for c in caches]
+
+
+def fork_pages(caches, refs: torch.Tensor, block_table: torch.Tensor, seq_lens: torch.Tensor, parents: torch.Tensor | None,
+               new_refs: torch.Tensor, new_block_table: torch.Tensor, new_seq_lens: torch.Tensor, needed: torch.Tensor, grow: int = 0,
+               window: int = -1, sinks: int = 0) -> None:
+    """The block tables of a serving step from those before it: rows that go on, fork or end, pages taken and given back (no
+    counterpart in the reference, whose engine keeps its tables on the host).
+
+    caches: a kvcache.PagedKVCache or its raw `kv` per layer, all of one geometry, the tables' pages; refs int32 [pages]: how many
+    table entries name each page (0: free); block_table int32 [B, columns], entries below 0 name no page; seq_lens int32 [B].
+    New row i goes on from old row parents[i] (int32 [N]; outside [0, B): an empty row), None: from row i. It shares the parent's full
+    pages and gets room for `grow` more keys. A page that still takes keys is its own: the first child keeps the parent's if no
+    other entry names it, the others take a free page, into which the keys that the parent has in it are copied, for all caches.
+    window > 0: a page whose keys all lie at or past `sinks` and before what the next token sees (seq_len + 1 - window) becomes
+    -1, as decode and forward_window never read it. Old rows lose their references: a page that nothing names any more is free
+    for the next call. Pages are taken in the order of (row, column), the lowest that were free before the call first.
+    Written: new_block_table int32 [N, columns], new_seq_lens int32 [N] (the parents' lengths), new_refs int32 [pages] (refs
+    itself, or another tensor) and needed int32 [1]: the pages that the call wanted. Where that is more than were free, the last
+    columns that wanted one hold -1, and keys that had to be copied there are in no page of the row. Without parents the
+    new tensors may be the old ones. Runs on the device alone: lengths and tables stay there, and it can be captured in a graph.
+    """
+    native().fork_pages(_entry("pth_cache_fork_pages"), _entry("pth_cache_pages_workspace"), _raw_caches(caches), refs, block_table,
+                        seq_lens, new_refs, new_block_table, new_seq_lens, needed, parents, int(grow), int(window), int(sinks))
+
+
+def compact_pages(caches, refs: torch.Tensor, block_table: torch.Tensor, new_refs: torch.Tensor, new_block_table: torch.Tensor,
+                  places: torch.Tensor, used: torch.Tensor) -> None:
+    """Moves the used pages of a cache into its lowest numbers, so that the rest of it is one free run (no counterpart in the
+    reference).
+
+    caches, refs and block_table as fork_pages takes them. Of n used pages (refs > 0) those numbered n or above go, in order, into
+    the free ones below n, for all caches. Written: new_block_table, new_refs (the old ones or others), places int32 [pages] (where
+    each page lies now, -1 for the free ones; other tables are renamed with it) and used int32 [1] (n). An entry that names no
+    used page becomes -1. The moved pages' old rows stay as they are. Runs on the device alone.
+    """
+    native().compact_pages(_entry("pth_cache_compact_pages"), _entry("pth_cache_pages_workspace"), _raw_caches(caches), refs, block_table,
+                           new_refs, new_block_table, places, used)
 
 
 def key_weights(q: torch.Tensor, key_cache: torch.Tensor, value_cache: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor,
