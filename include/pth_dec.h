@@ -160,6 +160,22 @@ int pth_dec_decode_lse(const pd_tensor* q, const pd_tensor* key_cache, const pd_
                        int64_t causal, hipStream_t stream, char* err, int errlen);
 
 /*
+ * pth_dec_decode for rows that see a sliding window and a few first keys, which stay visible however long the sequence grows. No
+ * counterpart in the reference.
+ *   lse          null, or as for pth_dec_decode_lse
+ *   sinks        >= 0: row j (absolute position p_j) sees key k < seq_len, k <= p_j where causal, if p_j - k < window or k < sinks;
+ *                without a window (<= 0) every row sees those keys anyway
+ * Pages in which no row of the sequence sees a key are not addressed: their table entries may name anything. Other arguments, checks
+ * and return codes are those of pth_dec_decode.
+ */
+int pth_dec_decode_sinks(const pd_tensor* q, const pd_tensor* key_cache, const pd_tensor* value_cache,
+                         const pd_tensor* k_scale, const pd_tensor* v_scale, const pd_tensor* block_table,
+                         const pd_tensor* seq_lens, const pd_tensor* query_start_loc, const pd_tensor* out,
+                         double scale, const pd_tensor* part_o, const pd_tensor* part_m, const pd_tensor* part_l,
+                         const pd_tensor* lse, int64_t num_seqs, int64_t qmax, int64_t nsplit, int64_t window,
+                         int64_t sinks, int64_t causal, hipStream_t stream, char* err, int errlen);
+
+/*
  * Decode attention of a batch whose sequences share their first prefix_len keys (a common prompt or document, samples of
  * one prompt): pth_dec_decode's causal attention without window, with the shared keys read once for the whole batch. No
  * counterpart in the reference.

@@ -52,6 +52,7 @@ LaunchArgs make_args(const void* q, int64_t q_st, const void* kc, int64_t k_sb, 
     x.window = window;
     x.causal = causal;
     x.lse = nullptr;
+    x.sinks = 0;
     return x;
 }
 
@@ -207,7 +208,7 @@ static int decode_entry(const pd_tensor* q, const pd_tensor* key_cache, const pd
                         const pd_tensor* seq_lens, const pd_tensor* query_start_loc, const pd_tensor* out, double scale,
                         const pd_tensor* part_o, const pd_tensor* part_m, const pd_tensor* part_l, const pd_tensor* lse,
                         int64_t num_seqs, int64_t qmax, int64_t nsplit, int64_t window, int64_t causal,
-                        hipStream_t stream, char* err, int errlen, int64_t prefix = -1) {
+                        hipStream_t stream, char* err, int errlen, int64_t prefix = -1, int64_t sinks = 0) {
     if (!q || !key_cache || !value_cache || !k_scale || !v_scale || !block_table || !seq_lens ||
         !query_start_loc || !out || !part_o || !part_m || !part_l)
         return fail(err, errlen, "null tensor descriptor");
@@ -255,6 +256,7 @@ static int decode_entry(const pd_tensor* q, const pd_tensor* key_cache, const pd
         if (!(Hq >= 1 && T <= ((int64_t)1 << 25) / Hq && tiles <= INT32_MAX / 2 && tiles * num_seqs <= INT32_MAX / (2 * Hkv)))
             return fail(err, errlen, "a shared-prefix decode takes at most 2^25 (token, head) rows and 2^30 key tiles");
     }
+    if (!(sinks >= 0 && sinks <= INT32_MAX)) return fail(err, errlen, "sinks must be at least 0 and fit in 32 bits");
     if (T == 0) return 0;
     LaunchArgs x = make_args(
         q->data, q->strides[0], key_cache->data, key_cache->strides[0], key_cache->strides[1],
@@ -265,6 +267,7 @@ static int decode_entry(const pd_tensor* q, const pd_tensor* key_cache, const pd
         static_cast<float*>(const_cast<void*>(part_l->data)), (int)nseg, (int)nsplit, const_cast<void*>(out->data),
         out->strides[0], out->strides[1], (int)window, (int)causal);
     x.lse = lse ? static_cast<float*>(const_cast<void*>(lse->data)) : nullptr;
+    x.sinks = window > 0 ? (int)sinks : 0;
     // (16-key block offsets fit a 32-bit LDS table in 8-byte units when the cache spans less than 2^35 bytes)
     const hipError_t e = prefix < 0 ? launch_all(x, stream, false)
                                     : launch_shared(x, (int)prefix, cache_span(key_cache) < ((int64_t)1 << 35), stream);
@@ -296,6 +299,16 @@ int pth_dec_decode_lse(const pd_tensor* q, const pd_tensor* key_cache, const pd_
     if (!lse) return fail(err, errlen, "null tensor descriptor");
     return decode_entry(q, key_cache, value_cache, k_scale, v_scale, block_table, seq_lens, query_start_loc, out, scale,
                         part_o, part_m, part_l, lse, num_seqs, qmax, nsplit, window, causal, stream, err, errlen);
+}
+
+int pth_dec_decode_sinks(const pd_tensor* q, const pd_tensor* key_cache, const pd_tensor* value_cache,
+                         const pd_tensor* k_scale, const pd_tensor* v_scale, const pd_tensor* block_table,
+                         const pd_tensor* seq_lens, const pd_tensor* query_start_loc, const pd_tensor* out, double scale,
+                         const pd_tensor* part_o, const pd_tensor* part_m, const pd_tensor* part_l, const pd_tensor* lse,
+                         int64_t num_seqs, int64_t qmax, int64_t nsplit, int64_t window, int64_t sinks, int64_t causal,
+                         hipStream_t stream, char* err, int errlen) {
+    return decode_entry(q, key_cache, value_cache, k_scale, v_scale, block_table, seq_lens, query_start_loc, out, scale,
+                        part_o, part_m, part_l, lse, num_seqs, qmax, nsplit, window, causal, stream, err, errlen, -1, sinks);
 }
 
 int pth_dec_decode_shared(const pd_tensor* q, const pd_tensor* key_cache, const pd_tensor* value_cache,

@@ -147,6 +147,56 @@ struct PartialLds {
     static_assert(kBytes <= 160 * 1024, "gfx950 has 160 KiB of LDS per CU");
 };
 
+// The keys that the rows of a sequence see: [lo, hi), and with sinks the first keys as well. Tiles are numbered over what is seen:
+// [0, head) hold the sinks, from `head` on a tile lies `gap` tiles further than its number says. Without sinks a tile's number is
+// its place.
+template <bool kSinks>
+struct Seen {
+    int lo, hi;
+    __device__ __forceinline__ Seen(const PartialParams&, int lo_, int hi_) : lo(lo_), hi(hi_) {}
+    __device__ __forceinline__ int first_tile() const { return lo / kTile; }
+    __device__ __forceinline__ int tiles() const { return (hi - 1) / kTile - first_tile() + 1; }
+    __device__ __forceinline__ int base(int tile) const { return tile * kTile; }
+    // a key of the tile at kb that is seen, k itself if it is
+    __device__ __forceinline__ int near(int kb, int k) const {
+        const int kfirst = max(kb, lo), klast = min(kb + kTile - 1, hi - 1);
+        return min(max(k, kfirst), klast);
+    }
+    __device__ __forceinline__ bool has(int k) const { return (k >= lo) & (k < hi); }
+};
+template <>
+struct Seen<true> {
+    int lo, hi, sinks, head, gap;
+    __device__ __forceinline__ Seen(const PartialParams& a, int lo_, int hi_) : lo(lo_), hi(hi_) {
+        sinks = min(a.sinks, hi);
+        head = (sinks + kTile - 1) / kTile;
+        gap = max(0, lo / kTile - head);
+    }
+    __device__ __forceinline__ int first_tile() const { return 0; }
+    __device__ __forceinline__ int tiles() const { return (hi - 1) / kTile + 1 - gap; }
+    __device__ __forceinline__ int base(int tile) const { return (tile < head ? tile : tile + gap) * kTile; }
+    __device__ __forceinline__ int near(int kb, int k) const {
+        if (k < sinks) return k;
+        return lo < kb + kTile ? min(max(k, lo), hi - 1) : sinks - 1;
+    }
+    __device__ __forceinline__ bool has(int k) const { return ((k >= lo) | (k < sinks)) & (k < hi); }
+};
+// tile_src for what a sequence's rows see, the tile at key kb.
+template <bool kFast, bool kLds, class P>
+__device__ __forceinline__ TileSrc tile_src_seen(const P& a, const PageTable& pt, const int8_t* gbase, int kb, int idx,
+                                                 const Seen<true>& seen, int lane) {
+    if constexpr (kFast && kLds) return tile_src<kFast, kLds>(a, pt, gbase, 0, idx, 0, 0, lane);
+    TileSrc src;
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+        const int key = kFast ? seen.near(kb, kb + 16 * u) & ~15 : seen.near(kb, kb + (lane & 31));
+        const int lb = a.bs_shift >= 0 ? key >> a.bs_shift : key / a.block_size;
+        const int64_t page = kFast ? pt.get_uniform<false>(lb) : pt.get<false>(lb);
+        src.base[u] = gbase + page * a.k_sb + (int64_t)(key - lb * a.block_size) * a.k_ss;
+    }
+    return src;
+}
+
 // What a workgroup computes: rows [row0, row0 + R) of one GQA group of one sequence over the key tiles
 // of one split, and the segment of the partial buffers it writes.
 struct Work {
@@ -158,7 +208,7 @@ struct Work {
     int t_first, ntiles, W;
 };
 
-template <int NRB, bool kFast>
+template <int NRB, bool kFast, bool kSinks>
 __device__ __forceinline__ void partial_body(const PartialParams& a, const Work& wk, unsigned char* lds) {
     // kEarly (block sizes that are multiples of 16): Q and the block-table slice are copied into
     // LDS like the tiles, and each wave's
@@ -182,6 +232,7 @@ __device__ __forceinline__ void partial_body(const PartialParams& a, const Work&
     const int ctx0 = seq_len - q_len;  // absolute position of query token 0
     const int lo = a.window > 0 ? max(0, ctx0 - a.window + 1) : 0;
     const int hi = seq_len;
+    const Seen<kSinks> seen(a, lo, hi);
     const int gw = kWaves * wk.seg + w;  // interleaved: this wave among the W of the (sequence, kv head)
 
     auto prow = [&](int r) -> int64_t {  // partial row index of query row r
@@ -262,9 +313,8 @@ __device__ __forceinline__ void partial_body(const PartialParams& a, const Work&
         // block j of this wave: the first key of its 16-key block clamped into the tile's visible
         // keys (the tile_src rule), and that key's page
         auto wave_block = [&](int j, int& key0, int& lb) {
-            const int kb = tile_of(j >> 1) * kTile;
-            const int kfirst = max(kb, lo), klast = min(kb + kTile - 1, hi - 1);
-            key0 = min(max(kb + 16 * (j & 1), kfirst), klast) & ~15;
+            const int kb = seen.base(tile_of(j >> 1));
+            key0 = seen.near(kb, kb + 16 * (j & 1)) & ~15;
             lb = a.bs_shift >= 0 ? key0 >> a.bs_shift : key0 / a.block_size;
         };
         // (0) the block-table entries of this wave's first two tiles (scalar loads), requested
@@ -274,9 +324,8 @@ __device__ __forceinline__ void partial_body(const PartialParams& a, const Work&
         int key0[4], lb[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const int kb = tile_of(i >> 1) * kTile;
-            const int kfirst = max(kb, lo), klast = min(kb + kTile - 1, hi - 1);
-            key0[i] = min(max(kb + 16 * (i & 1), kfirst), klast) & ~15;
+            const int kb = seen.base(tile_of(i >> 1));
+            key0[i] = seen.near(kb, kb + 16 * (i & 1)) & ~15;
             lb[i] = a.bs_shift >= 0 ? key0[i] >> a.bs_shift : key0[i] / a.block_size;
         }
         int ent[4];
@@ -378,7 +427,8 @@ __device__ __forceinline__ void partial_body(const PartialParams& a, const Work&
             }
         } else {
             const int npages = pk_last / a.block_size - pt.pfirst + 1;
-            pt.in_lds = npages <= kBtCache;
+            // (with sinks the split's pages need not be adjacent: they are looked up in the table itself)
+            pt.in_lds = !kSinks && npages <= kBtCache;
             if (pt.in_lds) {
                 lds_int* dst = (lds_int*)(L + kLdsBt);
                 for (int i = tid; i < npages; i += kThreads) dst[i] = bt_glob[pt.pfirst + i];
@@ -447,12 +497,17 @@ __device__ __forceinline__ void partial_body(const PartialParams& a, const Work&
         float ks[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) ks[e] = o.ks[e] * a.scale_log2;
-        const int kb = tile_cur * kTile;
+        const int kb = seen.base(tile_cur);
         // Interior tile: every key is visible to every row (padding rows have Q = 0 and are
         // never written out), so no per-element mask is needed.
-        interior = kb >= lo && kb + kTile <= hi;
-        if (a.causal) interior = interior && kb + kTile - 1 <= ctx0;
-        if (a.window > 0) interior = interior && (ctx0 + ql - 1) - kb < a.window;
+        if constexpr (kSinks) {
+            interior = kb + kTile <= hi && (kb + kTile <= seen.sinks || (kb >= lo && (ctx0 + ql - 1) - kb < a.window));
+            if (a.causal) interior = interior && kb + kTile - 1 <= ctx0;
+        } else {
+            interior = kb >= lo && kb + kTile <= hi;
+            if (a.causal) interior = interior && kb + kTile - 1 <= ctx0;
+            if (a.window > 0) interior = interior && (ctx0 + ql - 1) - kb < a.window;
+        }
         bool need = false;
 #pragma unroll
         for (int rb = 0; rb < NRB; ++rb) {
@@ -467,8 +522,12 @@ __device__ __forceinline__ void partial_body(const PartialParams& a, const Work&
                 for (int e = 0; e < 8; ++e) {
                     const int t = kb + 16 * (e >> 2) + 4 * lg + (e & 3);
                     const int rp = rpos[rb];
-                    const bool vis = rvalid[rb] & (t >= lo) & (t < hi) & (!a.causal | (t <= rp)) &
-                                     ((a.window <= 0) | ((rp - t) < a.window));
+                    bool vis;
+                    if constexpr (kSinks)
+                        vis = rvalid[rb] & (t < hi) & (!a.causal | (t <= rp)) & ((t < seen.sinks) | ((t >= lo) & ((rp - t) < a.window)));
+                    else
+                        vis = rvalid[rb] & (t >= lo) & (t < hi) & (!a.causal | (t <= rp)) &
+                              ((a.window <= 0) | ((rp - t) < a.window));
                     sv[rb][e] = vis ? sv[rb][e] : kNegInf;
                 }
             }
@@ -531,8 +590,8 @@ __device__ __forceinline__ void partial_body(const PartialParams& a, const Work&
         if (!interior) {  // outside [lo, hi) a scale may be garbage or NaN: use 0
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-                const int t = tile_cur * kTile + 16 * (e >> 2) + 4 * lg + (e & 3);
-                vsc[e] = (t >= lo) & (t < hi) ? vsc[e] : 0.f;
+                const int t = seen.base(tile_cur) + 16 * (e >> 2) + 4 * lg + (e & 3);
+                vsc[e] = seen.has(t) ? vsc[e] : 0.f;
             }
         }
         half8_t phi[NRB], plo[NRB];
@@ -592,9 +651,15 @@ __device__ __forceinline__ void partial_body(const PartialParams& a, const Work&
     // ---- the tile stream of this wave ----
     auto tile_loop = [&](auto lds_flag) __attribute__((always_inline)) {
         constexpr bool kLds = decltype(lds_flag)::value;
+        auto source = [&](int n) __attribute__((always_inline)) {
+            if constexpr (kSinks)
+                return tile_src_seen<kFast, kLds>(a, pt, gbase, seen.base(tile_of(n)), n, seen, l);
+            else
+                return tile_src<kFast, kLds>(a, pt, gbase, tile_of(n), n, lo, hi, l);
+        };
         auto issue = [&](int n) __attribute__((always_inline)) {
             wait_lds();  // every LDS access to the slot being refilled has completed
-            issue_tile<kFast>(a, tile_src<kFast, kLds>(a, pt, gbase, tile_of(n), n, lo, hi, l), dl,
+            issue_tile<kFast>(a, source(n), dl,
                               wslots + (unsigned)((n & 1) * kSlot), l);
         };
         // The same copies in two parts (16-key row blocks): the 8 K blocks, then the 8 V blocks
@@ -602,7 +667,7 @@ __device__ __forceinline__ void partial_body(const PartialParams& a, const Work&
         TileSrc nsrc;
         auto issue_k = [&](int n) __attribute__((always_inline)) {
             wait_lds();  // every LDS access to the slot being refilled has completed
-            nsrc = tile_src<kFast, kLds>(a, pt, gbase, tile_of(n), n, lo, hi, l);
+            nsrc = source(n);
             const unsigned slot = wslots + (unsigned)((n & 1) * kSlot);
             static_for<0, 8>([&](auto ic) {
                 constexpr int i = decltype(ic)::value;
@@ -823,10 +888,8 @@ __device__ __forceinline__ void partial_body(const PartialParams& a, const Work&
 }
 
 // One split of one (sequence, kv head) per workgroup: grid (nsplit, Hkv, num_seqs x slices).
-template <int NRB, bool kFast>
-__global__ void __launch_bounds__(kThreads, 1) pd_partial_kernel(const PartialParams a) {
-    __shared__ __attribute__((aligned(16))) unsigned char lds[PartialLds<NRB, kFast>::kBytes];
-
+template <int NRB, bool kFast, bool kSinks>
+__device__ __forceinline__ void partial_workgroup(const PartialParams& a, unsigned char* lds) {
     // grid z = row slice x sequence: with rslices > 1 the workgroup takes rows [row0, row0 + 16 NRB)
     // of its GQA group, and the group's other slices read the same tiles
     const int s = blockIdx.x, g = blockIdx.y;
@@ -850,8 +913,9 @@ __global__ void __launch_bounds__(kThreads, 1) pd_partial_kernel(const PartialPa
     const int R = min(16 * NRB, min(q_len, a.qmax) * a.G - row0);
     if (R <= 0) return;                          // a slice past the sequence's rows
     const int lo = a.window > 0 ? max(0, seq_len - q_len - a.window + 1) : 0;
-    const int t_first = lo / kTile;
-    const int ntiles = (seq_len - 1) / kTile - t_first + 1;
+    const Seen<kSinks> seen(a, lo, seq_len);
+    const int t_first = seen.first_tile();
+    const int ntiles = seen.tiles();
     // Tiles of each wave. Split s owns a contiguous run of tiles [tb, te) and its waves take every
     // kWaves-th tile of it, unless the block size is a multiple of 16 and there are at least as
     // many tiles as the W = kWaves * nsplit waves of a (sequence, kv head): then the waves
@@ -882,7 +946,7 @@ __global__ void __launch_bounds__(kThreads, 1) pd_partial_kernel(const PartialPa
         }
         return;
     }
-    partial_body<NRB, kFast>(a, wk, lds);
+    partial_body<NRB, kFast, kSinks>(a, wk, lds);
 }
 
 // ---------------------------------------------------------------------------------------
@@ -905,9 +969,8 @@ __global__ void __launch_bounds__(kThreads, 1) pd_partial_kernel(const PartialPa
 constexpr unsigned kSegmentUnits = 12;  // set-up and merge of a segment, ~10 us, in tiles of a workgroup (~0.8 us each)
 constexpr unsigned kSnapTiles = 6;      // a share's end this close to an item's boundary moves onto it
 
-template <int NRB, bool kFast>
-__global__ void __launch_bounds__(kThreads, 1) pd_balanced_kernel(const PartialParams a) {
-    __shared__ __attribute__((aligned(16))) unsigned char lds[PartialLds<NRB, kFast>::kBytes];
+template <int NRB, bool kFast, bool kSinks>
+__device__ __forceinline__ void balanced_workgroup(const PartialParams& a, unsigned char* lds) {
     asm volatile("" ::"s"(a.qsl), "s"(a.seq_lens), "s"(a.block_table), "s"(a.bt_stride), "s"(a.kc), "s"(a.k_sb),
                  "s"(a.k_ss), "s"(a.k_sh), "s"(a.q), "s"(a.q_st), "s"(a.qmax), "s"(a.G), "s"(a.window),
                  "s"(a.nsplit), "s"(a.block_size), "s"(a.bs_shift));
@@ -918,6 +981,7 @@ __global__ void __launch_bounds__(kThreads, 1) pd_balanced_kernel(const PartialP
         const int c = min(i, a.num_seqs - 1);
         const int q_len = a.qsl[c + 1] - a.qsl[c], len = a.seq_lens[c];
         const int lo = a.window > 0 ? max(0, len - q_len - a.window + 1) : 0;
+        if constexpr (kSinks) return i < a.num_seqs && q_len > 0 && len > 0 ? (unsigned)Seen<true>(a, lo, len).tiles() : 0u;
         return i < a.num_seqs && q_len > 0 && len > 0 ? (unsigned)((len - 1) / kTile - lo / kTile + 1) : 0u;
     };
     auto units_of = [&](unsigned t) __attribute__((always_inline)) { return t ? t + kSegmentUnits : 0u; };
@@ -997,8 +1061,9 @@ __global__ void __launch_bounds__(kThreads, 1) pd_balanced_kernel(const PartialP
         asm volatile("" ::"s"(wk.q0), "s"(q_end), "s"(wk.seq_len));
         wk.q_len = q_end - wk.q0;
         const int lo = a.window > 0 ? max(0, wk.seq_len - wk.q_len - a.window + 1) : 0;
-        wk.t_first = lo / kTile;
+        wk.t_first = kSinks ? 0 : lo / kTile;
         wk.ntiles = (wk.seq_len - 1) / kTile - wk.t_first + 1;
+        if constexpr (kSinks) wk.ntiles -= Seen<true>(a, lo, wk.seq_len).gap;
         if (aligned) {
             if (wk.q_len <= 0 || wk.seq_len <= 0) return;
             const unsigned per = ((unsigned)wk.ntiles + ns - 1) / ns;
@@ -1012,7 +1077,7 @@ __global__ void __launch_bounds__(kThreads, 1) pd_balanced_kernel(const PartialP
         wk.te = wk.t_first + (int)last;
         wk.W = 0;
         wk.interleave = false;
-        partial_body<NRB, kFast>(a, wk, lds);
+        partial_body<NRB, kFast, kSinks>(a, wk, lds);
         if (last == (unsigned)wk.ntiles) {  // the item's last workgroup: no other segments
             const int R = min(16 * NRB, min(wk.q_len, a.qmax) * a.G), spare = a.nsplit - 1 - wk.seg;
             for (int k = threadIdx.x; k < R * spare; k += kThreads) {
@@ -1027,6 +1092,35 @@ __global__ void __launch_bounds__(kThreads, 1) pd_balanced_kernel(const PartialP
         if (pos >= end) return;
         __syncthreads();  // every wave has read the merge's blocks: the slots can be refilled
     }
+}
+
+template <int NRB, bool kFast>
+__global__ void __launch_bounds__(kThreads, 1) pd_partial_kernel(const PartialParams a) {
+    __shared__ __attribute__((aligned(16))) unsigned char lds[PartialLds<NRB, kFast>::kBytes];
+    partial_workgroup<NRB, kFast, false>(a, lds);
+}
+
+template <int NRB, bool kFast>
+__global__ void __launch_bounds__(kThreads, 1) pd_balanced_kernel(const PartialParams a) {
+    __shared__ __attribute__((aligned(16))) unsigned char lds[PartialLds<NRB, kFast>::kBytes];
+    balanced_workgroup<NRB, kFast, false>(a, lds);
+}
+
+// The same for rows that see a sliding window and the first `sinks` keys: row j at position p sees key k < seq_len (and k <= p
+// where causal) if p - k < window or k < sinks. The keys between the sinks and the first row's window are in no tile of the launch
+// (Seen numbers the tiles without the gap), so splits, deal and waves are those of a sequence as long as what it sees, and pages that hold
+// nothing seen, given back long ago, are never addressed. One softmax runs over both parts. (Kernels of their own: the masks and the
+// numbering cost the others nothing.)
+template <int NRB, bool kFast>
+__global__ void __launch_bounds__(kThreads, 1) pd_sinks_kernel(const PartialParams a) {
+    __shared__ __attribute__((aligned(16))) unsigned char lds[PartialLds<NRB, kFast>::kBytes];
+    partial_workgroup<NRB, kFast, true>(a, lds);
+}
+
+template <int NRB, bool kFast>
+__global__ void __launch_bounds__(kThreads, 1) pd_sinks_balanced_kernel(const PartialParams a) {
+    __shared__ __attribute__((aligned(16))) unsigned char lds[PartialLds<NRB, kFast>::kBytes];
+    balanced_workgroup<NRB, kFast, true>(a, lds);
 }
 
 // Cross-row lane exchanges of gfx950 (v_permlane16/32_swap), as asm with both registers read and
@@ -1262,6 +1356,40 @@ static hipError_t launch_balanced_nrb(const PartialParams& p, int wgs, hipStream
     return hipGetLastError();
 }
 
+template <int NRB>
+static void launch_split(const PartialParams& p, dim3 grid, hipStream_t stream, bool fast) {
+    if (fast)
+        hipLaunchKernelGGL((pd_sinks_kernel<NRB, true>), grid, dim3(kThreads), 0, stream, p);
+    else
+        hipLaunchKernelGGL((pd_sinks_kernel<NRB, false>), grid, dim3(kThreads), 0, stream, p);
+}
+template <int NRB>
+static void launch_dealt(const PartialParams& p, int wgs, hipStream_t stream, bool fast) {
+    if (fast)
+        hipLaunchKernelGGL((pd_sinks_balanced_kernel<NRB, true>), dim3(wgs), dim3(kThreads), 0, stream, p);
+    else
+        hipLaunchKernelGGL((pd_sinks_balanced_kernel<NRB, false>), dim3(wgs), dim3(kThreads), 0, stream, p);
+}
+
+static hipError_t launch_sinks(const PartialParams& p, int splits, int groups, int heads_kv, int nrb, bool fast, hipStream_t stream) {
+    const dim3 grid(splits, heads_kv, groups);
+    if (nrb == 1)
+        launch_split<1>(p, grid, stream, fast);
+    else if (nrb == 2)
+        launch_split<2>(p, grid, stream, fast);
+    else
+        launch_split<3>(p, grid, stream, fast);
+    return hipGetLastError();
+}
+
+static hipError_t launch_sinks_balanced(const PartialParams& p, int wgs, int nrb, bool fast, hipStream_t stream) {
+    if (nrb == 1)
+        launch_dealt<1>(p, wgs, stream, fast);
+    else
+        launch_dealt<2>(p, wgs, stream, fast);
+    return hipGetLastError();
+}
+
 // Segments per item that a balanced launch may use (0: the batch is not one for it). A split count whose
 // workgroups fit one round of the CUs has been planned for the batch's lengths, and its kernel starts ~1.5 us earlier
 // (16 x 300 keys at 4 splits 11.5 us against 12.6, 64 x 4,096 at 1 split 109.2 against 111.3). Past one
@@ -1313,6 +1441,7 @@ hipError_t launch_partial(const LaunchArgs& x, hipStream_t stream, int* balanced
     p.qmax = x.qmax;
     p.Hq = x.heads_q;
     p.window = x.window > 0 ? x.window : 0;
+    p.sinks = x.window > 0 ? x.sinks : 0;
     p.causal = x.causal ? 1 : 0;
     p.bs_shift = (x.block_size & (x.block_size - 1)) == 0 ? __builtin_ctz((unsigned)x.block_size) : -1;
     const int rows = x.qmax * p.G;
@@ -1323,7 +1452,7 @@ hipError_t launch_partial(const LaunchArgs& x, hipStream_t stream, int* balanced
     // over 2,048-key windows: 23.8 -> 19.3 us per layer at 5 splits of 3 slices against 16
     // unsliced splits; past kSliceKeys, e.g. 4 x 8 rows over 8,192 keys, slicing lost).
     p.num_seqs = x.num_seqs;
-    p.rslices = nrb > 1 && x.window > 0 && (int64_t)x.window * x.num_seqs <= kSliceKeys &&
+    p.rslices = nrb > 1 && x.window > 0 && ((int64_t)x.window + p.sinks) * x.num_seqs <= kSliceKeys &&
                         (int64_t)x.nsplit * x.heads_kv * x.num_seqs * nrb <= compute_units(stream)
                     ? nrb
                     : 1;
@@ -1334,10 +1463,12 @@ hipError_t launch_partial(const LaunchArgs& x, hipStream_t stream, int* balanced
         *balanced = p.rslices == 1 && cus > 0 ? balanced_segments(x, cus) : 0;
         if (*balanced) {
             p.nsplit = *balanced;
+            if (p.sinks > 0) return launch_sinks_balanced(p, cus, rows <= 16 ? 1 : 2, fast, stream);
             if (rows <= 16) return launch_balanced_nrb<1>(p, cus, stream, fast);
             return launch_balanced_nrb<2>(p, cus, stream, fast);
         }
     }
+    if (p.sinks > 0) return launch_sinks(p, x.nsplit, x.num_seqs * p.rslices, x.heads_kv, p.rslices > 1 ? 1 : nrb, fast, stream);
     if (rows <= 16 || p.rslices > 1) return launch_partial_nrb<1>(p, grid, stream, fast);
     if (rows <= 32) return launch_partial_nrb<2>(p, grid, stream, fast);
     return launch_partial_nrb<3>(p, grid, stream, fast);

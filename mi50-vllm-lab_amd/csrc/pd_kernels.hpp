@@ -47,6 +47,7 @@ struct PartialParams {
     int bs_shift;            // log2(block_size) if it is a power of two, else -1
     int num_seqs;
     int rslices;             // workgroups per (sequence, kv head, split), each 16 NRB of the rows
+    int sinks;               // > 0 (with a window): first keys that every row sees
 };
 
 // Split-K decode, log-sum-exp merge of the partials (pd_combine_kernel).
@@ -258,6 +259,7 @@ struct LaunchArgs {
     int64_t o_st, o_sh;
     int window, causal;
     float* lse;              // [num_tokens, heads_q], or null
+    int sinks;               // first keys that every row sees (0 without a window)
 };
 
 // Row blocks of 16 keys never straddle a page when block_size is a multiple of 16: then every

@@ -301,6 +301,30 @@ PyObject* decode_lse(PyObject*, PyObject* const* a, Py_ssize_t n) {
     });
 }
 
+// decode_sinks(entry, q, key_cache, value_cache, k_scale, v_scale, block_table, seq_lens, query_start_loc, out, part_o, part_m,
+//              part_l, lse or None, scale, num_seqs, qmax, nsplit, window, sinks, causal)
+PyObject* decode_sinks(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    return guarded([&]() -> PyObject* {
+        decltype(&pth_dec_decode_sinks) fn;
+        pd_tensor t[13];
+        double scale;
+        int64_t v[6];
+        if (!count_is(n, 21) || !entry(a[0], fn)) return nullptr;
+        const bool lse = a[13] != Py_None;
+        if (!describe_all(a + 1, t, lse ? 13 : 12) || !same_gpu(a + 1, lse ? 13 : 12) || !as_double(a[14], scale)) return nullptr;
+        for (int i = 0; i < 6; ++i)
+            if (!as_int64(a[15 + i], v[i])) return nullptr;
+        char err[256] = "";
+        OnDevice dev(a[1]);
+        int rc;
+        Py_BEGIN_ALLOW_THREADS;
+        rc = fn(&t[0], &t[1], &t[2], &t[3], &t[4], &t[5], &t[6], &t[7], &t[8], scale, &t[9], &t[10], &t[11],
+                lse ? &t[12] : nullptr, v[0], v[1], v[2], v[3], v[4], v[5], dev.stream, err, (int)sizeof err);
+        Py_END_ALLOW_THREADS;
+        return done(rc, err);
+    });
+}
+
 // decode_shared(entry, q, key_cache, value_cache, k_scale, v_scale, block_table, seq_lens, query_start_loc, out, part_o,
 //               part_m, part_l, lse or None, scale, num_seqs, qmax, prefix_len)
 PyObject* decode_shared(PyObject*, PyObject* const* a, Py_ssize_t n) {
@@ -687,6 +711,7 @@ PyMethodDef methods[] = {
     PD_METHOD(prefill_balanced, "pth_fa_forward_balanced on torch tensors"),
     PD_METHOD(cache_write, "pth_cache_write on torch tensors"),
     PD_METHOD(decode_lse, "pth_dec_decode_lse on torch tensors"),
+    PD_METHOD(decode_sinks, "pth_dec_decode_sinks on torch tensors"),
     PD_METHOD(decode_shared, "pth_dec_decode_shared on torch tensors"),
     PD_METHOD(rotary_cache_write, "pth_cache_write_rotary on torch tensors"),
     PD_METHOD(key_weights, "pth_cache_key_weights on torch tensors"),

@@ -51,6 +51,7 @@ EXPORTED_SYMBOLS = (
     "pth_dec_supported_layout",
     "pth_dec_decode",
     "pth_dec_decode_lse",
+    "pth_dec_decode_sinks",
     "pth_dec_decode_shared",
     "pth_dec_version",
     "pth_fa_forward",
@@ -151,6 +152,8 @@ def load_library(path: str | None = None) -> ctypes.CDLL:
     lib.pth_cache_write.restype = c_int
     lib.pth_dec_decode_lse.argtypes = [tp] * 9 + [c_double, tp, tp, tp, tp] + [ctypes.c_int64] * 5 + [vp, ctypes.c_char_p, c_int]
     lib.pth_dec_decode_lse.restype = c_int
+    lib.pth_dec_decode_sinks.argtypes = [tp] * 9 + [c_double, tp, tp, tp, tp] + [ctypes.c_int64] * 6 + [vp, ctypes.c_char_p, c_int]
+    lib.pth_dec_decode_sinks.restype = c_int
     lib.pth_dec_decode_shared.argtypes = [tp] * 9 + [c_double, tp, tp, tp, tp] + [ctypes.c_int64] * 3 + [vp, ctypes.c_char_p, c_int]
     lib.pth_dec_decode_shared.restype = c_int
     lib.pth_cache_write_rotary.argtypes = [tp] * 11 + [ctypes.c_int64, vp, ctypes.c_char_p, c_int]
@@ -172,7 +175,7 @@ def load_library(path: str | None = None) -> ctypes.CDLL:
     _entries.update({name: ctypes.cast(getattr(lib, name), vp).value
                      for name in ("pth_dec_decode", "pth_fa_forward", "pth_fa_forward_exact", "pth_fa_forward_split",
                                   "pth_fa_forward_balanced", "pth_fa_balanced_workspace", "pth_cache_write", "pth_dec_decode_lse",
-                                  "pth_dec_decode_shared", "pth_cache_write_rotary", "pth_cache_key_weights", "pth_cache_evict",
+                                  "pth_dec_decode_sinks", "pth_dec_decode_shared", "pth_cache_write_rotary", "pth_cache_key_weights", "pth_cache_evict",
                                   "pth_cache_write_norm_rotary", "pth_cache_fork_pages", "pth_cache_compact_pages",
                                   "pth_cache_pages_workspace")})
     _lib, _lib_path = lib, os.path.realpath(p)
@@ -213,7 +216,7 @@ def decode(q: torch.Tensor, key_cache: torch.Tensor, value_cache: torch.Tensor, 
            v_scale: torch.Tensor, block_table: torch.Tensor, seq_lens: torch.Tensor,
            query_start_loc: torch.Tensor, out: torch.Tensor, scale: float, part_o: torch.Tensor,
            part_m: torch.Tensor, part_l: torch.Tensor, num_seqs: int, qmax: int, nsplit: int,
-           window: int = -1, causal: bool = True, lse: torch.Tensor | None = None) -> None:
+           window: int = -1, causal: bool = True, lse: torch.Tensor | None = None, sinks: int = 0) -> None:
     """Split-K decode attention over the int8 per-token-head paged KV cache, written into `out`.
 
     q: fp16 [T, Hq, 256] with head stride 256; out: fp16 [T, Hq, 256] with unit dim stride;
@@ -223,10 +226,17 @@ def decode(q: torch.Tensor, key_cache: torch.Tensor, value_cache: torch.Tensor, 
     scratch, vLLM's softmax segment buffers); 1 <= nsplit <= NSEG.
     lse (fp32 [>= T, Hq], no counterpart in the reference): also receives ln(sum over the visible keys of
     e^(scale q . k)) of each row, -inf for a row that sees none (pth_dec_decode_lse); key_weights reads it.
+    sinks (no counterpart in the reference): with a window, the rows also see the first `sinks` keys (a causal row up to its
+    position), however far behind the window they lie; pages that hold neither are not read (pth_dec_decode_sinks).
     Reference: kernels/pth_dec/pth_dec.cpp:43-91.
     """
     if not q.is_cuda:
         raise RuntimeError("q must be fp16 [T, Hq, 256] with contiguous heads")
+    if sinks:
+        native().decode_sinks(_entry("pth_dec_decode_sinks"), q, key_cache, value_cache, k_scale, v_scale, block_table, seq_lens,
+                              query_start_loc, out, part_o, part_m, part_l, lse, scale, int(num_seqs), int(qmax), int(nsplit),
+                              int(window), int(sinks), 1 if causal else 0)
+        return
     if lse is not None:
         native().decode_lse(_entry("pth_dec_decode_lse"), q, key_cache, value_cache, k_scale, v_scale, block_table, seq_lens,
                             query_start_loc, out, part_o, part_m, part_l, lse, scale, int(num_seqs), int(qmax), int(nsplit),
