@@ -282,6 +282,28 @@ int64_t pth_fa_balanced_workspace(int64_t num_seqs, const int* query_start, int6
                                   int64_t max_keys, int64_t table_keys);
 
 /*
+ * Causal chunked prefill of rows that see a sliding window and a few first keys. No counterpart in the reference.
+ *   q, out       fp16 [T, Hq, 256], unit dim stride, rows of q 16-byte and of out 8-byte aligned
+ *   query_start_loc  int32 [>= num_seqs + 1], device: sequence i has rows [query_start_loc[i], query_start_loc[i + 1]) of q and out, the last
+ *                tokens of its seq_lens[i] keys (block_table and seq_lens have a row per sequence). Rows outside the sequences, and of
+ *                sequences of no keys, are left alone
+ *   window >= 1, sinks >= 0   the row at position p sees key k <= p if p - k < window or k < sinks
+ *   nsplit       1..64: key splits per query tile (256 rows of one kv head); pth_fa_window_splits' count suits the sizes
+ *   workspace    fp32, contiguous, 16-byte aligned, of T * Hq * nsplit * 258 floats (null or ignored when nsplit is 1)
+ *   exact        0: each softmax weight enters P.V as one fp16; else as fp16 hi + lo. K and V are widened exactly in both
+ * Pages in which no row of a query tile sees a key are not addressed for it: the table's entries for pages between the sinks and
+ * the first row's window may name anything. Returns 0, 1 or 2 as above.
+ */
+int pth_fa_forward_window(const pd_tensor* q, const pd_tensor* key_cache, const pd_tensor* value_cache,
+                          const pd_tensor* block_table, const pd_tensor* seq_lens, double scale,
+                          const pd_tensor* query_start_loc, const pd_tensor* out, const pd_tensor* workspace, int64_t num_seqs,
+                          int64_t window, int64_t sinks, int64_t nsplit, int64_t exact, hipStream_t stream, char* err,
+                          int errlen);
+/* Splits that such a call is rated fastest with on the current device; table_keys: block_table columns x block size. */
+int64_t pth_fa_window_splits(int64_t tokens, int64_t num_seqs, int64_t heads_q, int64_t heads_kv, int64_t window,
+                             int64_t sinks, int64_t table_keys, int64_t exact);
+
+/*
  * KV-cache writer and quantiser: the producer of the 520-byte rows the two operators read.
  * Replaces vLLM's cache update for int8 per-token-head KV, which the reference calls as
  * do_kv_cache_update(layer, key, value, kv_cache, slot_mapping)

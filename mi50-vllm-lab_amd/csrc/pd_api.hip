@@ -14,6 +14,7 @@
 #pragma GCC visibility pop
 
 #include "pd_kernels.hpp"
+#include "pd_plan.hpp"
 
 namespace pd {
 namespace {
@@ -201,6 +202,9 @@ static const char* lse_refused(const pd_tensor* lse, int64_t T, int64_t Hq) {
 }
 
 static int64_t cache_span(const pd_tensor* kc);
+static bool int_rows(const pd_tensor* t, int64_t n);
+static bool int_table(const pd_tensor* t, int64_t n);
+static bool rows_apart(const pd_tensor* t, int64_t n0, int64_t len);
 
 // The decode entries' body; prefix >= 0: the shared-prefix decode (nsplit is not looked at beyond its check).
 static int decode_entry(const pd_tensor* q, const pd_tensor* key_cache, const pd_tensor* value_cache,
@@ -560,6 +564,96 @@ static int fa_forward_rows(const pd_tensor* q, const pd_tensor* kc, const pd_ten
     if (!balanced_ok(tiles * Hkv, bt->sizes[1] * bs)) return fail(err, errlen, "a balanced prefill takes at most 2^31 key tiles");
     if (const char* why = balanced_workspace(p, r, workspace, tiles * Hkv, max_keys, stream)) return fail(err, errlen, why);
     return fa_result(launch_prefill_balanced(p, r, (int)Hkv, q->dtype, stream, exact), err, errlen);
+}
+
+int64_t pth_fa_window_splits(int64_t tokens, int64_t num_seqs, int64_t heads_q, int64_t heads_kv, int64_t window, int64_t sinks,
+                             int64_t table_keys, int64_t exact) {
+    if (tokens < 1 || tokens > INT32_MAX || num_seqs < 1 || num_seqs > INT32_MAX || heads_kv < 1 || heads_q < heads_kv ||
+        heads_q % heads_kv != 0 || heads_q > (1 << 20) || window < 1 || window > INT32_MAX || sinks < 0 || sinks > INT32_MAX)
+        return 1;
+    const int64_t G = heads_q / heads_kv, span = window + (kFwRows + G - 1) / G + 31;  // keys that a query tile sees, aligned
+    const int64_t tiles = (std::min(span, std::max<int64_t>(1, table_keys)) + 31) / 32 + (std::min(sinks, std::max<int64_t>(0, table_keys - span)) + 31) / 32;
+    int dev = 0, cus = 0;
+    if (hipGetDevice(&dev) != hipSuccess ||
+        hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess || cus < 1)
+        cus = 256;
+    // (half of the sequences' last tiles are taken to be part-filled ones of their own)
+    const int64_t items = ((tokens * G + kFwRows - 1) / kFwRows + (num_seqs - 1) / 2) * heads_kv;
+    return window_splits(items, tiles, tokens * heads_q, cus, exact != 0);
+}
+
+int pth_fa_forward_window(const pd_tensor* q, const pd_tensor* key_cache, const pd_tensor* value_cache,
+                          const pd_tensor* block_table, const pd_tensor* seq_lens, double scale,
+                          const pd_tensor* query_start_loc, const pd_tensor* out, const pd_tensor* workspace, int64_t num_seqs,
+                          int64_t window, int64_t sinks, int64_t nsplit, int64_t exact, hipStream_t stream, char* err, int errlen) {
+    if (!q || !key_cache || !value_cache || !block_table || !seq_lens || !query_start_loc || !out)
+        return fail(err, errlen, "null tensor descriptor");
+    if (!(q->ndim == 3 && q->dtype == PD_DTYPE_FP16 && q->sizes[2] == kDim && q->strides[2] == 1 && q->sizes[0] <= INT32_MAX &&
+          q->sizes[1] <= (1 << 20)))
+        return fail(err, errlen, "q must be fp16 [T, Hq, 256] with unit dim stride");
+    if (!(out->ndim == 3 && out->dtype == PD_DTYPE_FP16 && out->sizes[0] == q->sizes[0] && out->sizes[1] == q->sizes[1] &&
+          out->sizes[2] == kDim && out->strides[2] == 1))
+        return fail(err, errlen, "out must be fp16 [T, Hq, 256] with unit dim stride");
+    if (!(reinterpret_cast<uintptr_t>(q->data) % 16 == 0 && q->strides[0] % 8 == 0 && q->strides[1] % 8 == 0 &&
+          reinterpret_cast<uintptr_t>(out->data) % 8 == 0 && out->strides[0] % 4 == 0 && out->strides[1] % 4 == 0))
+        return fail(err, errlen, "q rows must be 16-byte aligned and out rows 8-byte aligned");
+    if (!(key_cache->dtype == PD_DTYPE_INT8 && value_cache->dtype == PD_DTYPE_INT8 && key_cache->ndim == 4 && value_cache->ndim == 4 &&
+          key_cache->strides[3] == 1 && value_cache->strides[3] == 1 && key_cache->sizes[3] >= kDim + 4 && value_cache->sizes[3] >= kDim + 4))
+        return fail(err, errlen, "key/value cache views must be 4D int8 rows of D values and a fp32 scale");
+    const uintptr_t kb = reinterpret_cast<uintptr_t>(key_cache->data);
+    bool rows_ok = kb % 8 == 0 && reinterpret_cast<uintptr_t>(value_cache->data) == kb + 260;
+    for (int i = 0; i < 3; ++i)
+        rows_ok = rows_ok && key_cache->strides[i] == value_cache->strides[i] && key_cache->sizes[i] == value_cache->sizes[i] &&
+                  key_cache->strides[i] % 8 == 0 && key_cache->strides[i] <= INT32_MAX;
+    if (!rows_ok) return fail(err, errlen, "value_cache must view the same 8-byte aligned cache rows as key_cache, 260 bytes in");
+    const int64_t T = q->sizes[0], Hq = q->sizes[1], bs = key_cache->sizes[1], Hkv = key_cache->sizes[2];
+    if (!(Hkv > 0 && Hkv <= 65535 && Hq > 0 && Hq % Hkv == 0 && Hq <= 65535 && Hq / Hkv <= kFwRows && bs > 0 && bs <= INT32_MAX))
+        return fail(err, errlen, "heads_q must be a multiple of heads_kv, at most 256 times and 65535");
+    if (!(num_seqs >= 1 && num_seqs <= INT32_MAX && int_table(block_table, num_seqs) && int_rows(seq_lens, num_seqs) &&
+          int_rows(query_start_loc, num_seqs + 1)))
+        return fail(err, errlen, "block_table / seq_lens / query_start_loc must be int32 with a row for each of at least one sequence");
+    if (!(window >= 1 && window <= INT32_MAX && sinks >= 0 && sinks <= INT32_MAX))
+        return fail(err, errlen, "window must be at least 1, sinks at least 0, and both fit in 32 bits");
+    if (!(nsplit >= 1 && nsplit <= 64)) return fail(err, errlen, "nsplit must be in [1, 64]");
+    // a launch's workgroups, and the 32 bits that number query tiles and rows
+    const int64_t G = Hq / Hkv, tiles = window_tiles(T, num_seqs, G);
+    if (!(T * Hq <= ((int64_t)1 << 30) && tiles * nsplit <= (1 << 24) / Hkv - 1))
+        return fail(err, errlen, "at most 2^30 (token, head) rows and 2^24 workgroups per call");
+    if (!rows_apart(out, T, kDim)) return fail(err, errlen, "out rows must not overlap");
+    if (nsplit > 1 && !(workspace && workspace->dtype == PD_DTYPE_FP32 && workspace->ndim == 1 && is_contig(workspace) &&
+                        workspace->sizes[0] >= prefill_workspace_floats(1, T, Hq, nsplit) &&
+                        reinterpret_cast<uintptr_t>(workspace->data) % 16 == 0))
+        return fail(err, errlen, "workspace must be contiguous 16-byte aligned fp32 of T * Hq * nsplit * 258");
+    if (T == 0) return 0;
+    FaParams p = {};
+    p.q = q->data;
+    p.q_sh = q->strides[1];
+    p.q_st = q->strides[0];
+    p.kc = static_cast<const int8_t*>(key_cache->data);
+    p.k_sb = key_cache->strides[0];
+    p.k_ss = key_cache->strides[1];
+    p.k_sh = key_cache->strides[2];
+    p.block_table = static_cast<const int*>(block_table->data);
+    p.bt_stride = block_table->strides[0];
+    p.seq_lens = static_cast<const int*>(seq_lens->data);
+    p.out = const_cast<void*>(out->data);
+    p.o_st = out->strides[0];
+    p.o_sh = out->strides[1];
+    p.Hq = (int)Hq;
+    p.G = (int)G;
+    p.block_size = (int)bs;
+    p.bs_shift = (bs & (bs - 1)) == 0 ? __builtin_ctz((unsigned)bs) : -1;
+    p.bt32 = cache_span(key_cache) < ((int64_t)1 << 35);
+    p.scale_log2 = (float)scale * 1.4426950408889634f;
+    p.nsplit = (int)nsplit;
+    if (nsplit > 1) {
+        const int64_t rows = T * Hq * nsplit;
+        p.part_o = static_cast<float*>(const_cast<void*>(workspace->data));
+        p.part_m = p.part_o + rows * kDim;
+        p.part_l = p.part_m + rows;
+    }
+    const FaWindow w = {static_cast<const int*>(query_start_loc->data), (int)num_seqs, (int)T, (int)window, (int)sinks};
+    return fa_result(launch_window(p, w, (int)Hkv, stream, exact != 0), err, errlen);
 }
 
 int pth_fa_forward(const pd_tensor* q, const pd_tensor* key_cache, const pd_tensor* value_cache,

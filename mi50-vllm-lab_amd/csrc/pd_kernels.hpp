@@ -114,6 +114,16 @@ struct FaRowsParams {
     int nwg;                         // workgroups of the launch
 };
 
+// The rows of a windowed prefill (pd_window_kernel): sequence i has rows [query_start[i], query_start[i + 1]) of q and out, the last
+// tokens of its keys.
+struct FaWindow {
+    const int* query_start;
+    int num_seqs, num_tokens;
+    int window, sinks;
+};
+// query tiles of a kv head that such rows have at the most
+inline int64_t window_tiles(int64_t tokens, int64_t seqs, int64_t G) { return tokens * G / kFwRows + seqs; }
+
 // KV-cache writer (pd_cache_write_kernel).
 struct CacheWriteParams {
     const void* key;
@@ -293,6 +303,8 @@ hipError_t launch_prefill_balanced(const FaParams& p, const FaRowsParams& r, int
                                    bool exact);
 // workgroups of such a launch on `cus` CUs: as many as the work pays for, at least one per item while CUs last
 int64_t balanced_prefill_workgroups(int64_t items, int64_t max_keys, int cus);
+// the 256-row kernel for fp16 rows that see a window and sinks, p.nsplit splits and their merge (pd_prefill_wide.hip)
+hipError_t launch_window(const FaParams& p, const FaWindow& w, int heads_kv, hipStream_t stream, bool exact);
 constexpr int64_t kFaSlotFloats = (int64_t)kFaRows * (kDim + 2);
 // compute units of a stream's device (0 if unknown)
 int compute_units(hipStream_t stream);

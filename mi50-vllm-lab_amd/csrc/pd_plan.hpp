@@ -34,4 +34,20 @@ constexpr int64_t kFaDealSpareUnits = 20;
 constexpr double kFaDealFixedUs = 20.0;
 constexpr double kFaDealMargin = 0.95;
 
+// Key splits of a windowed launch (pd_window_kernel): `items` workgroups per split, each of `tiles` key tiles, one per CU at a time. A
+// workgroup's set-up and stores, the merge launch, and the partials' way to memory and back, us.
+constexpr double kFwSetupUs = 16.0, kFwMergeUs = 5.0, kFwPartialUsPerMb = 0.6;
+constexpr int64_t kFwMaxSplits = 16;
+inline int64_t window_splits(int64_t items, int64_t tiles, int64_t rows, int64_t cus, bool exact) {
+    int64_t best = 1;
+    double best_us = 0;
+    for (int64_t s = 1; s <= kFwMaxSplits && (s == 1 || s * 4 <= tiles); ++s) {
+        const int64_t rounds = (items * s + cus - 1) / cus;
+        double us = (double)rounds * ((double)((tiles + s - 1) / s) * fa_times(exact).wide_tile + kFwSetupUs);
+        if (s > 1) us += kFwMergeUs + kFwPartialUsPerMb * (double)rows * (double)s * 1032 / 1e6;
+        if (s == 1 || us < best_us) best = s, best_us = us;
+    }
+    return best;
+}
+
 }  // namespace pd

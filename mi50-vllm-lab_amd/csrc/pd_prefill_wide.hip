@@ -106,14 +106,53 @@ __device__ __forceinline__ void settle_weights(half8_t (&p)[kFwRB], half8_t (&lo
         asm volatile("s_nop 1" : "+v"(p[0]), "+v"(p[1]), "+v"(p[2]), "+v"(p[3]));
 }
 
-template <bool kFast, bool kExact, bool kSplit, class T>
-__global__ void __launch_bounds__(kFwWaves * 64, 1) pd_prefill_wide_kernel(const FaParams a) {
-    constexpr int kLdsBt = kFwRing * kFwSlot;
-    constexpr int kLdsScr = kLdsBt + kFwBt * 4;  // 4 KiB per wave for the rescale of O
-    constexpr int kLdsBytes = kLdsScr + kFwWaves * 4096;
-    static_assert(kLdsBytes <= 160 * 1024, "gfx950 has 160 KiB of LDS per CU");
-    __shared__ __attribute__((aligned(16))) unsigned char lds[kLdsBytes];
+constexpr int kFwLdsBt = kFwRing * kFwSlot;
+constexpr int kFwLdsScr = kFwLdsBt + kFwBt * 4;  // 4 KiB per wave for the rescale of O
+constexpr int kFwLdsBytes = kFwLdsScr + kFwWaves * 4096;
+static_assert(kFwLdsBytes <= 160 * 1024, "gfx950 has 160 KiB of LDS per CU");
 
+// The keys that the rows [tok0, tok_last] of a sequence see with a sliding window and sinks: [lo, hi) and the first `sinks`.
+// Tiles are numbered over what is seen: [0, head) hold the sinks, from `head` on a tile lies `gap` tiles further than its number.
+struct FwSeen {
+    int lo, hi, sinks, head, gap;
+    __device__ __forceinline__ int base(int tile) const { return (tile < head ? tile : tile + gap) * kTile; }
+    // a key of the tile at kb that is seen, k itself if it is
+    __device__ __forceinline__ int near(int kb, int k) const {
+        if (k < sinks) return k;
+        return lo < kb + kTile ? min(max(k, lo), hi - 1) : sinks - 1;
+    }
+    __device__ __forceinline__ bool has(int k) const { return ((k >= lo) | (k < sinks)) & (k < hi); }
+};
+
+// Query tile x of a windowed launch: the x-th 256 rows of all sequences, whose rows [query_start[i], query_start[i + 1]) each begin a
+// tile of their own. Sequences without keys have no tiles. (A wave looks 64 sequences up at a time.)
+struct FwItem {
+    int b, tile, first, ntok;  // sequence (-1: none), its tile, its first row, its tokens
+};
+__device__ __forceinline__ FwItem fw_item(const FaWindow& w, const int* seq_lens, int G, int x) {
+    const int lane = threadIdx.x & 63;
+    unsigned before = 0;
+    for (int c = 0; c < w.num_seqs; c += 64) {
+        const int i = min(c + lane, w.num_seqs - 1);
+        const int first = max(0, w.query_start[i]), end = min(w.query_start[i + 1], w.num_tokens);
+        const bool live = c + lane < w.num_seqs && end > first && seq_lens[i] > 0;
+        const unsigned tiles = live ? (unsigned)(((int64_t)(end - first) * G + kFwRows - 1) / kFwRows) : 0u;
+        const unsigned incl = wave_scan(tiles);
+        const int k = __popcll(__ballot(before + incl <= (unsigned)x));
+        if (k < 64) {
+            const unsigned at = before + (unsigned)__builtin_amdgcn_readlane((int)(incl - tiles), k);
+            const int q0 = __builtin_amdgcn_readlane(first, k), q1 = __builtin_amdgcn_readlane(end, k);
+            return {c + k, x - (int)at, q0, q1 - q0};
+        }
+        before += (unsigned)__builtin_amdgcn_readlane((int)incl, 63);
+    }
+    return {-1, 0, 0, 0};
+}
+
+// A workgroup of pd_prefill_wide_kernel and, with kWindow, of pd_window_kernel.
+template <bool kFast, bool kExact, bool kSplit, class T, bool kWindow>
+__device__ __forceinline__ void wide_workgroup(const FaParams& a, const FaWindow& win, unsigned char* lds) {
+    constexpr int kLdsBt = kFwLdsBt, kLdsScr = kFwLdsScr;
     // Workgroups are dispatched to the 8 XCDs round robin (linear id L to XCD L % 8), and each XCD
     // has its own L2. Every query tile of a (sequence, kv head) streams the same keys, so the
     // logical workgroup index (query tile fastest) is laid out XCD by XCD: XCD x takes a
@@ -124,23 +163,37 @@ __global__ void __launch_bounds__(kFwWaves * 64, 1) pd_prefill_wide_kernel(const
     const unsigned lidx = xcd * (nwg / 8u) + min(xcd, nwg % 8u) + lin / 8u;
     // x = split * (query tiles) + query tile: the query tiles of one split and kv head (which
     // stream the same keys) stay neighbours in the XCD order
-    const int x = (int)(lidx % nx), g = (int)((lidx / nx) % ny), b = (int)(lidx / (nx * ny));
+    const int x = (int)(lidx % nx), g = (int)((lidx / nx) % ny);
     const int nqt = kSplit ? (int)nx / a.nsplit : (int)nx;
-    const int qt = kSplit ? x % nqt : x, split = kSplit ? x / nqt : 0;
+    const int xt = kSplit ? x % nqt : x, split = kSplit ? x / nqt : 0;
     const int tid = threadIdx.x, l = tid & 63;
     const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int G = a.G;
-    // rows of this workgroup: [row0, row0 + nrow) of the sequence's Sq * G (token, head) rows
+    int b = (int)(lidx / (nx * ny)), qt = xt, ntok = a.Sq, first = 0;
+    if constexpr (kWindow) {
+        const FwItem item = fw_item(win, a.seq_lens, G, xt);
+        if (item.b < 0) return;
+        b = item.b, qt = item.tile, ntok = item.ntok, first = item.first;
+    }
+    // rows of this workgroup: [row0, row0 + nrow) of the sequence's (token, head) rows
     const int64_t row0 = (int64_t)qt * kFwRows;
-    const int nrow = (int)min((int64_t)kFwRows, (int64_t)a.Sq * G - row0);
+    const int nrow = (int)min((int64_t)kFwRows, (int64_t)ntok * G - row0);
     const int tok0 = (int)(row0 / G), tok_last = (int)((row0 + nrow - 1) / G);
     const int tok0_row = (int)(row0 - (int64_t)tok0 * G);  // rows of the first token that come before
     const int seq_len = a.seq_lens[b];
-    const int qabs = a.q_abs ? a.q_abs[b] : seq_len - a.Sq;
+    const int qabs = !kWindow && a.q_abs ? a.q_abs[b] : seq_len - ntok;
     // keys any row can see: [0, min(seq_len, last row's position + 1))
     const int hi = min(seq_len, qabs + tok_last + 1);
-    const int ntiles = hi > 0 ? (hi - 1) / kTile + 1 : 0;
+    int ntiles = hi > 0 ? (hi - 1) / kTile + 1 : 0;
     const int pmin = qabs + tok0;                      // smallest row position
+    FwSeen seen = {0, hi, 0, 0, 0};
+    if constexpr (kWindow) {
+        seen.lo = max(0, pmin - win.window + 1);
+        seen.sinks = max(0, min(win.sinks, hi));
+        seen.head = (seen.sinks + kTile - 1) / kTile;
+        seen.gap = max(0, seen.lo / kTile - seen.head);
+        ntiles = max(0, ntiles - seen.gap);
+    }
     // this workgroup's run of key tiles [t0, t1): all of them unless the keys are split
     const int per = kSplit ? (ntiles + a.nsplit - 1) / a.nsplit : ntiles;
     const int t0 = kSplit ? min(ntiles, split * per) : 0, t1 = kSplit ? min(ntiles, t0 + per) : ntiles;
@@ -173,8 +226,8 @@ __global__ void __launch_bounds__(kFwWaves * 64, 1) pd_prefill_wide_kernel(const
 #pragma unroll
     for (int rb = 0; rb < kFwRB; ++rb) {
         const Row r = row_of(rb);
-        const T* qrow = static_cast<const T*>(a.q) + (int64_t)b * a.q_sb + (int64_t)(g * G + r.head) * a.q_sh +
-                        (int64_t)r.tok * a.q_st;
+        const T* qrow = static_cast<const T*>(a.q) + (kWindow ? (int64_t)first * a.q_st : (int64_t)b * a.q_sb) +
+                        (int64_t)(g * G + r.head) * a.q_sh + (int64_t)r.tok * a.q_st;
 #pragma unroll
         for (int st = 0; st < 8; ++st) {
             const half8_t v = load_q8<T>(qrow + 64 * (st >> 1) + 16 * (l >> 4) + 8 * (st & 1));
@@ -204,9 +257,9 @@ __global__ void __launch_bounds__(kFwWaves * 64, 1) pd_prefill_wide_kernel(const
             pt.in_lds = a.bt32 && nblk <= kFwBt;
             if (pt.in_lds) {
                 for (int i = tid; i < nblk; i += kFwWaves * 64) {
-                    const int kb = (t0 + (i >> 1)) * kTile;
+                    const int kb = kWindow ? seen.base(t0 + (i >> 1)) : (t0 + (i >> 1)) * kTile;
                     const int klast = min(kb + kTile - 1, hi - 1);
-                    const int key0 = min(kb + 16 * (i & 1), klast) & ~15;
+                    const int key0 = (kWindow ? seen.near(kb, kb + 16 * (i & 1)) : min(kb + 16 * (i & 1), klast)) & ~15;
                     const int lb = a.bs_shift >= 0 ? key0 >> a.bs_shift : key0 / a.block_size;
                     const int64_t off = (int64_t)bt_glob[lb] * a.k_sb + (int64_t)(key0 - lb * a.block_size) * a.k_ss;
                     dst[i] = (int)(unsigned)((uint64_t)off >> 3);
@@ -318,7 +371,25 @@ __global__ void __launch_bounds__(kFwWaves * 64, 1) pd_prefill_wide_kernel(const
         for (int rb = 0; rb < kFwRB; ++rb)
 #pragma unroll
             for (int e = 0; e < 8; ++e) sv[rb][e] = __builtin_fmaf(sacc[rb][e >> 2][e & 3], ks[e], nm_run[rb]);
-        if (n >= n_int) {  // the tile crosses the causal diagonal or seq_len
+        if constexpr (kWindow) {
+            const int kb = seen.base(n);
+            if (kb + kTile - 1 > pmin || (kb + kTile > seen.sinks && qabs + tok_last - kb >= win.window)) {
+                // some row does not see all of the tile; keys that none sees may hold garbage scales: v_scale 0
+                const int key = kb + 4 * (lane_here() >> 4);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) vs[e] = seen.has(key + 16 * (e >> 2) + (e & 3)) ? vs[e] : 0.f;
+#pragma unroll
+                for (int rb = 0; rb < kFwRB; ++rb) {
+                    const Row row = row_of(rb);
+                    const int pos = qabs + row.tok, last = row.valid ? min(hi - 1, pos) : -1, from = pos - win.window;
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        const int k = key + 16 * (e >> 2) + (e & 3);
+                        sv[rb][e] = (k <= last) & ((k > from) | (k < seen.sinks)) ? sv[rb][e] : kNegInf;
+                    }
+                }
+            }
+        } else if (n >= n_int) {  // the tile crosses the causal diagonal or seq_len
             const int key = n * kTile + 4 * (lane_here() >> 4);
             // keys past seq_len may hold garbage scales (even NaN): v_scale 0 makes their P' 0
 #pragma unroll
@@ -430,14 +501,14 @@ __global__ void __launch_bounds__(kFwWaves * 64, 1) pd_prefill_wide_kernel(const
             if constexpr (kLds) {
                 return gbase + ((int64_t)(unsigned)__builtin_amdgcn_readfirstlane(entry) << 3);
             } else {
-                const int kb = n * kTile, klast = min(kb + kTile - 1, hi - 1);
-                const int key0 = min(kb + 16 * u, klast) & ~15;
+                const int kb = kWindow ? seen.base(n) : n * kTile, klast = min(kb + kTile - 1, hi - 1);
+                const int key0 = (kWindow ? seen.near(kb, kb + 16 * u) : min(kb + 16 * u, klast)) & ~15;
                 const int lb = a.bs_shift >= 0 ? key0 >> a.bs_shift : key0 / a.block_size;
                 return gbase + (int64_t)pt.glob[lb] * a.k_sb + (int64_t)(key0 - lb * a.block_size) * a.k_ss;
             }
         };
         auto row_base = [&](int n, int row) __attribute__((always_inline)) -> const int8_t* {
-            const int key = min(n * kTile + row, hi - 1);
+            const int key = kWindow ? seen.near(seen.base(n), seen.base(n) + row) : min(n * kTile + row, hi - 1);
             const int lb = a.bs_shift >= 0 ? key >> a.bs_shift : key / a.block_size;
             return gbase + pt.get<kLds>(lb) * a.k_sb + (int64_t)(key - lb * a.block_size) * a.k_ss;
         };
@@ -532,7 +603,7 @@ __global__ void __launch_bounds__(kFwWaves * 64, 1) pd_prefill_wide_kernel(const
         if (!row.valid) continue;
         const int tok = row.tok, head = g * G + row.head;
         if constexpr (kSplit) {
-            const int64_t pr = (((int64_t)b * a.Sq + tok) * a.Hq + head) * a.nsplit + split;
+            const int64_t pr = (((kWindow ? (int64_t)first : (int64_t)b * a.Sq) + tok) * a.Hq + head) * a.nsplit + split;
             float* prow = a.part_o + pr * kDim + 4 * lg;
 #pragma unroll
             for (int m = 0; m < 16; ++m) *reinterpret_cast<float4_t*>(prow + 16 * m) = oacc[rb][m];
@@ -542,11 +613,72 @@ __global__ void __launch_bounds__(kFwWaves * 64, 1) pd_prefill_wide_kernel(const
             }
         } else {
             const float inv = l_row > 0.f ? 1.f / l_row : 0.f;
-            T* orow = static_cast<T*>(a.out) + (int64_t)b * a.o_sb + (int64_t)tok * a.o_st + (int64_t)head * a.o_sh + 4 * lg;
+            T* orow = static_cast<T*>(a.out) + (kWindow ? (int64_t)first * a.o_st : (int64_t)b * a.o_sb) + (int64_t)tok * a.o_st +
+                      (int64_t)head * a.o_sh + 4 * lg;
 #pragma unroll
             for (int m = 0; m < 16; ++m) store_out4<T>(orow + 16 * m, oacc[rb][m] * inv);
         }
     }
+}
+
+template <bool kFast, bool kExact, bool kSplit, class T>
+__global__ void __launch_bounds__(kFwWaves * 64, 1) pd_prefill_wide_kernel(const FaParams a) {
+    __shared__ __attribute__((aligned(16))) unsigned char lds[kFwLdsBytes];
+    wide_workgroup<kFast, kExact, kSplit, T, false>(a, FaWindow{}, lds);
+}
+
+// Chunks whose rows see a sliding window and the first `sinks` keys: the row at position p sees key k <= p if p - k < window or
+// k < sinks. A query tile streams the tiles that hold a key that one of its rows sees, those of the sinks, then the window's (window + 43
+// keys for 256 rows of 6 heads), so a chunk's time goes with tokens x window, whatever lies before; pages that hold nothing
+// seen are never addressed. Tiles at the window's two ends and the last of the sinks are masked row by row, the others
+// are not. Several sequences' rows lie one after the other; which a workgroup has is looked up on the device, so that a captured
+// launch takes any batch of as many rows and sequences.
+template <bool kFast, bool kExact, bool kSplit>
+__global__ void __launch_bounds__(kFwWaves * 64, 1) pd_window_kernel(const FaParams a, const FaWindow win) {
+    __shared__ __attribute__((aligned(16))) unsigned char lds[kFwLdsBytes];
+    wide_workgroup<kFast, kExact, kSplit, _Float16, true>(a, win, lds);
+}
+
+// Log-sum-exp merge of a split windowed launch: a wave per (token, head) row, lane l owning dims 4 l .. 4 l + 3; M = max_s m_s,
+// out = sum_s 2^(m_s - M) O_s / sum_s 2^(m_s - M) l_s, 0 for a row that saw no key. Rows outside the sequences, and those of
+// sequences without keys, are left alone.
+__global__ void __launch_bounds__(256) pd_window_combine_kernel(const FaParams a, const FaWindow win) {
+    constexpr int kBatch = 8;
+    const int lane = threadIdx.x & 63, head = (int)blockIdx.y;
+    const int tok = (int)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+    if (tok >= win.num_tokens) return;
+    bool mine = false;
+    for (int c = 0; c < win.num_seqs; c += 64) {
+        const int i = min(c + lane, win.num_seqs - 1);
+        const int first = win.query_start[i], end = win.query_start[i + 1];
+        mine = mine || (tok >= first && tok < end && a.seq_lens[i] > 0);
+    }
+    if (__ballot(mine) == 0) return;
+    const int64_t base = ((int64_t)tok * a.Hq + head) * a.nsplit;
+    const float m_mine = lane < a.nsplit ? a.part_m[base + lane] : kNegInf;
+    const float l_mine = lane < a.nsplit ? a.part_l[base + lane] : 0.f;
+    float M = m_mine;
+#pragma unroll
+    for (int o = 32; o >= 1; o >>= 1) M = fmaxf(M, __shfl_xor(M, o, 64));
+    const float w_mine = m_mine != kNegInf ? exp2f(m_mine - M) : 0.f;
+    float L = w_mine * l_mine;
+#pragma unroll
+    for (int o = 32; o >= 1; o >>= 1) L += __shfl_xor(L, o, 64);
+    float4_t acc = (float4_t)0.f;
+    const float4_t* po = reinterpret_cast<const float4_t*>(a.part_o + base * kDim) + lane;
+    for (int s0 = 0; s0 < a.nsplit; s0 += kBatch) {
+        float4_t o[kBatch];
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) o[i] = s0 + i < a.nsplit ? po[(int64_t)(s0 + i) * (kDim / 4)] : (float4_t)0.f;
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) {
+            const float wi = __shfl(w_mine, min(s0 + i, 63), 64);
+            acc += (s0 + i < a.nsplit && wi != 0.f) ? wi * o[i] : (float4_t)0.f;
+        }
+    }
+    const float inv = L > 0.f ? 1.f / L : 0.f;
+    _Float16* orow = static_cast<_Float16*>(a.out) + (int64_t)tok * a.o_st + (int64_t)head * a.o_sh;
+    store_out4<_Float16>(orow + 4 * lane, acc * inv);
 }
 
 // ---------------------------------------------------------------------------------------
@@ -580,6 +712,33 @@ hipError_t launch_prefill_wide(const FaParams& p, int batch, int heads_kv, int d
         else
             launch_wide<true, float>(p, grid, stream, fast, exact);
     }
+    return hipGetLastError();
+}
+
+template <bool kSplit>
+static void launch_window_split(const FaParams& p, const FaWindow& w, dim3 grid, hipStream_t stream, bool fast, bool exact) {
+    const dim3 block(kFwWaves * 64);
+    if (fast && !exact)
+        hipLaunchKernelGGL((pd_window_kernel<true, false, kSplit>), grid, block, 0, stream, p, w);
+    else if (!exact)
+        hipLaunchKernelGGL((pd_window_kernel<false, false, kSplit>), grid, block, 0, stream, p, w);
+    else if (fast)
+        hipLaunchKernelGGL((pd_window_kernel<true, true, kSplit>), grid, block, 0, stream, p, w);
+    else
+        hipLaunchKernelGGL((pd_window_kernel<false, true, kSplit>), grid, block, 0, stream, p, w);
+}
+
+hipError_t launch_window(const FaParams& p, const FaWindow& w, int heads_kv, hipStream_t stream, bool exact) {
+    const dim3 grid((unsigned)(window_tiles(w.num_tokens, w.num_seqs, p.G) * p.nsplit), heads_kv);
+    const bool fast = fast_block_table(p.block_size, p.k_ss);
+    if (p.nsplit == 1) {
+        launch_window_split<false>(p, w, grid, stream, fast, exact);
+        return hipGetLastError();
+    }
+    launch_window_split<true>(p, w, grid, stream, fast, exact);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+    hipLaunchKernelGGL(pd_window_combine_kernel, dim3((unsigned)((w.num_tokens + 3) / 4), p.Hq), dim3(256), 0, stream, p, w);
     return hipGetLastError();
 }
 

@@ -127,6 +127,15 @@ PyObject* guarded(F&& f) {
     return nullptr;
 }
 
+// Whether all tensors lie on the first one's GPU; false with a Python error set.
+bool same_gpu(PyObject* const* o, int n) {
+    const c10::Device dev = THPVariable_Unpack(o[0]).device();
+    bool ok = dev.is_cuda();
+    for (int i = 1; i < n; ++i) ok = ok && THPVariable_Unpack(o[i]).device() == dev;
+    if (!ok) PyErr_SetString(PyExc_RuntimeError, "all tensors must be on one GPU");
+    return ok;
+}
+
 // decode(entry, q, key_cache, value_cache, k_scale, v_scale, block_table, seq_lens, query_start_loc, out, scale,
 //        part_o, part_m, part_l, num_seqs, qmax, nsplit, window, causal)
 PyObject* decode(PyObject*, PyObject* const* a, Py_ssize_t n) {
@@ -253,6 +262,49 @@ PyObject* prefill_balanced(PyObject*, PyObject* const* a, Py_ssize_t n) {
     });
 }
 
+// forward_window(entry, splits entry, q, key_cache, value_cache, block_table, seq_lens, query_start_loc, out, scale, window, sinks,
+//                nsplit (0: planned), exact): pth_fa_forward_window with its workspace from torch's allocator. Planned splits
+// whose workspace cannot be had run unsplit.
+PyObject* forward_window(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    return guarded([&]() -> PyObject* {
+        decltype(&pth_fa_forward_window) fn;
+        decltype(&pth_fa_window_splits) splits;
+        pd_tensor t[7], wd{};
+        double scale;
+        int64_t window, sinks, nsplit, exact;
+        if (!count_is(n, 14) || !entry(a[0], fn) || !entry(a[1], splits) || !describe_all(a + 2, t, 7) || !same_gpu(a + 2, 7) ||
+            !as_double(a[9], scale) || !as_int64(a[10], window) || !as_int64(a[11], sinks) || !as_int64(a[12], nsplit) ||
+            !as_int64(a[13], exact))
+            return nullptr;
+        OnDevice dev(a[2]);
+        const bool planned = nsplit == 0, shaped = t[0].ndim == 3 && t[1].ndim == 4 && t[3].ndim == 2 && t[5].ndim == 1;
+        const int64_t seqs = shaped ? t[5].sizes[0] - 1 : 0;
+        if (planned)
+            nsplit = shaped ? splits(t[0].sizes[0], seqs, t[0].sizes[1], t[1].sizes[2], window, sinks, t[3].sizes[1] * t[1].sizes[1], exact) : 1;
+        at::Tensor ws;
+        if (shaped && nsplit > 1 && nsplit <= 64) {
+            try {
+                ws = at::empty({t[0].sizes[0] * t[0].sizes[1] * nsplit * 258}, THPVariable_Unpack(a[2]).options().dtype(at::kFloat));
+                wd.data = ws.data_ptr();
+                wd.dtype = PD_DTYPE_FP32;
+                wd.ndim = 1;
+                wd.sizes[0] = ws.numel();
+                wd.strides[0] = 1;
+            } catch (const c10::OutOfMemoryError&) {
+                if (!planned) throw;
+                nsplit = 1;
+            }
+        }
+        char err[256] = "";
+        int rc;
+        Py_BEGIN_ALLOW_THREADS;
+        rc = fn(&t[0], &t[1], &t[2], &t[3], &t[4], scale, &t[5], &t[6], wd.data ? &wd : nullptr, seqs, window, sinks, nsplit, exact,
+                dev.stream, err, (int)sizeof err);
+        Py_END_ALLOW_THREADS;
+        return done(rc, err);
+    });
+}
+
 // cache_write(entry, key, value, key_cache, value_cache, k_scale, v_scale, slot_mapping)
 PyObject* cache_write(PyObject*, PyObject* const* a, Py_ssize_t n) {
     return guarded([&]() -> PyObject* {
@@ -267,15 +319,6 @@ PyObject* cache_write(PyObject*, PyObject* const* a, Py_ssize_t n) {
         Py_END_ALLOW_THREADS;
         return done(rc, err);
     });
-}
-
-// Whether all tensors lie on the first one's GPU; false with a Python error set.
-bool same_gpu(PyObject* const* o, int n) {
-    const c10::Device dev = THPVariable_Unpack(o[0]).device();
-    bool ok = dev.is_cuda();
-    for (int i = 1; i < n; ++i) ok = ok && THPVariable_Unpack(o[i]).device() == dev;
-    if (!ok) PyErr_SetString(PyExc_RuntimeError, "all tensors must be on one GPU");
-    return ok;
 }
 
 // decode_lse(entry, q, key_cache, value_cache, k_scale, v_scale, block_table, seq_lens, query_start_loc, out, part_o,
@@ -709,6 +752,7 @@ PyMethodDef methods[] = {
     PD_METHOD(prefill, "pth_fa_forward / pth_fa_forward_exact on torch tensors"),
     PD_METHOD(prefill_split, "pth_fa_forward_split on torch tensors"),
     PD_METHOD(prefill_balanced, "pth_fa_forward_balanced on torch tensors"),
+    PD_METHOD(forward_window, "pth_fa_forward_window on torch tensors"),
     PD_METHOD(cache_write, "pth_cache_write on torch tensors"),
     PD_METHOD(decode_lse, "pth_dec_decode_lse on torch tensors"),
     PD_METHOD(decode_sinks, "pth_dec_decode_sinks on torch tensors"),

@@ -59,6 +59,8 @@ EXPORTED_SYMBOLS = (
     "pth_fa_forward_split",
     "pth_fa_forward_balanced",
     "pth_fa_balanced_workspace",
+    "pth_fa_forward_window",
+    "pth_fa_window_splits",
     "pth_cache_write",
     "pth_cache_write_rotary",
     "pth_cache_key_weights",
@@ -148,6 +150,10 @@ def load_library(path: str | None = None) -> ctypes.CDLL:
     lib.pth_fa_forward_balanced.restype = c_int
     lib.pth_fa_balanced_workspace.argtypes = [ctypes.c_int64, ip] + [ctypes.c_int64] * 5
     lib.pth_fa_balanced_workspace.restype = ctypes.c_int64
+    lib.pth_fa_forward_window.argtypes = [tp] * 5 + [c_double, tp, tp, tp] + [ctypes.c_int64] * 5 + [vp, ctypes.c_char_p, c_int]
+    lib.pth_fa_forward_window.restype = c_int
+    lib.pth_fa_window_splits.argtypes = [ctypes.c_int64] * 8
+    lib.pth_fa_window_splits.restype = ctypes.c_int64
     lib.pth_cache_write.argtypes = [tp] * 7 + [vp, ctypes.c_char_p, c_int]
     lib.pth_cache_write.restype = c_int
     lib.pth_dec_decode_lse.argtypes = [tp] * 9 + [c_double, tp, tp, tp, tp] + [ctypes.c_int64] * 5 + [vp, ctypes.c_char_p, c_int]
@@ -174,7 +180,8 @@ def load_library(path: str | None = None) -> ctypes.CDLL:
     lib.pth_dec_version.restype = ctypes.c_char_p
     _entries.update({name: ctypes.cast(getattr(lib, name), vp).value
                      for name in ("pth_dec_decode", "pth_fa_forward", "pth_fa_forward_exact", "pth_fa_forward_split",
-                                  "pth_fa_forward_balanced", "pth_fa_balanced_workspace", "pth_cache_write", "pth_dec_decode_lse",
+                                  "pth_fa_forward_balanced", "pth_fa_balanced_workspace", "pth_fa_forward_window",
+                                  "pth_fa_window_splits", "pth_cache_write", "pth_dec_decode_lse",
                                   "pth_dec_decode_sinks", "pth_dec_decode_shared", "pth_cache_write_rotary", "pth_cache_key_weights", "pth_cache_evict",
                                   "pth_cache_write_norm_rotary", "pth_cache_fork_pages", "pth_cache_compact_pages",
                                   "pth_cache_pages_workspace")})
@@ -413,6 +420,25 @@ def forward_rows(query: torch.Tensor, key_cache: torch.Tensor, value_cache: torc
                                      max_keys, n, 1 if exact else 0):
             return True
     return False
+
+
+def forward_window(query: torch.Tensor, key_cache: torch.Tensor, value_cache: torch.Tensor, block_table: torch.Tensor,
+                   seq_lens: torch.Tensor, scale: float, query_start_loc: torch.Tensor, out: torch.Tensor, window: int, sinks: int = 0,
+                   exact: bool = False, nsplit: int | None = None) -> None:
+    """Causal prefill of rows that see a sliding window and the first keys (no counterpart in the reference, whose engine leaves
+    windowed layers' prefill to Triton).
+
+    Sequence i has rows [query_start_loc[i], query_start_loc[i + 1]) of query and out (fp16 [T, Hq, 256]), the last tokens of its
+    seq_lens[i] keys; the row at position p sees key k <= p if p - k < window or k < sinks. query_start_loc int32 [sequences + 1], seq_lens and
+    block_table are read on the device, as decode reads them, so a captured call takes any batch of as many rows and sequences. Rows
+    outside the sequences and of sequences without keys are left alone. Pages in which no row sees a key are not addressed.
+    exact: the softmax weights enter P.V as decode's fp16 hi + lo instead of one fp16, for outlier-heavy caches, at about 20 % more time.
+    nsplit: key splits per query tile, with a workspace from torch's allocator; None plans them by the call's sizes (splits of a
+    planned call whose workspace cannot be had are left).
+    """
+    native().forward_window(_entry("pth_fa_forward_window"), _entry("pth_fa_window_splits"), query, key_cache, value_cache, block_table,
+                            seq_lens, query_start_loc, out, scale, int(window), int(sinks), 0 if nsplit is None else int(nsplit),
+                            1 if exact else 0)
 
 
 def cache_write(key: torch.Tensor, value: torch.Tensor, key_cache: torch.Tensor, value_cache: torch.Tensor,
