@@ -112,10 +112,16 @@ constexpr int kFwLdsBytes = kFwLdsScr + kFwWaves * 4096;
 static_assert(kFwLdsBytes <= 160 * 1024, "gfx950 has 160 KiB of LDS per CU");
 
 // The keys that the rows [tok0, tok_last] of a sequence see with a sliding window and sinks: [lo, hi) and the first `sinks`.
-// Tiles are numbered over what is seen: [0, head) hold the sinks, from `head` on a tile lies `gap` tiles further than its number.
+// Tiles are numbered over what is seen: [0, head) hold the sinks, from `head` on a tile lies `gap` tiles further than its number. They are
+// taken from the first one on that every row sees all of, and those before it last: the rows' running maxima then start from 32
+// keys each, not from the few of the sinks or of the window's ragged end, and seldom have to be raised, which rescales O.
 struct FwSeen {
     int lo, hi, sinks, head, gap;
-    __device__ __forceinline__ int base(int tile) const { return (tile < head ? tile : tile + gap) * kTile; }
+    int turn, tiles;  // tile n is the (n + turn)-th of `tiles`
+    __device__ __forceinline__ int base(int n) const {
+        const int tile = n + turn - (n + turn >= tiles ? tiles : 0);
+        return (tile < head ? tile : tile + gap) * kTile;
+    }
     // a key of the tile at kb that is seen, k itself if it is
     __device__ __forceinline__ int near(int kb, int k) const {
         if (k < sinks) return k;
@@ -124,57 +130,101 @@ struct FwSeen {
     __device__ __forceinline__ bool has(int k) const { return ((k >= lo) | (k < sinks)) & (k < hi); }
 };
 
-// Query tile x of a windowed launch: the x-th 256 rows of all sequences, whose rows [query_start[i], query_start[i + 1]) each begin a
-// tile of their own. Sequences without keys have no tiles. (A wave looks 64 sequences up at a time.)
+// Query tiles of a windowed launch: each sequence's rows [query_start[i], query_start[i + 1]) in runs of 256, sequence by sequence;
+// sequences without keys have none. (A wave looks 64 sequences up at a time.)
 struct FwItem {
-    int b, tile, first, ntok;  // sequence (-1: none), its tile, its first row, its tokens
+    int b, tile, first, ntok;  // sequence, its query tile, its first row, its tokens
 };
-__device__ __forceinline__ FwItem fw_item(const FaWindow& w, const int* seq_lens, int G, int x) {
+struct FwTiles {
+    unsigned tiles0, incl0;    // this lane's sequence (of the first 64): its tiles, the tiles up to and with it
+    int first0, end0;
+    unsigned total;
+};
+__device__ __forceinline__ unsigned fw_tiles(const FaWindow& w, const int* seq_lens, int G, int i, int& first, int& end) {
+    const int c = min(i, w.num_seqs - 1);
+    first = max(0, w.query_start[c]);
+    end = min(w.query_start[c + 1], w.num_tokens);
+    const bool live = i < w.num_seqs && end > first && seq_lens[c] > 0;
+    return live ? (unsigned)(((int64_t)(end - first) * G + kFwRows - 1) / kFwRows) : 0u;
+}
+__device__ __forceinline__ FwTiles fw_count(const FaWindow& w, const int* seq_lens, int G) {
+    const int lane = threadIdx.x & 63;
+    FwTiles t;
+    t.tiles0 = fw_tiles(w, seq_lens, G, lane, t.first0, t.end0);
+    t.incl0 = wave_scan(t.tiles0);
+    t.total = (unsigned)__builtin_amdgcn_readlane((int)t.incl0, 63);
+    for (int c = 64; c < w.num_seqs; c += 64) {
+        int first, end;
+        t.total += (unsigned)__builtin_amdgcn_readlane((int)wave_scan(fw_tiles(w, seq_lens, G, c + lane, first, end)), 63);
+    }
+    return t;
+}
+// Query tile x < total.
+__device__ __forceinline__ FwItem fw_item(const FaWindow& w, const int* seq_lens, int G, const FwTiles& t, unsigned x) {
     const int lane = threadIdx.x & 63;
     unsigned before = 0;
-    for (int c = 0; c < w.num_seqs; c += 64) {
-        const int i = min(c + lane, w.num_seqs - 1);
-        const int first = max(0, w.query_start[i]), end = min(w.query_start[i + 1], w.num_tokens);
-        const bool live = c + lane < w.num_seqs && end > first && seq_lens[i] > 0;
-        const unsigned tiles = live ? (unsigned)(((int64_t)(end - first) * G + kFwRows - 1) / kFwRows) : 0u;
-        const unsigned incl = wave_scan(tiles);
-        const int k = __popcll(__ballot(before + incl <= (unsigned)x));
+    for (int c = 0;; c += 64) {
+        int first = t.first0, end = t.end0;
+        unsigned tiles = t.tiles0, incl = t.incl0;
+        if (c > 0) {
+            tiles = fw_tiles(w, seq_lens, G, c + lane, first, end);
+            incl = wave_scan(tiles);
+        }
+        const int k = __popcll(__ballot(before + incl <= x));
         if (k < 64) {
             const unsigned at = before + (unsigned)__builtin_amdgcn_readlane((int)(incl - tiles), k);
             const int q0 = __builtin_amdgcn_readlane(first, k), q1 = __builtin_amdgcn_readlane(end, k);
-            return {c + k, x - (int)at, q0, q1 - q0};
+            return {c + k, (int)(x - at), q0, q1 - q0};
         }
         before += (unsigned)__builtin_amdgcn_readlane((int)incl, 63);
     }
-    return {-1, 0, 0, 0};
+}
+// The place of workgroup `lin` of `count` in the order of the work: the 8 XCDs, which the hardware deals workgroups to in turn, take 32
+// neighbours (one per CU) each, in turn as well, so that what runs at once on an XCD shares an L2's keys, and no XCD
+// gets only the long or only the short ones; the rest of less than 256 goes to them in equal runs.
+__device__ __forceinline__ unsigned fw_order(unsigned lin, unsigned count) {
+    const unsigned xcd = lin % 8u, whole = count / 256u * 256u;
+    if (lin < whole) return lin / 256u * 256u + xcd * 32u + lin / 8u % 32u;
+    const unsigned rest = count - whole;
+    return whole + xcd * (rest / 8u) + min(xcd, rest % 8u) + (lin - whole) / 8u;
 }
 
 // A workgroup of pd_prefill_wide_kernel and, with kWindow, of pd_window_kernel.
 template <bool kFast, bool kExact, bool kSplit, class T, bool kWindow>
 __device__ __forceinline__ void wide_workgroup(const FaParams& a, const FaWindow& win, unsigned char* lds) {
     constexpr int kLdsBt = kFwLdsBt, kLdsScr = kFwLdsScr;
-    // Workgroups are dispatched to the 8 XCDs round robin (linear id L to XCD L % 8), and each XCD
-    // has its own L2. Every query tile of a (sequence, kv head) streams the same keys, so the
-    // logical workgroup index (query tile fastest) is laid out XCD by XCD: XCD x takes a
-    // contiguous range of it, and the query tiles sharing a kv head mostly share an L2.
-    const unsigned nx = gridDim.x, ny = gridDim.y, nwg = nx * ny * gridDim.z;
-    const unsigned lin = blockIdx.x + nx * (blockIdx.y + ny * blockIdx.z);
-    const unsigned xcd = lin % 8u;
-    const unsigned lidx = xcd * (nwg / 8u) + min(xcd, nwg % 8u) + lin / 8u;
-    // x = split * (query tiles) + query tile: the query tiles of one split and kv head (which
-    // stream the same keys) stay neighbours in the XCD order
-    const int x = (int)(lidx % nx), g = (int)((lidx / nx) % ny);
-    const int nqt = kSplit ? (int)nx / a.nsplit : (int)nx;
-    const int xt = kSplit ? x % nqt : x, split = kSplit ? x / nqt : 0;
+    int x, g, b, qt, split, ntok = a.Sq, first = 0;
+    if constexpr (kWindow) {
+        // The order of the work: runs of 32 query tiles, the last tiles first (those of a fresh prompt see the most keys), and for each
+        // run all kv heads and splits.
+        const FwTiles tiles = fw_count(win, a.seq_lens, a.G);
+        const unsigned lin = blockIdx.x + gridDim.x * blockIdx.y, each = gridDim.y * (unsigned)a.nsplit, count = tiles.total * each;
+        if (lin >= count) return;
+        const unsigned at = fw_order(lin, count), run = at / (32u * each), width = min(32u, tiles.total - 32u * run);
+        const unsigned in = at - run * 32u * each, job = in / width;
+        x = (int)(tiles.total - 1 - (32u * run + in - job * width));
+        g = (int)(job / (unsigned)a.nsplit);
+        split = (int)(job - (unsigned)g * (unsigned)a.nsplit);
+        const FwItem item = fw_item(win, a.seq_lens, a.G, tiles, (unsigned)x);
+        b = item.b, qt = item.tile, ntok = item.ntok, first = item.first;
+    } else {
+        // Workgroups are dispatched to the 8 XCDs round robin (linear id L to XCD L % 8), and each XCD
+        // has its own L2. Every query tile of a (sequence, kv head) streams the same keys, so the
+        // logical workgroup index (query tile fastest) is laid out XCD by XCD: XCD x takes a
+        // contiguous range of it, and the query tiles sharing a kv head mostly share an L2.
+        const unsigned nx = gridDim.x, ny = gridDim.y, nwg = nx * ny * gridDim.z;
+        const unsigned lin = blockIdx.x + nx * (blockIdx.y + ny * blockIdx.z);
+        const unsigned xcd = lin % 8u;
+        const unsigned lidx = xcd * (nwg / 8u) + min(xcd, nwg % 8u) + lin / 8u;
+        // x = split * (query tiles) + query tile: the query tiles of one split and kv head (which
+        // stream the same keys) stay neighbours in the XCD order
+        x = (int)(lidx % nx), g = (int)((lidx / nx) % ny), b = (int)(lidx / (nx * ny));
+        const int nqt = kSplit ? (int)nx / a.nsplit : (int)nx;
+        qt = kSplit ? x % nqt : x, split = kSplit ? x / nqt : 0;
+    }
     const int tid = threadIdx.x, l = tid & 63;
     const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int G = a.G;
-    int b = (int)(lidx / (nx * ny)), qt = xt, ntok = a.Sq, first = 0;
-    if constexpr (kWindow) {
-        const FwItem item = fw_item(win, a.seq_lens, G, xt);
-        if (item.b < 0) return;
-        b = item.b, qt = item.tile, ntok = item.ntok, first = item.first;
-    }
     // rows of this workgroup: [row0, row0 + nrow) of the sequence's (token, head) rows
     const int64_t row0 = (int64_t)qt * kFwRows;
     const int nrow = (int)min((int64_t)kFwRows, (int64_t)ntok * G - row0);
@@ -186,13 +236,15 @@ __device__ __forceinline__ void wide_workgroup(const FaParams& a, const FaWindow
     const int hi = min(seq_len, qabs + tok_last + 1);
     int ntiles = hi > 0 ? (hi - 1) / kTile + 1 : 0;
     const int pmin = qabs + tok0;                      // smallest row position
-    FwSeen seen = {0, hi, 0, 0, 0};
+    FwSeen seen = {0, hi, 0, 0, 0, 0, 0};
     if constexpr (kWindow) {
         seen.lo = max(0, pmin - win.window + 1);
         seen.sinks = max(0, min(win.sinks, hi));
         seen.head = (seen.sinks + kTile - 1) / kTile;
         seen.gap = max(0, seen.lo / kTile - seen.head);
-        ntiles = max(0, ntiles - seen.gap);
+        seen.tiles = ntiles = max(0, ntiles - seen.gap);
+        const int whole = (max(0, qabs + tok_last - win.window + 1) + kTile - 1) / kTile;  // the window's first tile that all rows see
+        if (whole > 0 && (whole + 1) * kTile <= pmin + 1 && whole - seen.gap >= seen.head) seen.turn = whole - seen.gap;
     }
     // this workgroup's run of key tiles [t0, t1): all of them unless the keys are split
     const int per = kSplit ? (ntiles + a.nsplit - 1) / a.nsplit : ntiles;
