@@ -35,8 +35,10 @@ constexpr double kFaDealFixedUs = 20.0;
 constexpr double kFaDealMargin = 0.95;
 
 // Key splits of a windowed launch (pd_window_kernel): `items` workgroups per split, each of `tiles` key tiles, one per CU at a time. A
-// workgroup's set-up and stores, the merge launch, and the partials' way to memory and back, us.
-constexpr double kFwSetupUs = 16.0, kFwMergeUs = 5.0, kFwPartialUsPerMb = 0.6;
+// workgroup's set-up and stores, the merge launch, and the partials' way to memory and back, us. Measured and rated (24 q / 4 kv heads): 64
+// tokens over 2,048 keys 137 unsplit, 40 at 10 splits, 39 at 16 (144, 39, 38); 600 over 4,096 261, 156 at 2, 100 at 4 (268, 157,
+// 103); 1,024 260 and 164 at 2 (268, 160), 2 rounds at 3 217; 4,096 521 and 489 at 2 (537, 487).
+constexpr double kFwSetupUs = 18.0, kFwMergeUs = 5.0, kFwPartialUsPerMb = 0.25;
 constexpr int64_t kFwMaxSplits = 16;
 inline int64_t window_splits(int64_t items, int64_t tiles, int64_t rows, int64_t cus, bool exact) {
     int64_t best = 1;

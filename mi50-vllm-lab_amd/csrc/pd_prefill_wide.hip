@@ -109,7 +109,9 @@ __device__ __forceinline__ void settle_weights(half8_t (&p)[kFwRB], half8_t (&lo
 constexpr int kFwLdsBt = kFwRing * kFwSlot;
 constexpr int kFwLdsScr = kFwLdsBt + kFwBt * 4;  // 4 KiB per wave for the rescale of O
 constexpr int kFwLdsBytes = kFwLdsScr + kFwWaves * 4096;
-static_assert(kFwLdsBytes <= 160 * 1024, "gfx950 has 160 KiB of LDS per CU");
+constexpr int kFwLdsPos = kFwLdsBytes;           // windowed: the rows' positions
+constexpr int kFwWindowLdsBytes = kFwLdsPos + kFwRows * 4;
+static_assert(kFwWindowLdsBytes <= 160 * 1024, "gfx950 has 160 KiB of LDS per CU");
 
 // The keys that the rows [tok0, tok_last] of a sequence see with a sliding window and sinks: [lo, hi) and the first `sinks`.
 // Tiles are numbered over what is seen: [0, head) hold the sinks, from `head` on a tile lies `gap` tiles further than its number. They are
@@ -264,31 +266,41 @@ __device__ __forceinline__ void wide_workgroup(const FaParams& a, const FaWindow
         bool valid;
         int tok, head;
     };
-    auto row_of = [&](int rb) __attribute__((always_inline)) {
-        int r = 64 * w + 16 * rb + (lane_here() & 15);
+    const float per_token = 1.f / (float)G;
+    auto row_at = [&](int r) __attribute__((always_inline)) {
         Row x;
         x.valid = r < nrow;
         r = tok0_row + (x.valid ? r : 0);  // row of the workgroup's first token's rows
-        x.tok = r / G;
+        if constexpr (kWindow)
+            x.tok = (int)(((float)r + 0.5f) * per_token);  // r / G: at most 512, half a row from the next token
+        else
+            x.tok = r / G;
         x.head = r - x.tok * G;
         x.tok += tok0;
         return x;
     };
+    auto row_of = [&](int rb) __attribute__((always_inline)) { return row_at(64 * w + 16 * rb + (lane_here() & 15)); };
     half8_t qop[kFwRB][8];
+    auto load_q = [&]() __attribute__((always_inline)) {
 #pragma unroll
-    for (int rb = 0; rb < kFwRB; ++rb) {
-        const Row r = row_of(rb);
-        const T* qrow = static_cast<const T*>(a.q) + (kWindow ? (int64_t)first * a.q_st : (int64_t)b * a.q_sb) +
-                        (int64_t)(g * G + r.head) * a.q_sh + (int64_t)r.tok * a.q_st;
+        for (int rb = 0; rb < kFwRB; ++rb) {
+            const Row r = row_of(rb);
+            const T* qrow = static_cast<const T*>(a.q) + (kWindow ? (int64_t)first * a.q_st : (int64_t)b * a.q_sb) +
+                            (int64_t)(g * G + r.head) * a.q_sh + (int64_t)r.tok * a.q_st;
 #pragma unroll
-        for (int st = 0; st < 8; ++st) {
-            const half8_t v = load_q8<T>(qrow + 64 * (st >> 1) + 16 * (l >> 4) + 8 * (st & 1));
-            qop[rb][st] = r.valid ? v : (half8_t)(_Float16)0.0f;
+            for (int st = 0; st < 8; ++st) {
+                const half8_t v = load_q8<T>(qrow + 64 * (st >> 1) + 16 * (l >> 4) + 8 * (st & 1));
+                // (windowed: a row that is not there holds the first one's values, which go nowhere)
+                qop[rb][st] = kWindow || r.valid ? v : (half8_t)(_Float16)0.0f;
+            }
+            // one row block's loads at a time: four do not fit the registers in fp32
+            if constexpr (!kWindow)
+                asm volatile("" : "+v"(qop[rb][0]), "+v"(qop[rb][1]), "+v"(qop[rb][2]), "+v"(qop[rb][3]), "+v"(qop[rb][4]),
+                             "+v"(qop[rb][5]), "+v"(qop[rb][6]), "+v"(qop[rb][7]));
         }
-        // one row block's loads at a time: four do not fit the registers in fp32
-        asm volatile("" : "+v"(qop[rb][0]), "+v"(qop[rb][1]), "+v"(qop[rb][2]), "+v"(qop[rb][3]), "+v"(qop[rb][4]),
-                     "+v"(qop[rb][5]), "+v"(qop[rb][6]), "+v"(qop[rb][7]));
-    }
+    };
+    // Windowed launches have few tiles each: their first copies are under way before Q is loaded, all of it in one trip.
+    if constexpr (!kWindow) load_q();
     asm volatile("" ::: "memory");  // every Q load is issued before the block table is read
 
     lds_u8* L = (lds_u8*)lds;
@@ -323,6 +335,10 @@ __device__ __forceinline__ void wide_workgroup(const FaParams& a, const FaWindow
             if (pt.in_lds)
                 for (int i = tid; i < npages; i += kFwWaves * 64) dst[i] = bt_glob[i];
         }
+    }
+    if constexpr (kWindow) {
+        const Row row = row_at(tid);
+        ((lds_int*)(L + kFwLdsPos))[tid] = row.valid ? qabs + row.tok : -1;
     }
     __syncthreads();  // the LDS block table is complete
 
@@ -427,17 +443,20 @@ __device__ __forceinline__ void wide_workgroup(const FaParams& a, const FaWindow
             const int kb = seen.base(n);
             if (kb + kTile - 1 > pmin || (kb + kTile > seen.sinks && qabs + tok_last - kb >= win.window)) {
                 // some row does not see all of the tile; keys that none sees may hold garbage scales: v_scale 0
-                const int key = kb + 4 * (lane_here() >> 4);
+                const int lane = lane_here(), key = kb + 4 * (lane >> 4);
+                const lds_int* pos = (const lds_int*)(L + kFwLdsPos) + 64 * w + (lane & 15);
+                const bool sinks = kb < seen.sinks;  // uniform
 #pragma unroll
                 for (int e = 0; e < 8; ++e) vs[e] = seen.has(key + 16 * (e >> 2) + (e & 3)) ? vs[e] : 0.f;
 #pragma unroll
                 for (int rb = 0; rb < kFwRB; ++rb) {
-                    const Row row = row_of(rb);
-                    const int pos = qabs + row.tok, last = row.valid ? min(hi - 1, pos) : -1, from = pos - win.window;
+                    const int ahead = pos[16 * rb] - key;  // of the tile's first key of this lane; a row that is not there is at -1
 #pragma unroll
                     for (int e = 0; e < 8; ++e) {
-                        const int k = key + 16 * (e >> 2) + (e & 3);
-                        sv[rb][e] = (k <= last) & ((k > from) | (k < seen.sinks)) ? sv[rb][e] : kNegInf;
+                        const int d = ahead - 16 * (e >> 2) - (e & 3);
+                        bool sees = (unsigned)d < (unsigned)win.window;  // 0 <= d < window
+                        if (sinks) sees = sees | ((d >= 0) & (key + 16 * (e >> 2) + (e & 3) < seen.sinks));
+                        sv[rb][e] = sees ? sv[rb][e] : kNegInf;
                     }
                 }
             }
@@ -614,6 +633,7 @@ __device__ __forceinline__ void wide_workgroup(const FaParams& a, const FaWindow
             slot_in = slot_in + kStepBytes == kRingBytes ? 0 : slot_in + kStepBytes;
         };
         for (int s = 0; s < min(nsteps, kFwAhead); ++s) issue_next(s);
+        if constexpr (kWindow) load_q();
         const int ntl = t1 - t0;
 #pragma unroll 1
         for (int i = 0; i < ntl; ++i) {
@@ -646,6 +666,44 @@ __device__ __forceinline__ void wide_workgroup(const FaParams& a, const FaWindow
 
     // ---- normalise and store: out[b, tok, g G + hh, :]; with the keys split, the unnormalised
     //      partial O, the running max m and the sum l of the row instead ----
+    if constexpr (kWindow && !kSplit) {
+        // Through LDS (the ring is free once every wave is done): a lane has 4 dims of 16 rows' worth in each accumulator, and its stores
+        // of 8 bytes take 7.4 us of a workgroup, whole rows side by side 4.0. Each thread works out one row's place.
+        constexpr int kRow = 2 * kDim + 16;  // bytes of a row in LDS, its neighbours on other banks
+        constexpr int kPart = kFwRing * kFwSlot / kFwWaves / 16 * 16;
+        static_assert(16 * kRow <= kPart && kFwRows * 8 <= kFwWaves * 4096, "a row block's rows fit a wave's part of the ring, places the scratch");
+        typedef _Float16 half4_t __attribute__((ext_vector_type(4)));
+        typedef __attribute__((address_space(3))) half4_t lds_half4;
+        lds_u64* place = (lds_u64*)(L + kLdsScr);
+        __syncthreads();
+        {
+            const Row row = row_at(tid);
+            place[tid] = (uint64_t)(((int64_t)first + row.tok) * a.o_st + (int64_t)(g * G + row.head) * a.o_sh);
+        }
+        __syncthreads();
+        if (!busy) return;
+        lds_u8* mine = L + w * kPart;
+#pragma unroll
+        for (int rb = 0; rb < kFwRB; ++rb) {
+            const int lane = lane_here(), lg = lane >> 4, li = lane & 15;
+            settle_values(oacc[rb]);
+            const float l_row = xor_sum(xor_sum(l_run[rb], 16), 32);
+            const float inv = l_row > 0.f ? 1.f / l_row : 0.f;
+#pragma unroll
+            for (int m = 0; m < 16; ++m) {
+                const float4_t v = oacc[rb][m] * inv;
+                *(lds_half4*)(mine + li * kRow + 32 * m + 8 * lg) = half4_t{(_Float16)v.x, (_Float16)v.y, (_Float16)v.z, (_Float16)v.w};
+            }
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {  // two rows at a time
+                const int at = 2 * j + (lane >> 5), r = 64 * w + 16 * rb + at;
+                const uint4_t v = *(const lds_uint4*)(mine + at * kRow + 16 * (lane & 31));
+                T* to = static_cast<T*>(a.out) + (int64_t)place[r] + 8 * (lane & 31);
+                if (r < nrow) __builtin_memcpy(__builtin_assume_aligned(to, 8), &v, 16);
+            }
+        }
+        return;
+    }
 #pragma unroll
     for (int rb = 0; rb < kFwRB; ++rb) {
         const int lg = l >> 4;
@@ -665,8 +723,7 @@ __device__ __forceinline__ void wide_workgroup(const FaParams& a, const FaWindow
             }
         } else {
             const float inv = l_row > 0.f ? 1.f / l_row : 0.f;
-            T* orow = static_cast<T*>(a.out) + (kWindow ? (int64_t)first * a.o_st : (int64_t)b * a.o_sb) + (int64_t)tok * a.o_st +
-                      (int64_t)head * a.o_sh + 4 * lg;
+            T* orow = static_cast<T*>(a.out) + (int64_t)b * a.o_sb + (int64_t)tok * a.o_st + (int64_t)head * a.o_sh + 4 * lg;
 #pragma unroll
             for (int m = 0; m < 16; ++m) store_out4<T>(orow + 16 * m, oacc[rb][m] * inv);
         }
@@ -687,7 +744,7 @@ __global__ void __launch_bounds__(kFwWaves * 64, 1) pd_prefill_wide_kernel(const
 // launch takes any batch of as many rows and sequences.
 template <bool kFast, bool kExact, bool kSplit>
 __global__ void __launch_bounds__(kFwWaves * 64, 1) pd_window_kernel(const FaParams a, const FaWindow win) {
-    __shared__ __attribute__((aligned(16))) unsigned char lds[kFwLdsBytes];
+    __shared__ __attribute__((aligned(16))) unsigned char lds[kFwWindowLdsBytes];
     wide_workgroup<kFast, kExact, kSplit, _Float16, true>(a, win, lds);
 }
 
