@@ -11,6 +11,9 @@ few fields the routing reads.
   size 256, no sinks / alibi / softcap / chunked lookback / TD, on gfx950. Prefill also needs no
   sliding window. Decode accepts a left sliding window (the operator implements the window
   rule) and any GQA group with qmax * G <= 48, where the reference required GQA 6 and no window.
+  Layers with a left window whose fp16 rows the operator takes have their prefill in forward_window (not in the reference, which
+  leaves it to Triton); sink_tokens first keys then stay visible to all rows, in decode as well. (`sinks` are vLLM's learned
+  per-head logits, another thing, which no operator here takes.)
 - forward_pth_dec (triton_attn.patch:116-174): the cache layout is checked once; the call falls
   back (returns False) without the softmax segment buffers, with more query tokens than segment
   rows, or with query / output strides the operator does not take. nsplit = min(splits,
@@ -52,6 +55,7 @@ PTH_DEC_SPLITS = int(os.environ.get("VLLM_GFX950_PTH_DEC_SPLITS", "64"))
 PTH_DEC_CUS = int(os.environ.get("VLLM_GFX950_PTH_DEC_CUS", "0"))  # 0: the device's CU count
 PTH_FA_EXACT = os.environ.get("VLLM_GFX950_PTH_FA_EXACT", "0") == "1"  # prefill through pth_fa_forward_exact
 MAX_ROWS_PER_KV_HEAD = 48  # qmax * G the decode operator takes
+MAX_GROUP_WINDOW = 256     # G that forward_window takes
 # decode_shared against decode over 461 batches (24 / 4, 12 / 2 and 32 / 8 heads, 1, 2 and 4 query tokens, 2 to 512 sequences, 64 to
 # 32,768 shared and 50 to 4,000 own keys, 40 to 1,200 MB of spared reads): it is taken where both hold, the bytes and the estimated gain (shared_gain_us).
 # It is then at most 8 % slower (256 sequences of 32 / 8 heads over 256 keys 155 us, decode 144) and by more than 2 % in 5 batches; by the
@@ -217,6 +221,7 @@ class _Operators:
         self.decode_shared = _pd.decode_shared
         self.forward_pth = _pd.forward_pth
         self.forward_rows = _pd.forward_rows
+        self.forward_window = _pd.forward_window
 
 
 def _load(env_switch: str, env_lib: str, what: str):
@@ -281,15 +286,18 @@ class Gfx950Int8Attention:
                  kv_quant_int8_per_token_head: bool, is_rocm: bool, is_decoder: bool,
                  sliding_window=(-1, -1), sinks=None, alibi_slopes=None, logits_soft_cap=0.0,
                  chunk_lookback: int = -1, use_td: bool = False, on_gfx950: bool = True,
-                 max_q: int = PTH_DEC_MAX_Q):
+                 max_q: int = PTH_DEC_MAX_Q, sink_tokens: int = 0):
         self.scale = float(scale)
         self.num_heads, self.num_kv_heads = num_heads, num_kv_heads
         self.pth_fa = None
+        self.pth_fa_window = None  # prefill of a windowed layer
         self.pth_dec = None
         self.layout_ok: Optional[bool] = None  # cache layout, checked on first use
         self.max_q = max_q
         # left window W: vLLM's sliding_window (W - 1, 0); -1 = none
         self.window = sliding_window[0] + 1 if sliding_window[0] >= 0 else -1
+        # first keys that stay visible beside the window
+        self.sink_tokens = max(0, int(sink_tokens)) if self.window > 0 else 0
         common = (kv_quant_int8_per_token_head and is_rocm and is_decoder and head_size == 256 and sinks is None
                   and alibi_slopes is None and not logits_soft_cap and chunk_lookback == -1 and not use_td
                   and on_gfx950)
@@ -298,6 +306,9 @@ class Gfx950Int8Attention:
         if self.window < 0 and sliding_window[1] < 0:
             self.pth_fa = load_pth_fa()
         G = num_heads // num_kv_heads if num_kv_heads > 0 else 0
+        if self.window > 0 and sliding_window[1] <= 0 and num_heads % max(num_kv_heads, 1) == 0 and 1 <= G <= MAX_GROUP_WINDOW:
+            fa = load_pth_fa()
+            self.pth_fa_window = fa if hasattr(fa, "forward_window") else None
         if num_heads % max(num_kv_heads, 1) == 0 and 1 <= max_q * G <= MAX_ROWS_PER_KV_HEAD and sliding_window[1] < 0:
             self.pth_dec = load_pth_dec()
 
@@ -321,7 +332,7 @@ class Gfx950Int8Attention:
         # for windowed rows).
         if seq_lens_host is not None and _capturing(query.device):
             seq_lens_host = None
-        batch = (segm_o.shape[2], self.window, self.num_kv_heads, seq_lens.shape[0], query.device, seq_lens_host,
+        batch = (segm_o.shape[2], self.window + self.sink_tokens, self.num_kv_heads, seq_lens.shape[0], query.device, seq_lens_host,
                  max(1, max_q), query.shape[1])
         prefix = shared_prefix(meta, self.window, self.num_kv_heads, seq_lens.shape[0], key_cache.shape[1],
                                block_table.shape[1], segm_o.shape[2], query.shape[0], query.shape[1])
@@ -333,7 +344,8 @@ class Gfx950Int8Attention:
         self.pth_dec.decode(query, key_cache, value_cache, k_scale_cache, v_scale_cache, block_table, seq_lens,
                             query_start_loc, output, self.scale, segm_o, meta.softmax_segm_max,
                             meta.softmax_segm_expsum, seq_lens.shape[0], max(1, max_q),
-                            launched_splits(decode_splits(*batch), *batch), window=self.window, causal=True)
+                            launched_splits(decode_splits(*batch), *batch), window=self.window, causal=True,
+                            **({"sinks": self.sink_tokens} if self.sink_tokens else {}))
         return True
 
     # -------------------------------------------------------------------------------------
@@ -348,7 +360,8 @@ class Gfx950Int8Attention:
         p = n
         while p > 0 and qsl[p] - qsl[p - 1] >= PTH_FA_MIN_Q:
             p -= 1
-        if p == n:
+        if p == n or (self.pth_fa is None and not self._window_takes(query, key_cache, value_cache, k_scale_cache, v_scale_cache,
+                                                                     output, qsl[n])):
             return False
         max_q_prefix = max((qsl[i + 1] - qsl[i] for i in range(p)), default=0)
         if p > 0 and not (
@@ -358,6 +371,12 @@ class Gfx950Int8Attention:
                                      output[:qsl[p]], max_q_prefix, meta,
                                      None if meta.seq_lens_cpu is None else meta.seq_lens_cpu[:p])):
             triton_fallback(0, qsl[p], 0, p, max_q_prefix)
+        if self.pth_fa is None:
+            # (sized by the window, and the rows are found on the device: nothing here depends on the lengths)
+            self.pth_fa_window.forward_window(query[:qsl[n]], key_cache, value_cache, meta.block_table[p:n], meta.seq_lens[p:n],
+                                              self.scale, meta.query_start_loc[p:n + 1], output[:qsl[n]], self.window,
+                                              sinks=self.sink_tokens, exact=PTH_FA_EXACT)
+            return True
         # A launch is planned for the keys that its sequences see: the host lengths when they are known and
         # no graph is being captured (vLLM's block table is as wide as the model's maximum length, so the table
         # alone would plan every chunk for the longest context), else the batch's max_seq_len, else the
@@ -384,6 +403,18 @@ class Gfx950Int8Attention:
             output[start:start + nq] = out[0].to(output.dtype)
         return True
 
+    def _window_takes(self, query, key_cache, value_cache, k_scale_cache, v_scale_cache, output, rows: int) -> bool:
+        """Whether forward_window takes the batch's rows: fp16 heads of 256, aligned as its vectors need, over the int8 row layout."""
+        if self.layout_ok is None:
+            self.layout_ok = bool(self.pth_fa_window.supported_layout(key_cache, value_cache, k_scale_cache, v_scale_cache))
+            if not self.layout_ok:
+                logger.warning("gfx950: unexpected int8 KV cache layout; windowed prefill stays on Triton")
+        return bool(self.layout_ok and query.dim() == 3 and output.dim() == 3 and query.dtype == torch.float16
+                    and output.dtype == torch.float16 and query.shape[0] >= rows and output.shape[0] >= rows
+                    and query.shape[2] == 256 and output.shape[1:] == query.shape[1:] and query.stride(2) == 1
+                    and output.stride(2) == 1 and query.stride(0) % 8 == 0 and query.stride(1) % 8 == 0 and query.data_ptr() % 16 == 0
+                    and output.stride(0) % 4 == 0 and output.stride(1) % 4 == 0 and output.data_ptr() % 8 == 0)
+
     # -------------------------------------------------------------------------------------
     def route(self, query, key_cache, value_cache, k_scale_cache, v_scale_cache, meta: AttnMeta, output,
               max_seqlen_q: int, num_actual_tokens: int, triton_fallback: Callable[..., None],
@@ -391,7 +422,7 @@ class Gfx950Int8Attention:
         """The forward() glue: True when one of the operators handled the batch."""
         plain = (meta.causal is True and meta.mm_prefix_range_tensor is None and meta.rswa_prefix_lens is None
                  and output_scale is None)
-        if (self.pth_fa is not None and max_seqlen_q >= PTH_FA_MIN_Q and plain
+        if ((self.pth_fa is not None or self.pth_fa_window is not None) and max_seqlen_q >= PTH_FA_MIN_Q and plain
                 and self.forward_pth_fa(query, key_cache, value_cache, k_scale_cache, v_scale_cache, meta, output,
                                         triton_fallback)):
             return True
