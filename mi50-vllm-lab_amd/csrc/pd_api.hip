@@ -1122,7 +1122,7 @@ static bool table_rows_apart(const pd_tensor* t) { return t->sizes[0] <= 1 || t-
 // Workspace ints: both masks, the counts, and for a fork the rows' plans.
 static int64_t page_work_ints(int64_t pages, int64_t rows, int64_t new_rows) {
     const int64_t chunks = (pages + 1023) / 1024;
-    return chunks * (2 * 32 + 1) + rows + 3 * new_rows + 1;
+    return chunks * (2 * 32 + 1) + rows + 4 * new_rows + 1;
 }
 static const char* page_work(const pd_tensor* ws, int64_t pages, int64_t ints, PageWork& w) {
     if (!(ws->dtype == PD_DTYPE_INT32 && ws->ndim == 1 && is_contig(ws) && ws->sizes[0] >= ints &&
@@ -1210,9 +1210,8 @@ int pth_cache_fork_pages(const pd_tensor* caches, int64_t layers, const pd_tenso
     p.sinks = sinks;
     p.eldest = p.w.counts + p.w.chunks;
     p.first_taken = p.eldest + B;
-    p.copy_row = p.first_taken + N;
-    p.copy_from = p.copy_row + N;
-    p.copies = p.copy_from + N;
+    p.copies = p.first_taken + N;
+    p.copy_list = reinterpret_cast<PageCopy*>(p.copies + 1);
     return op_result(launch_fork(p, k, stream), "fork pages", err, errlen);
 }
 

@@ -218,6 +218,10 @@ struct PageCaches {
     int layers, Hkv, block_size;
     int form, runs, cuts;            // runs of adjacent bytes in a page, pieces of a run (set by the launch)
 };
+// The first `keys` keys of page `from` into the rank-th lowest free page.
+struct PageCopy {
+    int from, rank, keys;
+};
 struct ForkParams {
     PageWork w;
     const int* refs;
@@ -232,7 +236,8 @@ struct ForkParams {
     int* needed;
     int rows, new_rows, cols, block_size;
     int64_t grow, window, sinks;     // window <= 0: none
-    int *eldest, *first_taken, *copy_row, *copy_from, *copies;  // workspace: first child of each old row; per new row; the copies
+    int *eldest, *first_taken, *copies;  // workspace: first child of each old row, rank of each new row's first page, copies
+    PageCopy* copy_list;
 };
 struct CompactParams {
     PageWork w;

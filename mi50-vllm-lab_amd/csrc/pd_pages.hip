@@ -177,7 +177,7 @@ __device__ __forceinline__ RowPlan row_plan(const ForkParams& a, int i) {
 __device__ __forceinline__ bool names_page(const ForkParams& a, int e) { return e >= 0 && e < a.w.pages; }
 
 // First launch of a fork: workgroup 0 plans the new rows (the first child of each old row, how many pages the rows before
-// each new row take, and the list of rows and pages whose keys are copied), the others take one chunk of the counts each.
+// each new row take, and the list of the pages whose keys are copied), the others take one chunk of the counts each.
 __global__ void __launch_bounds__(kPgThreads) pd_fork_plan_kernel(const ForkParams a) {
     __shared__ int eldest[kMaxForkRows];
     __shared__ unsigned part[kPgThreads / 64];
@@ -200,7 +200,7 @@ __global__ void __launch_bounds__(kPgThreads) pd_fork_plan_kernel(const ForkPara
     for (int i0 = 0; i0 < a.new_rows; i0 += kPgThreads) {
         const int i = i0 + tid;
         unsigned takes = 0;
-        int src = -1;
+        int src = -1, keys = 0;
         if (i < a.new_rows) {
             const RowPlan r = row_plan(a, i);
             if (r.parent >= 0) {
@@ -219,18 +219,16 @@ __global__ void __launch_bounds__(kPgThreads) pd_fork_plan_kernel(const ForkPara
                 if (r.full < r.end && (int64_t)r.full * a.block_size < r.n && !first_kept) {
                     const int e = row[r.full];
                     src = names_page(a, e) ? e : -1;
+                    keys = (int)(r.n - (int64_t)r.full * a.block_size);
                 }
             }
         }
         unsigned total;
-        const unsigned ex = block_scan(takes, part, total);
+        const unsigned ex = block_scan(takes, part, total), run_before = run;
         if (i < a.new_rows) a.first_taken[i] = (int)(run + ex);
         run += total;
         const unsigned at = ncopies + block_scan(src >= 0 ? 1u : 0u, part, total);
-        if (src >= 0) {
-            a.copy_row[at] = i;
-            a.copy_from[at] = src;
-        }
+        if (src >= 0) a.copy_list[at] = PageCopy{src, (int)(run_before + ex), keys};
         ncopies += total;
     }
     if (tid == 0) {
@@ -298,36 +296,53 @@ __global__ void __launch_bounds__(kPgThreads) pd_fork_kernel(const ForkParams a,
         const bool heir = r.parent >= 0 && (!a.parents || a.eldest[r.parent] == i);
         const int* row = a.table + (int64_t)max(0, r.parent) * a.t_st;
         int* out = a.new_table + (int64_t)i * a.n_st;
+        // Full pages, and the columns behind the row's: each entry stands for itself, so four of a thread's are in flight.
+        auto plain = [&](int c0, int c1, bool full) __attribute__((always_inline)) {
+            constexpr int kAhead = 4;
+            for (int b = c0 + tid; b < c1; b += kAhead * kPgThreads) {
+                int e[kAhead];
+#pragma unroll
+                for (int k = 0; k < kAhead; ++k) e[k] = b + k * kPgThreads < c1 && r.parent >= 0 ? row[b + k * kPgThreads] : -1;
+#pragma unroll
+                for (int k = 0; k < kAhead; ++k) {
+                    const int c = b + k * kPgThreads;
+                    if (c >= c1) break;
+                    const int64_t k0 = (int64_t)c * a.block_size;
+                    const bool named = names_page(a, e[k]);
+                    const bool stays = full && named && !(a.window > 0 && k0 >= a.sinks && k0 + a.block_size <= r.n + 1 - a.window);
+                    if (heir && named && !stays) atomicAdd(a.new_refs + e[k], -1);
+                    if (!heir && stays) atomicAdd(a.new_refs + e[k], 1);
+                    out[c] = stays ? e[k] : -1;
+                }
+            }
+        };
+        const int full = min(r.full, r.end);
+        plain(0, full, true);
+        plain(r.end, a.cols, false);
+        // the row's own columns
         unsigned run = (unsigned)a.first_taken[i], nfree = 0;
         bool have_prefix = false;
-        for (int c0 = 0; c0 < a.cols; c0 += kPgThreads) {
+        for (int c0 = full; c0 < r.end; c0 += kPgThreads) {
             const int c = c0 + tid;
             int e = -1, v = -1;
             bool takes = false;
-            if (c < a.cols && r.parent >= 0) {
+            if (c < r.end) {
                 e = row[c];
                 if (!names_page(a, e)) e = -1;
-                const int64_t k0 = (int64_t)c * a.block_size;
-                if (c < r.full)
-                    v = c < r.end && !(a.window > 0 && k0 >= a.sinks && k0 + a.block_size <= r.n + 1 - a.window) ? e : -1;
-                else if (c < r.end && heir && e >= 0 && mask_bit(a.w.alone_mask, e))
-                    v = e;
-                else
-                    takes = c < r.end;
+                takes = !(heir && e >= 0 && mask_bit(a.w.alone_mask, e));
+                v = takes ? -1 : e;
             }
-            if (c0 + kPgThreads > r.full && c0 < r.end) {  // (uniform) some column of these may take a page
-                unsigned total;
-                const unsigned rank = run + block_scan(takes ? 1u : 0u, part, total);
-                if (total > 0 && !have_prefix) {
-                    nfree = load_prefix(a.w, before, part);
-                    have_prefix = true;
-                }
-                if (takes && rank < nfree) v = select_page<true>(a.w, before, rank);
-                run += total;
+            unsigned total;
+            const unsigned rank = run + block_scan(takes ? 1u : 0u, part, total);
+            if (total > 0 && !have_prefix) {
+                nfree = load_prefix(a.w, before, part);
+                have_prefix = true;
             }
-            if (c < a.cols) {
-                if (heir && e >= 0 && v != e) atomicAdd(a.new_refs + e, -1);
-                if (v >= 0 && (takes || !heir)) atomicAdd(a.new_refs + v, 1);
+            if (takes && rank < nfree) v = select_page<true>(a.w, before, rank);
+            run += total;
+            if (c < r.end) {
+                if (heir && e >= 0 && takes) atomicAdd(a.new_refs + e, -1);
+                if (v >= 0 && takes) atomicAdd(a.new_refs + v, 1);
                 out[c] = v;
             }
         }
@@ -351,21 +366,18 @@ __global__ void __launch_bounds__(kPgThreads) pd_fork_kernel(const ForkParams a,
     const int nwg = (int)gridDim.x - a.new_rows - (a.parents ? a.rows : 0);
     const int pieces = k.runs * k.cuts, each = k.layers * pieces;
     const int64_t tasks = (int64_t)a.copies[0] * each, per = (tasks + nwg - 1) / nwg;
-    int known = -1, to = -1, from = -1;
-    int64_t keys = 0;
-    unsigned nfree = 0;
+    if (wg * per >= tasks) return;
+    const unsigned nfree = load_prefix(a.w, before, part);
+    int known = -1, to = -1;
+    PageCopy copy = {};
     for (int64_t t = wg * per; t < min(tasks, wg * per + per); ++t) {
         const int j = (int)(t / each), x = (int)(t - (int64_t)j * each), layer = x / pieces;
         if (j != known) {
-            if (known < 0) nfree = load_prefix(a.w, before, part);
             known = j;
-            const int i = a.copy_row[j];
-            const unsigned rank = (unsigned)a.first_taken[i];
-            from = a.copy_from[j];
-            to = rank < nfree ? select_page<true>(a.w, before, rank) : -1;
-            keys = a.seq_lens[a.parents ? a.parents[i] : i] % a.block_size;
+            copy = a.copy_list[j];
+            to = (unsigned)copy.rank < nfree ? select_page<true>(a.w, before, (unsigned)copy.rank) : -1;
         }
-        if (to >= 0) copy_piece(k, layer, from, to, x - layer * pieces, keys);
+        if (to >= 0) copy_piece(k, layer, copy.from, to, x - layer * pieces, copy.keys);
     }
 }
 

@@ -157,7 +157,7 @@ def test_pools_and_rows_beyond_the_limits(lib):
         assert rc == 1 and b"2^22 pages" in err.value
     w = lib.pth_cache_pages_workspace
     assert w(0, 1, 1) == 0 and w((1 << 22) + 1, 1, 1) == 0 and w(1, -1, 1) == 0
-    assert w(1, 0, 0) == 66 and w(1025, 3, 5) == 2 * 65 + 3 + 15 + 1
+    assert w(1, 0, 0) == 66 and w(1025, 3, 5) == 2 * 65 + 3 + 20 + 1
 
 
 def test_norm_rotary_refusals(lib):
