@@ -237,28 +237,28 @@ __global__ void __launch_bounds__(kPgThreads) pd_fork_plan_kernel(const ForkPara
     }
 }
 
-// `len` bytes, 8-byte aligned, by the threads of a workgroup.
+// `len` bytes, 8-byte aligned, by a wave, 8 KiB of them in flight.
 __device__ __forceinline__ void copy_bytes(int8_t* dst, const int8_t* src, int64_t len) {
-    const int tid = threadIdx.x;
+    const int lane = threadIdx.x & 63;
     const uintptr_t d = reinterpret_cast<uintptr_t>(dst);
     if (((d ^ reinterpret_cast<uintptr_t>(src)) & 15) == 0) {
         const int64_t head = (d & 15) && len ? 8 : 0, body = (len - head) / 16, tail = len - head - 16 * body;
         const uint4_t* s = reinterpret_cast<const uint4_t*>(src + head);
         uint4_t* o = reinterpret_cast<uint4_t*>(dst + head);
-        constexpr int kAhead = 4;
-        for (int64_t i0 = tid; i0 < body; i0 += kAhead * kPgThreads) {
+        if (lane == 0 && head) *reinterpret_cast<uint64_t*>(dst) = *reinterpret_cast<const uint64_t*>(src);
+        if (lane == 1 && tail) *reinterpret_cast<uint64_t*>(dst + len - 8) = *reinterpret_cast<const uint64_t*>(src + len - 8);
+        constexpr int kAhead = 8;
+        for (int64_t i0 = lane; i0 < body; i0 += kAhead * 64) {
             uint4_t x[kAhead];
 #pragma unroll
             for (int k = 0; k < kAhead; ++k)
-                if (i0 + k * kPgThreads < body) x[k] = s[i0 + k * kPgThreads];
+                if (i0 + k * 64 < body) x[k] = s[i0 + k * 64];
 #pragma unroll
             for (int k = 0; k < kAhead; ++k)
-                if (i0 + k * kPgThreads < body) o[i0 + k * kPgThreads] = x[k];
+                if (i0 + k * 64 < body) o[i0 + k * 64] = x[k];
         }
-        if (tid == 0 && head) *reinterpret_cast<uint64_t*>(dst) = *reinterpret_cast<const uint64_t*>(src);
-        if (tid == 64 && tail) *reinterpret_cast<uint64_t*>(dst + len - 8) = *reinterpret_cast<const uint64_t*>(src + len - 8);
     } else {
-        for (int64_t i = tid; i < len / 8; i += kPgThreads)
+        for (int64_t i = lane; i < len / 8; i += 64)
             reinterpret_cast<uint64_t*>(dst)[i] = reinterpret_cast<const uint64_t*>(src)[i];
     }
 }
@@ -362,15 +362,16 @@ __global__ void __launch_bounds__(kPgThreads) pd_fork_kernel(const ForkParams a,
         }
         wg -= a.rows;
     }
-    // (a run of pieces per workgroup: they are mostly of one page, which is then looked up once)
-    const int nwg = (int)gridDim.x - a.new_rows - (a.parents ? a.rows : 0);
+    // (a run of pieces per wave: they are mostly of one page, which is then looked up once)
+    const int64_t nwave = (int64_t)((int)gridDim.x - a.new_rows - (a.parents ? a.rows : 0)) * (kPgThreads / 64);
     const int pieces = k.runs * k.cuts, each = k.layers * pieces;
-    const int64_t tasks = (int64_t)a.copies[0] * each, per = (tasks + nwg - 1) / nwg;
-    if (wg * per >= tasks) return;
+    const int64_t tasks = (int64_t)a.copies[0] * each, per = (tasks + nwave - 1) / nwave;
+    if ((int64_t)wg * (kPgThreads / 64) * per >= tasks) return;
     const unsigned nfree = load_prefix(a.w, before, part);
+    const int64_t t0 = ((int64_t)wg * (kPgThreads / 64) + __builtin_amdgcn_readfirstlane(tid >> 6)) * per;
     int known = -1, to = -1;
     PageCopy copy = {};
-    for (int64_t t = wg * per; t < min(tasks, wg * per + per); ++t) {
+    for (int64_t t = t0; t < min(tasks, t0 + per); ++t) {
         const int j = (int)(t / each), x = (int)(t - (int64_t)j * each), layer = x / pieces;
         if (j != known) {
             known = j;
@@ -424,12 +425,13 @@ __global__ void __launch_bounds__(kPgThreads) pd_compact_kernel(const CompactPar
         return;
     }
     wg -= a.rows;
-    const int nwg = (int)gridDim.x - a.w.chunks - a.rows;
+    const int64_t nwave = (int64_t)((int)gridDim.x - a.w.chunks - a.rows) * (kPgThreads / 64);
     const int pieces = k.runs * k.cuts, each = k.layers * pieces;
-    const int64_t tasks = (int64_t)moves * each, per = (tasks + nwg - 1) / nwg;
+    const int64_t tasks = (int64_t)moves * each, per = (tasks + nwave - 1) / nwave;
+    const int64_t t0 = ((int64_t)wg * (kPgThreads / 64) + __builtin_amdgcn_readfirstlane(tid >> 6)) * per;
     unsigned known = 0xffffffffu;
     int from = 0, to = 0;
-    for (int64_t t = wg * per; t < min(tasks, wg * per + per); ++t) {
+    for (int64_t t = t0; t < min(tasks, t0 + per); ++t) {
         const unsigned m = (unsigned)(t / each);
         const int x = (int)(t - (int64_t)m * each), layer = x / pieces;
         if (m != known) {
@@ -459,13 +461,18 @@ static void plan_copies(PageCaches& k, bool whole) {
     k.cuts = (int)((longest + kPagePiece - 1) / kPagePiece);
 }
 
+static int64_t copy_groups(int64_t tasks) {
+    const int64_t wanted = (tasks + kPgThreads / 64 - 1) / (kPgThreads / 64);
+    return wanted < kPageCopyGroups ? wanted : kPageCopyGroups;
+}
+
 hipError_t launch_fork(ForkParams p, PageCaches k, hipStream_t stream) {
     plan_copies(k, false);
     hipLaunchKernelGGL(pd_fork_plan_kernel, dim3(1 + p.w.chunks), dim3(kPgThreads), 0, stream, p);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
     const int64_t tasks = (int64_t)p.new_rows * k.layers * k.runs * k.cuts;
-    const int64_t wgs = p.new_rows + (p.parents ? p.rows : 0) + (tasks < kPageCopyGroups ? tasks : kPageCopyGroups);
+    const int64_t wgs = p.new_rows + (p.parents ? p.rows : 0) + copy_groups(tasks);
     if (wgs == 0) return hipSuccess;
     hipLaunchKernelGGL(pd_fork_kernel, dim3((unsigned)wgs), dim3(kPgThreads), 0, stream, p, k);
     return hipGetLastError();
@@ -477,7 +484,7 @@ hipError_t launch_compact(const CompactParams& p, PageCaches k, hipStream_t stre
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
     const int64_t tasks = (int64_t)(p.w.pages / 2) * k.layers * k.runs * k.cuts;  // at most half of the pages move
-    const int64_t wgs = p.w.chunks + p.rows + (tasks < kPageCopyGroups ? tasks : kPageCopyGroups);
+    const int64_t wgs = p.w.chunks + p.rows + copy_groups(tasks);
     hipLaunchKernelGGL(pd_compact_kernel, dim3((unsigned)wgs), dim3(kPgThreads), 0, stream, p, k);
     return hipGetLastError();
 }
