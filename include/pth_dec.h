@@ -288,7 +288,8 @@ int64_t pth_fa_balanced_workspace(int64_t num_seqs, const int* query_start, int6
  *                tokens of its seq_lens[i] keys (block_table and seq_lens have a row per sequence). Rows outside the sequences, and of
  *                sequences of no keys, are left alone
  *   window >= 1, sinks >= 0   the row at position p sees key k <= p if p - k < window or k < sinks
- *   nsplit       1..64: key splits per query tile (256 rows of one kv head); pth_fa_window_splits' count suits the sizes
+ *   nsplit       1..64: key splits per query tile (256 or 128 rows of one kv head, as the sizes suggest); pth_fa_window_splits' count
+ *                suits the sizes
  *   workspace    fp32, contiguous, 16-byte aligned, of T * Hq * nsplit * 258 floats (null or ignored when nsplit is 1)
  *   exact        0: each softmax weight enters P.V as one fp16; else as fp16 hi + lo. K and V are widened exactly in both
  * Pages in which no row of a query tile sees a key are not addressed for it: the table's entries for pages between the sinks and

@@ -571,15 +571,11 @@ int64_t pth_fa_window_splits(int64_t tokens, int64_t num_seqs, int64_t heads_q, 
     if (tokens < 1 || tokens > INT32_MAX || num_seqs < 1 || num_seqs > INT32_MAX || heads_kv < 1 || heads_q < heads_kv ||
         heads_q % heads_kv != 0 || heads_q > (1 << 20) || window < 1 || window > INT32_MAX || sinks < 0 || sinks > INT32_MAX)
         return 1;
-    const int64_t G = heads_q / heads_kv, span = window + (kFwRows + G - 1) / G + 31;  // keys that a query tile sees, aligned
-    const int64_t tiles = (std::min(span, std::max<int64_t>(1, table_keys)) + 31) / 32 + (std::min(sinks, std::max<int64_t>(0, table_keys - span)) + 31) / 32;
     int dev = 0, cus = 0;
     if (hipGetDevice(&dev) != hipSuccess ||
         hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess || cus < 1)
         cus = 256;
-    // (half of the sequences' last tiles are taken to be part-filled ones of their own)
-    const int64_t items = ((tokens * G + kFwRows - 1) / kFwRows + (num_seqs - 1) / 2) * heads_kv;
-    return window_splits(items, tiles, tokens * heads_q, cus, exact != 0);
+    return fw_splits({tokens, num_seqs, heads_q, heads_kv, window, sinks, std::max<int64_t>(0, table_keys), cus, exact != 0});
 }
 
 int pth_fa_forward_window(const pd_tensor* q, const pd_tensor* key_cache, const pd_tensor* value_cache,
@@ -616,7 +612,7 @@ int pth_fa_forward_window(const pd_tensor* q, const pd_tensor* key_cache, const 
         return fail(err, errlen, "window must be at least 1, sinks at least 0, and both fit in 32 bits");
     if (!(nsplit >= 1 && nsplit <= 64)) return fail(err, errlen, "nsplit must be in [1, 64]");
     // a launch's workgroups, and the 32 bits that number query tiles and rows
-    const int64_t G = Hq / Hkv, tiles = window_tiles(T, num_seqs, G);
+    const int64_t G = Hq / Hkv, tiles = window_tiles(T, num_seqs, G, kFwNarrowRows);
     if (!(T * Hq <= ((int64_t)1 << 30) && tiles * nsplit <= (1 << 24) / Hkv - 1))
         return fail(err, errlen, "at most 2^30 (token, head) rows and 2^24 workgroups per call");
     if (!rows_apart(out, T, kDim)) return fail(err, errlen, "out rows must not overlap");
@@ -653,7 +649,9 @@ int pth_fa_forward_window(const pd_tensor* q, const pd_tensor* key_cache, const 
         p.part_l = p.part_m + rows;
     }
     const FaWindow w = {static_cast<const int*>(query_start_loc->data), (int)num_seqs, (int)T, (int)window, (int)sinks};
-    return fa_result(launch_window(p, w, (int)Hkv, stream, exact != 0), err, errlen);
+    const int cus = compute_units(stream);
+    const FwCall call = {T, num_seqs, Hq, Hkv, window, sinks, block_table->sizes[1] * bs, cus > 0 ? cus : 256, exact != 0};
+    return fa_result(launch_window(p, w, fw_narrow(call, nsplit) ? kFwNarrowRows : kFwRows, (int)Hkv, stream, exact != 0), err, errlen);
 }
 
 int pth_fa_forward(const pd_tensor* q, const pd_tensor* key_cache, const pd_tensor* value_cache,

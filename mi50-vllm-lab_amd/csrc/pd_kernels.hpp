@@ -20,6 +20,7 @@ constexpr int64_t kSliceKeys = 16384; // decode: largest sequences x window whos
 constexpr int kFaWaves = 4;
 constexpr int kFaRB = 3;                        // row blocks per wave
 constexpr int kFaRows = kFaWaves * kFaRB * 16;  // 192
+constexpr int kFwNarrowRows = 128;              // rows of a narrow workgroup of pd_window_kernel
 constexpr int kFwRows = 256;                    // query rows (token, head) of a workgroup of pd_prefill_wide_kernel
 
 // Split-K decode, partial pass (pd_partial_kernel).
@@ -122,7 +123,7 @@ struct FaWindow {
     int window, sinks;
 };
 // query tiles of a kv head that such rows have at the most
-inline int64_t window_tiles(int64_t tokens, int64_t seqs, int64_t G) { return tokens * G / kFwRows + seqs; }
+inline int64_t window_tiles(int64_t tokens, int64_t seqs, int64_t G, int64_t rows) { return tokens * G / rows + seqs; }
 
 // KV-cache writer (pd_cache_write_kernel).
 struct CacheWriteParams {
@@ -308,8 +309,8 @@ hipError_t launch_prefill_balanced(const FaParams& p, const FaRowsParams& r, int
                                    bool exact);
 // workgroups of such a launch on `cus` CUs: as many as the work pays for, at least one per item while CUs last
 int64_t balanced_prefill_workgroups(int64_t items, int64_t max_keys, int cus);
-// the 256-row kernel for fp16 rows that see a window and sinks, p.nsplit splits and their merge (pd_prefill_wide.hip)
-hipError_t launch_window(const FaParams& p, const FaWindow& w, int heads_kv, hipStream_t stream, bool exact);
+// fp16 rows that see a window and sinks, kFwRows or kFwNarrowRows to a workgroup, p.nsplit splits and their merge (pd_prefill_wide.hip)
+hipError_t launch_window(const FaParams& p, const FaWindow& w, int rows, int heads_kv, hipStream_t stream, bool exact);
 constexpr int64_t kFaSlotFloats = (int64_t)kFaRows * (kDim + 2);
 // compute units of a stream's device (0 if unknown)
 int compute_units(hipStream_t stream);

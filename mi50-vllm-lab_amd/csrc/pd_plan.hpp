@@ -34,19 +34,43 @@ constexpr int64_t kFaDealSpareUnits = 20;
 constexpr double kFaDealFixedUs = 20.0;
 constexpr double kFaDealMargin = 0.95;
 
-// Key splits of a windowed launch (pd_window_kernel): `items` workgroups per split, each of `tiles` key tiles, one per CU at a time. A
-// workgroup's set-up and stores, the merge launch, and the partials' way to memory and back, us. Measured and rated (24 q / 4 kv heads): 64
-// tokens over 2,048 keys 137 unsplit, 40 at 10 splits, 39 at 16 (144, 39, 38); 600 over 4,096 261, 156 at 2, 100 at 4 (268, 157,
-// 103); 1,024 260 and 164 at 2 (268, 160), 2 rounds at 3 217; 4,096 521 and 489 at 2 (537, 487).
-constexpr double kFwSetupUs = 18.0, kFwMergeUs = 5.0, kFwPartialUsPerMb = 0.25;
-constexpr int64_t kFwMaxSplits = 16;
-inline int64_t window_splits(int64_t items, int64_t tiles, int64_t rows, int64_t cus, bool exact) {
+// Windowed launches (pd_window_kernel): workgroups of 256 rows, or of 128, which take 1.5 us a key tile instead of 1.85 but fewer to
+// set up and store, and are twice as many, for launches that do not fill the GPU. us, one workgroup per CU at a time: a
+// tile, exact numerics' tile, set-up and stores with the launch; the merge launch of splits and their partials' way to memory and back.
+// Measured and rated (24 q / 4 kv heads, over 30,000 keys), wide and narrow: 2,048 tokens over 512 keys 58 (56) and 79 (82), over 4,096
+// 265 (263) and 416 (417); 1,024 over 1,024 85 (85) and 65 (64); 64 over 2,048 in 10 splits 39 (42) and 31 (31); 600 over
+// 4,096 in 2 153 (155) and 124 (123); 4,096 in 2 482 (482).
+struct FwTimes {
+    double tile, tile_exact, setup;
+};
+constexpr FwTimes kFwWide = {1.85, 2.38, 20.0}, kFwNarrow = {1.5, 1.76, 12.0};
+constexpr double kFwMergeUs = 5.0, kFwPartialUsPerMb = 0.25;
+constexpr int64_t kFwMaxSplits = 16;  // of the plan, with 4 tiles each at the least
+struct FwCall {
+    int64_t tokens, seqs, heads_q, heads_kv, window, sinks, table_keys, cus;
+    bool exact;
+};
+// key tiles of a query tile of `rows` rows
+inline int64_t fw_key_tiles(const FwCall& c, int64_t rows) {
+    const int64_t G = c.heads_q / c.heads_kv, span = c.window + (rows + G - 1) / G + 31;
+    const int64_t keys = c.table_keys > 1 ? c.table_keys : 1, far = c.table_keys > span ? c.table_keys - span : 0;
+    return ((span < keys ? span : keys) + 31) / 32 + ((c.sinks < far ? c.sinks : far) + 31) / 32;
+}
+inline double fw_us(const FwCall& c, int64_t rows, int64_t splits, const FwTimes& t) {
+    const int64_t G = c.heads_q / c.heads_kv, tiles = (fw_key_tiles(c, rows) + splits - 1) / splits;
+    // (half of the sequences' last query tiles are taken to be part-filled ones of their own)
+    const int64_t items = ((c.tokens * G + rows - 1) / rows + (c.seqs - 1) / 2) * c.heads_kv * splits;
+    const double us = (double)((items + c.cus - 1) / c.cus) * ((double)tiles * (c.exact ? t.tile_exact : t.tile) + t.setup);
+    return splits == 1 ? us : us + kFwMergeUs + kFwPartialUsPerMb * (double)(c.tokens * c.heads_q) * (double)splits * 1032 / 1e6;
+}
+// Whether a call with this many splits runs on narrow workgroups.
+inline bool fw_narrow(const FwCall& c, int64_t splits) { return fw_us(c, 128, splits, kFwNarrow) < fw_us(c, 256, splits, kFwWide); }
+// The splits that are rated fastest on either.
+inline int64_t fw_splits(const FwCall& c) {
     int64_t best = 1;
     double best_us = 0;
-    for (int64_t s = 1; s <= kFwMaxSplits && (s == 1 || s * 4 <= tiles); ++s) {
-        const int64_t rounds = (items * s + cus - 1) / cus;
-        double us = (double)rounds * ((double)((tiles + s - 1) / s) * fa_times(exact).wide_tile + kFwSetupUs);
-        if (s > 1) us += kFwMergeUs + kFwPartialUsPerMb * (double)rows * (double)s * 1032 / 1e6;
+    for (int64_t s = 1; s <= kFwMaxSplits && (s == 1 || s * 4 <= fw_key_tiles(c, 128)); ++s) {
+        const double wide = fw_us(c, 256, s, kFwWide), narrow = fw_us(c, 128, s, kFwNarrow), us = narrow < wide ? narrow : wide;
         if (s == 1 || us < best_us) best = s, best_us = us;
     }
     return best;

@@ -87,8 +87,47 @@ __device__ __forceinline__ void value_products_only(float4_t& o0, float4_t& o1, 
                  : "+a"(o0), "+a"(o1), "+a"(o2), "+a"(o3)
                  : "v"(cur), "v"(p0), "v"(p1), "v"(p2), "v"(p3));
 }
+// The same for two row blocks (narrow workgroups): four conversions behind each product. A product reads an accumulator of the block
+// before 11 issue slots after it was written, or as the very register it accumulates into, which needs none.
+#define PD_PRODUCTS_AND_WIDEN_2(C0, C1)                                          \
+    "v_mfma_f32_16x16x32_f16 %0, %6, %7, " C0 "\n\t"                              \
+    PD_CVT("%2", "%9", "0", "0", "PAD") PD_CVT("%3", "%9", "0", "2", "PAD") PD_CVT("%4", "%10", "0", "0", "PAD") \
+    PD_CVT("%5", "%10", "0", "2", "PAD")                                         \
+    "v_mfma_f32_16x16x32_f16 %1, %6, %8, " C1 "\n\t"                              \
+    PD_CVT("%2", "%9", "1", "1", "PRESERVE") PD_CVT("%3", "%9", "1", "3", "PRESERVE") \
+    PD_CVT("%4", "%10", "1", "1", "PRESERVE") PD_CVT("%5", "%10", "1", "3", "PRESERVE") "s_nop 1"
+template <bool kFirst>
+__device__ __forceinline__ half8_t score_products(float4_t& s0, float4_t& s1, half8_t cur, half8_t q0, half8_t q1, unsigned w0,
+                                                  unsigned w1) {
+    uint4_t n;
+    if constexpr (kFirst)
+        asm volatile(PD_PRODUCTS_AND_WIDEN_2("0", "0")
+                     : "=&v"(s0), "=&v"(s1), "=&v"(n.x), "=&v"(n.y), "=&v"(n.z), "=&v"(n.w)
+                     : "v"(cur), "v"(q0), "v"(q1), "v"(w0), "v"(w1));
+    else
+        asm volatile(PD_PRODUCTS_AND_WIDEN_2("%0", "%1")
+                     : "+v"(s0), "+v"(s1), "=&v"(n.x), "=&v"(n.y), "=&v"(n.z), "=&v"(n.w)
+                     : "v"(cur), "v"(q0), "v"(q1), "v"(w0), "v"(w1));
+    return __builtin_bit_cast(half8_t, n);
+}
+__device__ __forceinline__ half8_t value_products(float4_t& o0, float4_t& o1, half8_t cur, half8_t p0, half8_t p1, unsigned w0,
+                                                  unsigned w1) {
+    uint4_t n;
+    asm volatile(PD_PRODUCTS_AND_WIDEN_2("%0", "%1")
+                 : "+a"(o0), "+a"(o1), "=&v"(n.x), "=&v"(n.y), "=&v"(n.z), "=&v"(n.w)
+                 : "v"(cur), "v"(p0), "v"(p1), "v"(w0), "v"(w1));
+    return __builtin_bit_cast(half8_t, n);
+}
+__device__ __forceinline__ void value_products_only(float4_t& o0, float4_t& o1, half8_t cur, half8_t p0, half8_t p1) {
+    asm volatile("v_mfma_f32_16x16x32_f16 %0, %2, %3, %0\n\tv_mfma_f32_16x16x32_f16 %1, %2, %4, %1"
+                 : "+a"(o0), "+a"(o1)
+                 : "v"(cur), "v"(p0), "v"(p1));
+}
 // Wait states between asm MFMAs and the first other instruction that touches their results (the
 // operands keep the compiler from moving such an instruction before the wait).
+__device__ __forceinline__ void settle_scores(float4_t (&s)[2][2]) {
+    asm volatile("s_nop 15" : "+v"(s[0][0]), "+v"(s[0][1]), "+v"(s[1][0]), "+v"(s[1][1]));
+}
 __device__ __forceinline__ void settle_scores(float4_t (&s)[kFwRB][2]) {
     asm volatile("s_nop 15" : "+v"(s[0][0]), "+v"(s[0][1]), "+v"(s[1][0]), "+v"(s[1][1]), "+v"(s[2][0]), "+v"(s[2][1]),
                  "+v"(s[3][0]), "+v"(s[3][1]));
@@ -98,6 +137,13 @@ __device__ __forceinline__ void settle_values(float4_t (&o)[16]) {
     asm volatile("" : "+a"(o[8]), "+a"(o[9]), "+a"(o[10]), "+a"(o[11]), "+a"(o[12]), "+a"(o[13]), "+a"(o[14]), "+a"(o[15]));
 }
 // The wait before the products of P' (see settle_operand), once for all of its row blocks.
+template <bool kExact>
+__device__ __forceinline__ void settle_weights(half8_t (&p)[2], half8_t (&lo)[2]) {
+    if constexpr (kExact)
+        asm volatile("s_nop 1" : "+v"(p[0]), "+v"(p[1]), "+v"(lo[0]), "+v"(lo[1]));
+    else
+        asm volatile("s_nop 1" : "+v"(p[0]), "+v"(p[1]));
+}
 template <bool kExact>
 __device__ __forceinline__ void settle_weights(half8_t (&p)[kFwRB], half8_t (&lo)[kFwRB]) {
     if constexpr (kExact)
@@ -132,7 +178,7 @@ struct FwSeen {
     __device__ __forceinline__ bool has(int k) const { return ((k >= lo) | (k < sinks)) & (k < hi); }
 };
 
-// Query tiles of a windowed launch: each sequence's rows [query_start[i], query_start[i + 1]) in runs of 256, sequence by sequence;
+// Query tiles of a windowed launch: each sequence's rows [query_start[i], query_start[i + 1]) in runs of kRows, sequence by sequence;
 // sequences without keys have none. (A wave looks 64 sequences up at a time.)
 struct FwItem {
     int b, tile, first, ntok;  // sequence, its query tile, its first row, its tokens
@@ -142,26 +188,29 @@ struct FwTiles {
     int first0, end0;
     unsigned total;
 };
+template <int kRows>
 __device__ __forceinline__ unsigned fw_tiles(const FaWindow& w, const int* seq_lens, int G, int i, int& first, int& end) {
     const int c = min(i, w.num_seqs - 1);
     first = max(0, w.query_start[c]);
     end = min(w.query_start[c + 1], w.num_tokens);
     const bool live = i < w.num_seqs && end > first && seq_lens[c] > 0;
-    return live ? (unsigned)(((int64_t)(end - first) * G + kFwRows - 1) / kFwRows) : 0u;
+    return live ? (unsigned)(((int64_t)(end - first) * G + kRows - 1) / kRows) : 0u;
 }
+template <int kRows>
 __device__ __forceinline__ FwTiles fw_count(const FaWindow& w, const int* seq_lens, int G) {
     const int lane = threadIdx.x & 63;
     FwTiles t;
-    t.tiles0 = fw_tiles(w, seq_lens, G, lane, t.first0, t.end0);
+    t.tiles0 = fw_tiles<kRows>(w, seq_lens, G, lane, t.first0, t.end0);
     t.incl0 = wave_scan(t.tiles0);
     t.total = (unsigned)__builtin_amdgcn_readlane((int)t.incl0, 63);
     for (int c = 64; c < w.num_seqs; c += 64) {
         int first, end;
-        t.total += (unsigned)__builtin_amdgcn_readlane((int)wave_scan(fw_tiles(w, seq_lens, G, c + lane, first, end)), 63);
+        t.total += (unsigned)__builtin_amdgcn_readlane((int)wave_scan(fw_tiles<kRows>(w, seq_lens, G, c + lane, first, end)), 63);
     }
     return t;
 }
 // Query tile x < total.
+template <int kRows>
 __device__ __forceinline__ FwItem fw_item(const FaWindow& w, const int* seq_lens, int G, const FwTiles& t, unsigned x) {
     const int lane = threadIdx.x & 63;
     unsigned before = 0;
@@ -169,7 +218,7 @@ __device__ __forceinline__ FwItem fw_item(const FaWindow& w, const int* seq_lens
         int first = t.first0, end = t.end0;
         unsigned tiles = t.tiles0, incl = t.incl0;
         if (c > 0) {
-            tiles = fw_tiles(w, seq_lens, G, c + lane, first, end);
+            tiles = fw_tiles<kRows>(w, seq_lens, G, c + lane, first, end);
             incl = wave_scan(tiles);
         }
         const int k = __popcll(__ballot(before + incl <= x));
@@ -192,14 +241,14 @@ __device__ __forceinline__ unsigned fw_order(unsigned lin, unsigned count) {
 }
 
 // A workgroup of pd_prefill_wide_kernel and, with kWindow, of pd_window_kernel.
-template <bool kFast, bool kExact, bool kSplit, class T, bool kWindow>
+template <bool kFast, bool kExact, bool kSplit, class T, bool kWindow, int kRB>
 __device__ __forceinline__ void wide_workgroup(const FaParams& a, const FaWindow& win, unsigned char* lds) {
-    constexpr int kLdsBt = kFwLdsBt, kLdsScr = kFwLdsScr;
+    constexpr int kLdsBt = kFwLdsBt, kLdsScr = kFwLdsScr, kRows = 16 * kRB * kFwWaves;
     int x, g, b, qt, split, ntok = a.Sq, first = 0;
     if constexpr (kWindow) {
         // The order of the work: runs of 32 query tiles, the last tiles first (those of a fresh prompt see the most keys), and for each
         // run all kv heads and splits.
-        const FwTiles tiles = fw_count(win, a.seq_lens, a.G);
+        const FwTiles tiles = fw_count<kRows>(win, a.seq_lens, a.G);
         const unsigned lin = blockIdx.x + gridDim.x * blockIdx.y, each = gridDim.y * (unsigned)a.nsplit, count = tiles.total * each;
         if (lin >= count) return;
         const unsigned at = fw_order(lin, count), run = at / (32u * each), width = min(32u, tiles.total - 32u * run);
@@ -207,7 +256,7 @@ __device__ __forceinline__ void wide_workgroup(const FaParams& a, const FaWindow
         x = (int)(tiles.total - 1 - (32u * run + in - job * width));
         g = (int)(job / (unsigned)a.nsplit);
         split = (int)(job - (unsigned)g * (unsigned)a.nsplit);
-        const FwItem item = fw_item(win, a.seq_lens, a.G, tiles, (unsigned)x);
+        const FwItem item = fw_item<kRows>(win, a.seq_lens, a.G, tiles, (unsigned)x);
         b = item.b, qt = item.tile, ntok = item.ntok, first = item.first;
     } else {
         // Workgroups are dispatched to the 8 XCDs round robin (linear id L to XCD L % 8), and each XCD
@@ -228,8 +277,8 @@ __device__ __forceinline__ void wide_workgroup(const FaParams& a, const FaWindow
     const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int G = a.G;
     // rows of this workgroup: [row0, row0 + nrow) of the sequence's (token, head) rows
-    const int64_t row0 = (int64_t)qt * kFwRows;
-    const int nrow = (int)min((int64_t)kFwRows, (int64_t)ntok * G - row0);
+    const int64_t row0 = (int64_t)qt * kRows;
+    const int nrow = (int)min((int64_t)kRows, (int64_t)ntok * G - row0);
     const int tok0 = (int)(row0 / G), tok_last = (int)((row0 + nrow - 1) / G);
     const int tok0_row = (int)(row0 - (int64_t)tok0 * G);  // rows of the first token that come before
     const int seq_len = a.seq_lens[b];
@@ -279,11 +328,11 @@ __device__ __forceinline__ void wide_workgroup(const FaParams& a, const FaWindow
         x.tok += tok0;
         return x;
     };
-    auto row_of = [&](int rb) __attribute__((always_inline)) { return row_at(64 * w + 16 * rb + (lane_here() & 15)); };
-    half8_t qop[kFwRB][8];
+    auto row_of = [&](int rb) __attribute__((always_inline)) { return row_at(16 * kRB * w + 16 * rb + (lane_here() & 15)); };
+    half8_t qop[kRB][8];
     auto load_q = [&]() __attribute__((always_inline)) {
 #pragma unroll
-        for (int rb = 0; rb < kFwRB; ++rb) {
+        for (int rb = 0; rb < kRB; ++rb) {
             const Row r = row_of(rb);
             const T* qrow = static_cast<const T*>(a.q) + (kWindow ? (int64_t)first * a.q_st : (int64_t)b * a.q_sb) +
                             (int64_t)(g * G + r.head) * a.q_sh + (int64_t)r.tok * a.q_st;
@@ -345,13 +394,13 @@ __device__ __forceinline__ void wide_workgroup(const FaParams& a, const FaWindow
     // Relative scores carry +kPLog2: p' = 2^(s - m + kPLog2) = 16 p, so P' = p' * v_scale spans the
     // same fp16 range as in the decode kernel; l accumulates p' and the final 1 / l removes it.
     constexpr float kPLog2 = 4.0f;
-    float l_run[kFwRB];
+    float l_run[kRB];
     // per row: the score offset -m + kPLog2 (kPLog2 while the row has seen no key) and the
     // relative score above which the running max m must be raised (any finite score while fresh)
-    float nm_run[kFwRB], thr_run[kFwRB];
-    float4_t oacc[kFwRB][16];
+    float nm_run[kRB], thr_run[kRB];
+    float4_t oacc[kRB][16];
 #pragma unroll
-    for (int rb = 0; rb < kFwRB; ++rb) {
+    for (int rb = 0; rb < kRB; ++rb) {
         l_run[rb] = 0.f;
         nm_run[rb] = kPLog2;
         thr_run[rb] = kNegInf;
@@ -396,8 +445,8 @@ __device__ __forceinline__ void wide_workgroup(const FaParams& a, const FaWindow
     // ---- tile n from its slot S (its first reads are under way); mid() runs between the scores and the
     //      softmax, next() before the last products ----
     auto tile = [&](int n, const lds_u8* S, auto mid, auto next) __attribute__((always_inline)) {
-        float4_t sacc[kFwRB][2];
-        constexpr int kVAhead = 2;
+        float4_t sacc[kRB][2];
+        constexpr int kVAhead = kRB == 4 ? 2 : 4;  // (a narrow workgroup's products of an operand take half as long)
         int2_t vr[16];
         auto vread = [&](int m) __attribute__((always_inline)) {
             vr[m] = __builtin_amdgcn_ds_read_tr8_b64_v2i32((lds_int2*)(S + (m < 8 ? vro_lo : vro_hi) + 16 * m));
@@ -415,16 +464,24 @@ __device__ __forceinline__ void wide_workgroup(const FaParams& a, const FaWindow
 #pragma unroll
                 for (int m = 1; m < kVAhead; ++m) vread(m);
             }
-            if (c == 0)
-                op = score_products<true>(sacc[0][u], sacc[1][u], sacc[2][u], sacc[3][u], op, qop[0][2 * c], qop[1][2 * c],
-                                          qop[2][2 * c], qop[3][2 * c], kr[i % 3].z, kr[i % 3].w);
-            else
-                op = score_products<false>(sacc[0][u], sacc[1][u], sacc[2][u], sacc[3][u], op, qop[0][2 * c], qop[1][2 * c],
-                                           qop[2][2 * c], qop[3][2 * c], kr[i % 3].z, kr[i % 3].w);
             // the operand after the last is the first of V
             const unsigned w0 = i < 7 ? kr[(i + 1) % 3].x : (unsigned)vr[0].x, w1 = i < 7 ? kr[(i + 1) % 3].y : (unsigned)vr[0].y;
-            op = score_products<false>(sacc[0][u], sacc[1][u], sacc[2][u], sacc[3][u], op, qop[0][2 * c + 1],
-                                       qop[1][2 * c + 1], qop[2][2 * c + 1], qop[3][2 * c + 1], w0, w1);
+            if constexpr (kRB == 4) {
+                if (c == 0)
+                    op = score_products<true>(sacc[0][u], sacc[1][u], sacc[2][u], sacc[3][u], op, qop[0][2 * c], qop[1][2 * c],
+                                              qop[2][2 * c], qop[3][2 * c], kr[i % 3].z, kr[i % 3].w);
+                else
+                    op = score_products<false>(sacc[0][u], sacc[1][u], sacc[2][u], sacc[3][u], op, qop[0][2 * c], qop[1][2 * c],
+                                               qop[2][2 * c], qop[3][2 * c], kr[i % 3].z, kr[i % 3].w);
+                op = score_products<false>(sacc[0][u], sacc[1][u], sacc[2][u], sacc[3][u], op, qop[0][2 * c + 1],
+                                           qop[1][2 * c + 1], qop[2][2 * c + 1], qop[3][2 * c + 1], w0, w1);
+            } else {
+                if (c == 0)
+                    op = score_products<true>(sacc[0][u], sacc[1][u], op, qop[0][2 * c], qop[1][2 * c], kr[i % 3].z, kr[i % 3].w);
+                else
+                    op = score_products<false>(sacc[0][u], sacc[1][u], op, qop[0][2 * c], qop[1][2 * c], kr[i % 3].z, kr[i % 3].w);
+                op = score_products<false>(sacc[0][u], sacc[1][u], op, qop[0][2 * c + 1], qop[1][2 * c + 1], w0, w1);
+            }
         }
         float ks[8], vs[8];
 #pragma unroll
@@ -434,9 +491,9 @@ __device__ __forceinline__ void wide_workgroup(const FaParams& a, const FaWindow
         }
         mid();
         settle_scores(sacc);
-        float sv[kFwRB][8];
+        float sv[kRB][8];
 #pragma unroll
-        for (int rb = 0; rb < kFwRB; ++rb)
+        for (int rb = 0; rb < kRB; ++rb)
 #pragma unroll
             for (int e = 0; e < 8; ++e) sv[rb][e] = __builtin_fmaf(sacc[rb][e >> 2][e & 3], ks[e], nm_run[rb]);
         if constexpr (kWindow) {
@@ -444,12 +501,12 @@ __device__ __forceinline__ void wide_workgroup(const FaParams& a, const FaWindow
             if (kb + kTile - 1 > pmin || (kb + kTile > seen.sinks && qabs + tok_last - kb >= win.window)) {
                 // some row does not see all of the tile; keys that none sees may hold garbage scales: v_scale 0
                 const int lane = lane_here(), key = kb + 4 * (lane >> 4);
-                const lds_int* pos = (const lds_int*)(L + kFwLdsPos) + 64 * w + (lane & 15);
+                const lds_int* pos = (const lds_int*)(L + kFwLdsPos) + 16 * kRB * w + (lane & 15);
                 const bool sinks = kb < seen.sinks;  // uniform
 #pragma unroll
                 for (int e = 0; e < 8; ++e) vs[e] = seen.has(key + 16 * (e >> 2) + (e & 3)) ? vs[e] : 0.f;
 #pragma unroll
-                for (int rb = 0; rb < kFwRB; ++rb) {
+                for (int rb = 0; rb < kRB; ++rb) {
                     const int ahead = pos[16 * rb] - key;  // of the tile's first key of this lane; a row that is not there is at -1
 #pragma unroll
                     for (int e = 0; e < 8; ++e) {
@@ -466,7 +523,7 @@ __device__ __forceinline__ void wide_workgroup(const FaParams& a, const FaWindow
 #pragma unroll
             for (int e = 0; e < 8; ++e) vs[e] = key + 16 * (e >> 2) + (e & 3) < hi ? vs[e] : 0.f;
 #pragma unroll
-            for (int rb = 0; rb < kFwRB; ++rb) {
+            for (int rb = 0; rb < kRB; ++rb) {
                 const Row row = row_of(rb);
                 const int last = row.valid ? min(hi - 1, qabs + row.tok) : -1;
 #pragma unroll
@@ -475,7 +532,7 @@ __device__ __forceinline__ void wide_workgroup(const FaParams& a, const FaWindow
         }
         uint64_t need = 0;
 #pragma unroll
-        for (int rb = 0; rb < kFwRB; ++rb) {
+        for (int rb = 0; rb < kRB; ++rb) {
             float mx = kNegInf;
 #pragma unroll
             for (int e = 0; e < 8; ++e) mx = fmaxf(mx, sv[rb][e]);
@@ -485,7 +542,7 @@ __device__ __forceinline__ void wide_workgroup(const FaParams& a, const FaWindow
         // state (O is still zero while every row of a block is fresh: no rescale then)
         if (need != 0) {
 #pragma unroll
-            for (int rb = 0; rb < kFwRB; ++rb) {
+            for (int rb = 0; rb < kRB; ++rb) {
                 float mloc = kNegInf;
 #pragma unroll
                 for (int e = 0; e < 8; ++e) mloc = fmaxf(mloc, sv[rb][e]);
@@ -509,9 +566,9 @@ __device__ __forceinline__ void wide_workgroup(const FaParams& a, const FaWindow
             }
         }
         // p' = 2^sv, P' = p' * v_scale in fp16, O^T += V^T P'^T
-        half8_t pop[kFwRB], plo[kFwRB];
+        half8_t pop[kRB], plo[kRB];
 #pragma unroll
-        for (int rb = 0; rb < kFwRB; ++rb) {
+        for (int rb = 0; rb < kRB; ++rb) {
             float psum = 0.f;
 #pragma unroll
             for (int e = 0; e < 8; e += 2) {
@@ -538,18 +595,26 @@ __device__ __forceinline__ void wide_workgroup(const FaParams& a, const FaWindow
 #pragma unroll
         for (int m = 0; m < 16; ++m) {
             if (m + kVAhead < 16) vread(m + kVAhead);
-            if (m == 14) next();
-            if constexpr (kExact) value_products_only(oacc[0][m], oacc[1][m], oacc[2][m], oacc[3][m], op, plo[0], plo[1], plo[2], plo[3]);
-            if (m < 15)
-                op = value_products(oacc[0][m], oacc[1][m], oacc[2][m], oacc[3][m], op, pop[0], pop[1], pop[2], pop[3],
-                                    (unsigned)vr[m + 1].x, (unsigned)vr[m + 1].y);
-            else
-                value_products_only(oacc[0][m], oacc[1][m], oacc[2][m], oacc[3][m], op, pop[0], pop[1], pop[2], pop[3]);
+            if (m == (kRB == 4 ? 14 : 12)) next();
+            if constexpr (kRB == 4) {
+                if constexpr (kExact) value_products_only(oacc[0][m], oacc[1][m], oacc[2][m], oacc[3][m], op, plo[0], plo[1], plo[2], plo[3]);
+                if (m < 15)
+                    op = value_products(oacc[0][m], oacc[1][m], oacc[2][m], oacc[3][m], op, pop[0], pop[1], pop[2], pop[3],
+                                        (unsigned)vr[m + 1].x, (unsigned)vr[m + 1].y);
+                else
+                    value_products_only(oacc[0][m], oacc[1][m], oacc[2][m], oacc[3][m], op, pop[0], pop[1], pop[2], pop[3]);
+            } else {
+                if constexpr (kExact) value_products_only(oacc[0][m], oacc[1][m], op, plo[0], plo[1]);
+                if (m < 15)
+                    op = value_products(oacc[0][m], oacc[1][m], op, pop[0], pop[1], (unsigned)vr[m + 1].x, (unsigned)vr[m + 1].y);
+                else
+                    value_products_only(oacc[0][m], oacc[1][m], op, pop[0], pop[1]);
+            }
         }
     };
 
     const int nsteps = (t1 - t0 + kFwStep - 1) / kFwStep;
-    const bool busy = 64 * w < nrow;  // a wave without rows only copies
+    const bool busy = 16 * kRB * w < nrow;  // a wave without rows only copies
 
     auto tile_loop = [&](auto lds_flag) __attribute__((always_inline)) {
         constexpr bool kLds = decltype(lds_flag)::value;
@@ -671,7 +736,7 @@ __device__ __forceinline__ void wide_workgroup(const FaParams& a, const FaWindow
         // of 8 bytes take 7.4 us of a workgroup, whole rows side by side 4.0. Each thread works out one row's place.
         constexpr int kRow = 2 * kDim + 16;  // bytes of a row in LDS, its neighbours on other banks
         constexpr int kPart = kFwRing * kFwSlot / kFwWaves / 16 * 16;
-        static_assert(16 * kRow <= kPart && kFwRows * 8 <= kFwWaves * 4096, "a row block's rows fit a wave's part of the ring, places the scratch");
+        static_assert(16 * kRow <= kPart && kRows * 8 <= kFwWaves * 4096, "a row block's rows fit a wave's part of the ring, places the scratch");
         typedef _Float16 half4_t __attribute__((ext_vector_type(4)));
         typedef __attribute__((address_space(3))) half4_t lds_half4;
         lds_u64* place = (lds_u64*)(L + kLdsScr);
@@ -684,7 +749,7 @@ __device__ __forceinline__ void wide_workgroup(const FaParams& a, const FaWindow
         if (!busy) return;
         lds_u8* mine = L + w * kPart;
 #pragma unroll
-        for (int rb = 0; rb < kFwRB; ++rb) {
+        for (int rb = 0; rb < kRB; ++rb) {
             const int lane = lane_here(), lg = lane >> 4, li = lane & 15;
             settle_values(oacc[rb]);
             const float l_row = xor_sum(xor_sum(l_run[rb], 16), 32);
@@ -696,7 +761,7 @@ __device__ __forceinline__ void wide_workgroup(const FaParams& a, const FaWindow
             }
 #pragma unroll
             for (int j = 0; j < 8; ++j) {  // two rows at a time
-                const int at = 2 * j + (lane >> 5), r = 64 * w + 16 * rb + at;
+                const int at = 2 * j + (lane >> 5), r = 16 * kRB * w + 16 * rb + at;
                 const uint4_t v = *(const lds_uint4*)(mine + at * kRow + 16 * (lane & 31));
                 T* to = static_cast<T*>(a.out) + (int64_t)place[r] + 8 * (lane & 31);
                 if (r < nrow) __builtin_memcpy(__builtin_assume_aligned(to, 8), &v, 16);
@@ -705,7 +770,7 @@ __device__ __forceinline__ void wide_workgroup(const FaParams& a, const FaWindow
         return;
     }
 #pragma unroll
-    for (int rb = 0; rb < kFwRB; ++rb) {
+    for (int rb = 0; rb < kRB; ++rb) {
         const int lg = l >> 4;
         settle_values(oacc[rb]);
         const float l_row = xor_sum(xor_sum(l_run[rb], 16), 32);
@@ -733,19 +798,20 @@ __device__ __forceinline__ void wide_workgroup(const FaParams& a, const FaWindow
 template <bool kFast, bool kExact, bool kSplit, class T>
 __global__ void __launch_bounds__(kFwWaves * 64, 1) pd_prefill_wide_kernel(const FaParams a) {
     __shared__ __attribute__((aligned(16))) unsigned char lds[kFwLdsBytes];
-    wide_workgroup<kFast, kExact, kSplit, T, false>(a, FaWindow{}, lds);
+    wide_workgroup<kFast, kExact, kSplit, T, false, kFwRB>(a, FaWindow{}, lds);
 }
 
 // Chunks whose rows see a sliding window and the first `sinks` keys: the row at position p sees key k <= p if p - k < window or
 // k < sinks. A query tile streams the tiles that hold a key that one of its rows sees, those of the sinks, then the window's (window + 43
 // keys for 256 rows of 6 heads), so a chunk's time goes with tokens x window, whatever lies before; pages that hold nothing
-// seen are never addressed. Tiles at the window's two ends and the last of the sinks are masked row by row, the others
+// seen are never addressed. kRB: 16-row blocks of a wave, 4 or 2 (pd_plan.hpp says which call takes which; two wait less for set-up,
+// Q and stores, but each conversion then serves half the products). Tiles at the window's two ends and the last of the sinks are masked row by row, the others
 // are not. Several sequences' rows lie one after the other; which a workgroup has is looked up on the device, so that a captured
 // launch takes any batch of as many rows and sequences.
-template <bool kFast, bool kExact, bool kSplit>
+template <bool kFast, bool kExact, bool kSplit, int kRB>
 __global__ void __launch_bounds__(kFwWaves * 64, 1) pd_window_kernel(const FaParams a, const FaWindow win) {
     __shared__ __attribute__((aligned(16))) unsigned char lds[kFwWindowLdsBytes];
-    wide_workgroup<kFast, kExact, kSplit, _Float16, true>(a, win, lds);
+    wide_workgroup<kFast, kExact, kSplit, _Float16, true, kRB>(a, win, lds);
 }
 
 // Log-sum-exp merge of a split windowed launch: a wave per (token, head) row, lane l owning dims 4 l .. 4 l + 3; M = max_s m_s,
@@ -824,27 +890,27 @@ hipError_t launch_prefill_wide(const FaParams& p, int batch, int heads_kv, int d
     return hipGetLastError();
 }
 
-template <bool kSplit>
-static void launch_window_split(const FaParams& p, const FaWindow& w, dim3 grid, hipStream_t stream, bool fast, bool exact) {
+template <bool kSplit, int kRB>
+static void launch_window_rows(const FaParams& p, const FaWindow& w, dim3 grid, hipStream_t stream, bool fast, bool exact) {
     const dim3 block(kFwWaves * 64);
     if (fast && !exact)
-        hipLaunchKernelGGL((pd_window_kernel<true, false, kSplit>), grid, block, 0, stream, p, w);
+        hipLaunchKernelGGL((pd_window_kernel<true, false, kSplit, kRB>), grid, block, 0, stream, p, w);
     else if (!exact)
-        hipLaunchKernelGGL((pd_window_kernel<false, false, kSplit>), grid, block, 0, stream, p, w);
+        hipLaunchKernelGGL((pd_window_kernel<false, false, kSplit, kRB>), grid, block, 0, stream, p, w);
     else if (fast)
-        hipLaunchKernelGGL((pd_window_kernel<true, true, kSplit>), grid, block, 0, stream, p, w);
+        hipLaunchKernelGGL((pd_window_kernel<true, true, kSplit, kRB>), grid, block, 0, stream, p, w);
     else
-        hipLaunchKernelGGL((pd_window_kernel<false, true, kSplit>), grid, block, 0, stream, p, w);
+        hipLaunchKernelGGL((pd_window_kernel<false, true, kSplit, kRB>), grid, block, 0, stream, p, w);
 }
 
-hipError_t launch_window(const FaParams& p, const FaWindow& w, int heads_kv, hipStream_t stream, bool exact) {
-    const dim3 grid((unsigned)(window_tiles(w.num_tokens, w.num_seqs, p.G) * p.nsplit), heads_kv);
-    const bool fast = fast_block_table(p.block_size, p.k_ss);
+hipError_t launch_window(const FaParams& p, const FaWindow& w, int rows, int heads_kv, hipStream_t stream, bool exact) {
+    const dim3 grid((unsigned)(window_tiles(w.num_tokens, w.num_seqs, p.G, rows) * p.nsplit), heads_kv);
+    const bool fast = fast_block_table(p.block_size, p.k_ss), narrow = rows != kFwRows;
     if (p.nsplit == 1) {
-        launch_window_split<false>(p, w, grid, stream, fast, exact);
+        narrow ? launch_window_rows<false, 2>(p, w, grid, stream, fast, exact) : launch_window_rows<false, 4>(p, w, grid, stream, fast, exact);
         return hipGetLastError();
     }
-    launch_window_split<true>(p, w, grid, stream, fast, exact);
+    narrow ? launch_window_rows<true, 2>(p, w, grid, stream, fast, exact) : launch_window_rows<true, 4>(p, w, grid, stream, fast, exact);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
     hipLaunchKernelGGL(pd_window_combine_kernel, dim3((unsigned)((w.num_tokens + 3) / 4), p.Hq), dim3(256), 0, stream, p, w);

@@ -14,7 +14,7 @@ import torch
 import workload as kvc
 from mi50_vllm_lab_amd import pth_dec
 
-TILE, ROWS = 32, 256
+TILE = 32
 CSRC = os.path.join(os.path.dirname(pth_dec.__file__), "csrc")
 
 
@@ -47,7 +47,8 @@ def test_tiles_of_all_sequences_fit_the_launch(group):
     rng = random.Random(group)
     for _ in range(300):
         news = [rng.choice([0, 1, rng.randint(1, 700)]) for _ in range(rng.randint(1, 90))]
-        assert sum(-(-n * group // ROWS) for n in news) <= sum(news) * group // ROWS + len(news)
+        for rows in (128, 256):
+            assert sum(-(-n * group // rows) for n in news) <= sum(news) * group // rows + len(news)
 
 
 class Seen:
@@ -104,23 +105,28 @@ def test_tiles_cover_what_is_seen(span, sinks):
 
 def test_planned_splits():
     text = open(os.path.join(CSRC, "pd_plan.hpp")).read()
-    setup, merge, mb = map(float, re.search(r"kFwSetupUs = ([\d.]+), kFwMergeUs = ([\d.]+), kFwPartialUsPerMb = ([\d.]+);", text).groups())
+    times = [tuple(map(float, re.search(r"%s = \{([\d.]+), ([\d.]+), ([\d.]+)\}" % n, text).groups())) for n in ("kFwWide", "kFwNarrow")]
+    merge, mb = map(float, re.search(r"kFwMergeUs = ([\d.]+), kFwPartialUsPerMb = ([\d.]+);", text).groups())
     most = int(re.search(r"kFwMaxSplits = (\d+);", text).group(1))
-    tile = [float(re.search(r"%s = \{[\d.]+, ([\d.]+)," % n, text).group(1)) for n in ("kFaTimes", "kFaTimesExact")]
     lib = pth_dec.load_library()
 
     def want(T, seqs, hq, hkv, window, sinks, keys, exact, cus=256):
         g = hq // hkv
-        span = window + -(-ROWS // g) + 31
-        tiles = -(-min(span, max(1, keys)) // 32) + -(-min(sinks, max(0, keys - span)) // 32)
-        items = (-(-T * g // ROWS) + (seqs - 1) // 2) * hkv
+
+        def key_tiles(rows):
+            span = window + -(-rows // g) + 31
+            return -(-min(span, max(1, keys)) // 32) + -(-min(sinks, max(0, keys - span)) // 32)
+
         best = None
         for s in range(1, most + 1):
-            if s > 1 and s * 4 > tiles:
+            if s > 1 and s * 4 > key_tiles(128):
                 break
-            us = -(-items * s // cus) * (-(-tiles // s) * tile[exact] + setup) + (merge + mb * T * hq * s * 1032 / 1e6 if s > 1 else 0)
-            if best is None or us < best[0]:
-                best = (us, s)
+            for rows, t in ((256, times[0]), (128, times[1])):
+                items = (-(-T * g // rows) + (seqs - 1) // 2) * hkv * s
+                us = -(-items // cus) * (-(-key_tiles(rows) // s) * t[exact] + t[2])
+                us += merge + mb * T * hq * s * 1032 / 1e6 if s > 1 else 0
+                if best is None or us < best[0]:
+                    best = (us, s)
         return best[1]
 
     rng = random.Random(3)
@@ -129,8 +135,9 @@ def test_planned_splits():
         a = (rng.choice([1, 16, 64, 300, 2048, 8192]), rng.choice([1, 2, 9, 70]), hq, hkv, rng.choice([1, 100, 1000, 4096]),
              rng.choice([0, 4, 500]), rng.choice([0, 100, 5000, 100000]), rng.choice([0, 1]))
         assert lib.pth_fa_window_splits(*a) == want(*a), a
-    assert lib.pth_fa_window_splits(8192, 1, 24, 4, 4096, 4, 100000, 0) == 1   # several rounds of workgroups
-    assert lib.pth_fa_window_splits(64, 1, 24, 4, 2048, 4, 100000, 0) > 4      # 8 of them
+    assert lib.pth_fa_window_splits(8192, 1, 24, 4, 4096, 4, 100000, 0) == 1   # three rounds of wide workgroups
+    assert lib.pth_fa_window_splits(1024, 1, 24, 4, 1024, 4, 100000, 0) == 1   # 192 narrow ones
+    assert lib.pth_fa_window_splits(64, 1, 24, 4, 2048, 4, 100000, 0) > 4      # 12 of them
     for bad in ((0, 1, 24, 4, 9, 0, 9, 0), (9, 0, 24, 4, 9, 0, 9, 0), (9, 1, 24, 5, 9, 0, 9, 0), (9, 1, 24, 4, 0, 0, 9, 0), (9, 1, 24, 0, 9, 0, 9, 0)):
         assert lib.pth_fa_window_splits(*bad) == 1
 

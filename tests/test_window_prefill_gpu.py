@@ -87,12 +87,14 @@ def test_outlier_sinks_with_hi_and_lo_weights():
     check(case, 512, 4, ((1, True), (4, True)))
 
 
-def test_long_chunk_against_float64_of_some_rows():
-    """3,000 fresh tokens on top of 500 over a window of 1,500: several rounds of workgroups, interior tiles without masks."""
+@pytest.mark.parametrize("exact", [False, True])
+def test_long_chunk_against_float64_of_some_rows(exact):
+    """3,000 fresh tokens on top of 500 over a window of 1,500: wide workgroups (the shorter calls here run narrow ones), several
+    rounds of them, interior tiles without masks."""
     window, sinks, ctx, new = 1500, 37, 500, 3000
     case = kvc.make_case([ctx], [new], seed=9)
     bt, _ = window_oracle.freed(case, window, sinks)
-    out = run(case, bt, window, sinks).double().numpy()
+    out = run(case, bt, window, sinks, exact=exact).double().numpy()
     key = torch.arange(ctx + new)
     c = case.cache
     k, v = (x[bt[0].long()[key // 16], key % 16, :, :256].double() * s[bt[0].long()[key // 16], key % 16].double()[..., None]
@@ -104,6 +106,14 @@ def test_long_chunk_against_float64_of_some_rows():
             x = torch.mv(k[see, h // 6], case.q[i, h].double()) * case.scale
             ref = torch.softmax(x, 0) @ v[see, h // 6]
             assert kvc.fp16_output_errors(out[i, h], ref.numpy())[2] <= 0, (i, h)
+
+
+@pytest.mark.parametrize("lens,bs,layout,nsplit,exact", [
+    ([2100, 700], 16, "HND", 1, False), ([1500, 900, 5, 800], 16, "NHD", 2, False), ([2500], 24, "HND", 1, True), ([2900], 1, "NHD", 2, True)])
+def test_wide_workgroups(lens, bs, layout, nsplit, exact):
+    """More rows than narrow workgroups take in a round, over a short window: every row against float64."""
+    case = kvc.make_case([300, 0, 70, 41][:len(lens)], lens, block_size=bs, layout=layout, seed=bs + len(lens))
+    check(case, 150, 21, ((nsplit, exact),))
 
 
 def test_a_window_of_everything_is_the_prefill():
