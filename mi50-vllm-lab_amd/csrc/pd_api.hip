@@ -648,7 +648,8 @@ int pth_fa_forward_window(const pd_tensor* q, const pd_tensor* key_cache, const 
         p.part_m = p.part_o + rows * kDim;
         p.part_l = p.part_m + rows;
     }
-    const FaWindow w = {static_cast<const int*>(query_start_loc->data), (int)num_seqs, (int)T, (int)window, (int)sinks};
+    const FaWindow w = {static_cast<const int*>(query_start_loc->data), (int)num_seqs, (int)T,
+                         (int)std::min<int64_t>(window, 1 << 30), (int)sinks};  // (no sequence is longer; see launch_partial)
     const int cus = compute_units(stream);
     const FwCall call = {T, num_seqs, Hq, Hkv, window, sinks, block_table->sizes[1] * bs, cus > 0 ? cus : 256, exact != 0};
     return fa_result(launch_window(p, w, fw_narrow(call, nsplit) ? kFwNarrowRows : kFwRows, (int)Hkv, stream, exact != 0), err, errlen);

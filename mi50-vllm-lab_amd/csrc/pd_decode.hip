@@ -62,6 +62,7 @@
 //
 // Nothing is allocated, nothing waits for the host, and every split range is derived on
 // the device from seq_lens / query_start_loc, so launches can be captured in a HIP graph.
+#include <algorithm>
 #include <atomic>
 #include <mutex>
 
@@ -1440,7 +1441,7 @@ hipError_t launch_partial(const LaunchArgs& x, hipStream_t stream, int* balanced
     p.G = x.heads_q / x.heads_kv;
     p.qmax = x.qmax;
     p.Hq = x.heads_q;
-    p.window = x.window > 0 ? x.window : 0;
+    p.window = x.window > 0 ? std::min(x.window, 1 << 30) : 0;  // (no sequence is longer; positions below 0 less it stay in 32 bits)
     p.sinks = x.window > 0 ? x.sinks : 0;
     p.causal = x.causal ? 1 : 0;
     p.bs_shift = (x.block_size & (x.block_size - 1)) == 0 ? __builtin_ctz((unsigned)x.block_size) : -1;

@@ -430,8 +430,8 @@ def forward_window(query: torch.Tensor, key_cache: torch.Tensor, value_cache: to
 
     Sequence i has rows [query_start_loc[i], query_start_loc[i + 1]) of query and out (fp16 [T, Hq, 256]), the last tokens of its
     seq_lens[i] keys; the row at position p sees key k <= p if p - k < window or k < sinks. query_start_loc int32 [sequences + 1], seq_lens and
-    block_table are read on the device, as decode reads them, so a captured call takes any batch of as many rows and sequences. Rows
-    outside the sequences and of sequences without keys are left alone. Pages in which no row sees a key are not addressed.
+    block_table are read on the device, as decode reads them, so a captured call takes any batch of as many rows and sequences. out must
+    not overlap query. Rows outside the sequences and of sequences without keys are left alone. Pages in which no row sees a key are not addressed.
     exact: the softmax weights enter P.V as decode's fp16 hi + lo instead of one fp16, for outlier-heavy caches, at about 20 % more time.
     nsplit: key splits per query tile, with a workspace from torch's allocator; None plans them by the call's sizes (splits of a
     planned call whose workspace cannot be had are left).

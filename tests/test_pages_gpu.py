@@ -183,6 +183,42 @@ def test_steps_in_a_captured_graph():
         lens = [n + 1 for n in lens]
 
 
+def test_the_largest_pool():
+    """4,194,304 pages (of one 520-byte row): as many counts as the prefix holds."""
+    pages = 1 << 22
+    g = torch.Generator(device="cuda").manual_seed(0)
+    kv = torch.randint(-128, 128, (pages, 1, 1, 520), dtype=torch.int8, device="cuda", generator=g)
+    refs = (torch.rand(pages, device="cuda", generator=g) < 0.6).int()
+    free = (refs == 0).nonzero()[:, 0]
+    rows, cols = 40, 60000
+    table = torch.full((rows, cols), -1, dtype=torch.int32, device="cuda")
+    lens = torch.zeros(rows, dtype=torch.int32, device="cuda")
+    new, needed = (torch.empty_like(refs), torch.empty_like(table), torch.empty_like(lens)), torch.zeros(1, dtype=torch.int32, device="cuda")
+    pth_dec.fork_pages([kv], refs, table, lens, None, *new, needed, grow=cols)
+    want = torch.full((rows * cols,), -1, dtype=torch.int32, device="cuda")
+    n = min(free.numel(), rows * cols)
+    want[:n] = free[:n].int()
+    assert int(needed) == rows * cols and free.numel() < rows * cols  # (more than there are)
+    assert torch.equal(new[1].view(-1), want)
+    counts = refs.clone()
+    counts[free[:n]] = 1
+    assert torch.equal(new[0], counts)
+    # compaction of the pool as it was, with tables that name some of its pages
+    live = (refs > 0).nonzero()[:, 0]
+    used, moved = live.numel(), int((live >= live.numel()).sum())
+    table[:, ::3] = live[torch.randint(0, used, table[:, ::3].shape, device="cuda", generator=g)].int()
+    places = torch.full((pages,), -1, dtype=torch.int32, device="cuda")
+    places[live[:used - moved]] = live[:used - moved].int()
+    places[live[used - moved:]] = free[:moved].int()
+    rows_want = kv.clone()
+    rows_want[free[:moved]] = kv[live[used - moved:]]
+    got, count = torch.empty_like(places), torch.zeros(1, dtype=torch.int32, device="cuda")
+    pth_dec.compact_pages([kv], refs, table, new[0], new[1], got, count)
+    assert int(count) == used and torch.equal(got, places) and torch.equal(kv, rows_want)
+    assert torch.equal(new[1], torch.where(table >= 0, places[table.clamp(min=0).long()], -1))
+    assert torch.equal(new[0], (torch.arange(pages, device="cuda") < used).int())
+
+
 def test_two_streams_at_once():
     rng = random.Random(4)
     states = [pool(rng, 40, 1500, 30, 16) for _ in range(2)]

@@ -124,6 +124,22 @@ def test_without_a_window_or_sinks_nothing_changes():
     assert kvc.fp16_output_errors(plain[1].double().numpy()[written], ref[written])[2] <= 0
 
 
+@pytest.mark.parametrize("window,sinks", [((1 << 31) - 1, 5), (1 << 30, (1 << 31) - 1), (40, (1 << 31) - 1)])
+def test_the_largest_windows_and_sinks(window, sinks):
+    """Every key is seen; the first sequence has fewer keys than rows."""
+    case = kvc.make_case([0, 300], [4, 4], seed=13)
+    d = case.to("cuda")
+    lens = torch.tensor([2, 304], dtype=torch.int32)
+    out = torch.full((8, 24, 256), 7.0, dtype=torch.float16, device="cuda")
+    pth_dec.decode(d.q, d.cache.key_cache, d.cache.value_cache, d.cache.k_scale, d.cache.v_scale, d.block_table, lens.cuda(), d.query_start_loc,
+                   out, d.scale, *kvc.partial_buffers(8, 24, 4, "cuda"), 2, 4, 4, window=window, sinks=sinks)
+    assert bool((out[:2] == 0).all())  # positions -2 and -1
+    tail = kvc.DecodeCase(case.q[2:], case.cache, case.block_table, lens, torch.tensor([0, 2, 6], dtype=torch.int32), [0, 300], [2, 4], 24,
+                          case.scale)
+    ref, _, _ = window_oracle.windowed(tail, -1, 0)
+    assert kvc.fp16_output_errors(out[2:].double().cpu().numpy(), ref)[2] <= 0
+
+
 def test_rows_beyond_qmax_and_padding_stay():
     case = kvc.make_case([700, 300, 40], [4, 0, 3], seed=7)
     check(case, 100, 4, True, 4, qmax=2, lse=True)

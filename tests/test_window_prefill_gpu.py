@@ -58,6 +58,8 @@ BOTH = ((1, False), (3, False), (1, True), (7, True))
     (2500, 130, 2048, 4, 32, "HND", 24, 4),
     (200, 20, 90, 5, 16, "HND", 200, 1),         # few tokens to a workgroup
     (200, 9, 90, 5, 16, "HND", 256, 1),
+    (99000, 8, 98500, 40, 16, "HND", 6, 1),      # more 16-key blocks than the LDS table holds, unsplit
+    (150000, 5, 300, 20, 24, "NHD", 6, 1),       # more pages than it holds
 ])
 def test_one_sequence(ctx, new, window, sinks, bs, layout, hq, hkv):
     case = kvc.make_case([ctx], [new], num_q_heads=hq, num_kv_heads=hkv, block_size=bs, layout=layout, seed=ctx + window + sinks)
@@ -174,6 +176,23 @@ def test_offsets_beyond_the_rows_are_left_out():
                                torch.tensor([0, last], dtype=torch.int32, device="cuda"), out, 64, sinks=2)
         outs.append(out)
     assert torch.equal(*outs)
+
+
+@pytest.mark.parametrize("window", [1 << 30, (1 << 31) - 1])
+def test_the_largest_windows(window):
+    """Rows before their sequence's first key beside a window that no position less it fits 32 bits."""
+    case = kvc.make_case([0, 50], [40, 30], seed=12)
+    d = case.to("cuda")
+    lens = torch.tensor([10, 80], dtype=torch.int32)
+    for sinks in (0, 7, (1 << 31) - 1):
+        out = torch.full((70, 24, 256), 7.0, dtype=torch.float16, device="cuda")
+        pth_dec.forward_window(d.q, d.cache.key_cache, d.cache.value_cache, d.block_table, lens.cuda(), d.scale, d.query_start_loc, out, window,
+                               sinks=sinks)
+        assert bool((out[:30] == 0).all())
+        tail = kvc.DecodeCase(case.q[30:], case.cache, case.block_table, lens, torch.tensor([0, 10, 40], dtype=torch.int32), [0, 50], [10, 30],
+                              24, case.scale)
+        ref, _, _ = window_oracle.windowed(tail, -1, 0)
+        assert kvc.fp16_output_errors(out[30:].double().cpu().numpy(), ref)[2] <= 0
 
 
 def test_no_tokens_and_views_with_gaps():
