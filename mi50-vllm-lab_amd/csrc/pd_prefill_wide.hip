@@ -700,6 +700,12 @@ __device__ __forceinline__ void wide_workgroup(const FaParams& a, const FaWindow
         for (int s = 0; s < min(nsteps, kFwAhead); ++s) issue_next(s);
         if constexpr (kWindow) load_q();
         const int ntl = t1 - t0;
+        // Where the loop lies matters, because one wave per SIMD hides no instruction fetch, of 32 bytes each: the same loop at eight
+        // places, 4 bytes apart, takes 3.65 to 3.75 ms for 2,560 tokens over 61,440 keys with
+        // fp16 rows (4.68 to 4.79 exact), 782 to 792 us for 8,192 tokens with a window of 4,096, 118.5 to 122 for 512 of them split in two.
+        // So it is placed, at what was best for each form. The padding runs once.
+        constexpr int kPlace = kSplit ? 1 : kExact && !kWindow ? 3 : 4;
+        asm volatile(".p2align 5\n\t.rept %0\n\ts_nop 0\n\t.endr" ::"n"(kPlace));
 #pragma unroll 1
         for (int i = 0; i < ntl; ++i) {
             const int s = i / kFwStep;
