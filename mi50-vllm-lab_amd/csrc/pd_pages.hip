@@ -18,7 +18,10 @@
 // words and population counts: no list of free pages is built, and tables, counts and copies run in one launch.
 // The masks also hold the counts as they were, so refs may be updated in place.
 //
-// What bounds it: see the figures at each kernel.
+// What bounds it: small calls their two launches. A step of 48 rows of 1,876 columns takes 3.1 us for masks and plan and 4.9 for the
+// tables, each a few trips to memory that wait for one another. Large calls move pages: 64 rows that each copy a part-filled page in 16
+// layers 2.9 + 7.8 us for 25 MB; a pool of 6,144 pages of 33,280 bytes, 55 % used, in 8 layers 4.8 + 177 us for 807 MB, 4.56 TB/s, where
+// a 4 GiB copy reaches 4.72.
 #include "pd_tile.hpp"
 #include "pth_dec.h"
 
@@ -153,6 +156,8 @@ __device__ __forceinline__ void count_chunk(const PageWork& w, const int* refs, 
     }
 }
 
+// First launch of a compaction: a chunk of the counts per workgroup, 64 pages a wave and step: a launch and one trip to memory,
+// 2.6 to 4.8 us.
 __global__ void __launch_bounds__(kPgThreads) pd_pages_count_kernel(const PageWork w, const int* refs) {
     __shared__ unsigned part[kPgThreads / 64];
     count_chunk(w, refs, nullptr, (int)blockIdx.x, part);
