@@ -231,13 +231,27 @@ __device__ __forceinline__ FwItem fw_item(const FaWindow& w, const int* seq_lens
     }
 }
 // The place of workgroup `lin` of `count` in the order of the work: the 8 XCDs, which the hardware deals workgroups to in turn, take 32
-// neighbours (one per CU) each, in turn as well, so that what runs at once on an XCD shares an L2's keys, and no XCD
-// gets only the long or only the short ones; the rest of less than 256 goes to them in equal runs.
+// neighbours (one per CU) each, in turn as well, so that what runs at once on an XCD shares an L2's keys; the rest of less than 256
+// goes to them in equal runs.
 __device__ __forceinline__ unsigned fw_order(unsigned lin, unsigned count) {
     const unsigned xcd = lin % 8u, whole = count / 256u * 256u;
     if (lin < whole) return lin / 256u * 256u + xcd * 32u + lin / 8u % 32u;
     const unsigned rest = count - whole;
     return whole + xcd * (rest / 8u) + min(xcd, rest % 8u) + (lin - whole) / 8u;
+}
+
+// The order of the work of `total` query tiles with `each` jobs (kv heads and splits) of every one: runs of 32 query tiles, the last tiles first
+// (those of a fresh prompt see the most keys), and in a run job by job. With fewer than 8 jobs a run is as many times longer as fills the 8
+// XCDs, and those that share a job take its tiles by turns, so that none gets only the long or the short ones: 8,192 fresh tokens over a window
+// of 4,096 take 628 us so and 683 where each takes 32 neighbours, 4,096 of them 248 and 268, 4 chunks of 2,048 257 and 282.
+struct FwJob {
+    unsigned tile, job;
+};
+__device__ __forceinline__ FwJob fw_job(unsigned at, unsigned total, unsigned each) {
+    const unsigned sharers = each < 8u ? 8u / each : 1u, most = 32u * sharers;
+    const unsigned run = at / (most * each), width = min(most, total - most * run);
+    const unsigned in = at - run * most * each, job = in / width, pos = in - job * width;
+    return {total - 1 - most * run - (width == most ? pos % 32u * sharers + pos / 32u : pos), job};
 }
 
 // A workgroup of pd_prefill_wide_kernel and, with kWindow, of pd_window_kernel.
@@ -246,16 +260,13 @@ __device__ __forceinline__ void wide_workgroup(const FaParams& a, const FaWindow
     constexpr int kLdsBt = kFwLdsBt, kLdsScr = kFwLdsScr, kRows = 16 * kRB * kFwWaves;
     int x, g, b, qt, split, ntok = a.Sq, first = 0;
     if constexpr (kWindow) {
-        // The order of the work: runs of 32 query tiles, the last tiles first (those of a fresh prompt see the most keys), and for each
-        // run all kv heads and splits.
         const FwTiles tiles = fw_count<kRows>(win, a.seq_lens, a.G);
         const unsigned lin = blockIdx.x + gridDim.x * blockIdx.y, each = gridDim.y * (unsigned)a.nsplit, count = tiles.total * each;
         if (lin >= count) return;
-        const unsigned at = fw_order(lin, count), run = at / (32u * each), width = min(32u, tiles.total - 32u * run);
-        const unsigned in = at - run * 32u * each, job = in / width;
-        x = (int)(tiles.total - 1 - (32u * run + in - job * width));
-        g = (int)(job / (unsigned)a.nsplit);
-        split = (int)(job - (unsigned)g * (unsigned)a.nsplit);
+        const FwJob mine = fw_job(fw_order(lin, count), tiles.total, each);
+        x = (int)mine.tile;
+        g = (int)(mine.job / (unsigned)a.nsplit);
+        split = (int)(mine.job - (unsigned)g * (unsigned)a.nsplit);
         const FwItem item = fw_item<kRows>(win, a.seq_lens, a.G, tiles, (unsigned)x);
         b = item.b, qt = item.tile, ntok = item.ntok, first = item.first;
     } else {
@@ -814,8 +825,8 @@ __global__ void __launch_bounds__(kFwWaves * 64, 1) pd_prefill_wide_kernel(const
 // Q and stores, but each conversion then serves half the products). Tiles at the window's two ends and the last of the sinks are masked row by row, the others
 // are not. Several sequences' rows lie one after the other; which a workgroup has is looked up on the device, so that a captured
 // launch takes any batch of as many rows and sequences.
-// What bounds it: for long chunks the tile loop, as in pd_prefill_wide_kernel: 8,192 tokens of 24 / 4 heads over a window of 4,096 703 us
-// (619 GFLOP, 880 TFLOP/s; behind 30,000 keys, where every row sees a whole window, 785 us and 1,050), 2,048 tokens over windows of 512 / 1,024 /
+// What bounds it: for long chunks the tile loop, as in pd_prefill_wide_kernel: 8,192 tokens of 24 / 4 heads over a window of 4,096 620 to 640 us
+// (619 GFLOP, 980 TFLOP/s; behind 30,000 keys, where every row sees a whole window, 785 us and 1,050), 2,048 tokens over windows of 512 / 1,024 /
 // 2,048 / 4,096 / 8,192 57 / 87 / 146 / 267 / 507. A workgroup's fixed part is about 12 us: block table, first copies, Q and stores. Short
 // chunks pay it once and the merge: 64 tokens over 2,048 keys 31 us.
 template <bool kFast, bool kExact, bool kSplit, int kRB>

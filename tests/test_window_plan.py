@@ -26,20 +26,34 @@ def order(lin, count):
     return whole + xcd * (rest // 8) + min(xcd, rest % 8) + (lin - whole) // 8
 
 
-@pytest.mark.parametrize("hkv,nsplit", [(1, 1), (4, 1), (2, 3), (4, 16)])
+def job_of(at, total, each):
+    sharers = 8 // each if each < 8 else 1
+    most = 32 * sharers
+    run = at // (most * each)
+    width = min(most, total - most * run)
+    job, pos = divmod(at - run * most * each, width)
+    return total - 1 - most * run - (pos % 32 * sharers + pos // 32 if width == most else pos), job
+
+
+@pytest.mark.parametrize("hkv,nsplit", [(1, 1), (4, 1), (2, 3), (4, 16), (3, 1), (5, 1), (2, 1)])
 def test_every_workgroup_has_work_of_its_own(hkv, nsplit):
-    for total in (1, 2, 7, 31, 32, 33, 64, 65, 192, 193, 300):
+    for total in (1, 2, 7, 31, 32, 33, 64, 65, 127, 128, 129, 192, 193, 256, 257, 300):
         each = hkv * nsplit
         count, seen = total * each, set()
         for lin in range(count):
-            at = order(lin, count)
-            run = at // (32 * each)
-            width = min(32, total - 32 * run)
-            inside = at - run * 32 * each
-            job = inside // width
-            x = total - 1 - (32 * run + inside - job * width)
+            x, job = job_of(order(lin, count), total, each)
             seen.add((x, job // nsplit, job % nsplit))
         assert len(seen) == count and all(0 <= x < total and 0 <= g < hkv for x, g, _ in seen)
+
+
+@pytest.mark.parametrize("hkv", [1, 2, 4, 8])
+def test_no_xcd_has_more_of_a_fresh_prompt(hkv):
+    """A prompt's tiles grow with their number: in whole rounds of 256 workgroups the XCDs get the same sum but for a tile's step."""
+    total = 768 // hkv
+    work = [0] * 8
+    for lin in range(total * hkv):
+        work[lin % 8] += job_of(order(lin, total * hkv), total, hkv)[0]
+    assert max(work) - min(work) <= 8 * 96
 
 
 @pytest.mark.parametrize("group", [1, 6, 200])
