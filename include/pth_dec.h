@@ -422,7 +422,7 @@ int pth_cache_write_norm_rotary(const pd_tensor* query, const pd_tensor* query_o
  *                themselves
  *   needed       int32 [1], written: the pages wanted. Where more than were free, the last columns that wanted one are -1
  *   grow, sinks  >= 0; window <= 0: none
- * At most 8,192 rows in either table.
+ * At most 8,192 rows in either table and 2^31 - 1 entries in the new one; new_refs of a page that is free is 0.
  *
  * pth_cache_compact_pages: of n used pages, those numbered n or above move, in order, into the free ones below n, for all caches.
  *   new_refs, new_block_table   as above, each the old one or apart from it; an entry that names no used page becomes -1

@@ -1163,6 +1163,8 @@ int pth_cache_fork_pages(const pd_tensor* caches, int64_t layers, const pd_tenso
           new_block_table->sizes[1] == block_table->sizes[1]))
         return fail(err, errlen, "block tables must be int32 of at most 8192 rows, with the same columns");
     const int64_t B = block_table->sizes[0], N = new_block_table->sizes[0];
+    // (the pages that all rows want are counted in 32 bits)
+    if (N * new_block_table->sizes[1] > INT32_MAX) return fail(err, errlen, "at most 2^31 - 1 entries in the new block table");
     if (!(int_rows(seq_lens, B) && int_rows(new_seq_lens, N))) return fail(err, errlen, "sequence lengths must be contiguous int32 with an entry for each row");
     if (parents ? !int_rows(parents, N) : N != B)
         return fail(err, errlen, "parents must be contiguous int32 with an entry for each new row (none: as many new rows as old)");

@@ -131,7 +131,8 @@ __device__ __forceinline__ unsigned rank_free(const PageWork& w, const unsigned*
 }
 __device__ __forceinline__ bool mask_bit(const word_t* mask, int page) { return (mask[page >> 6] >> (page & 63)) & 1; }
 
-// One chunk's masks and count; the counts also go to new_refs where that is another array (fork).
+// One chunk's masks and count; a fork's counts also go to new_refs, where that is another array or they are below 0 (as 0: the page
+// may be taken, and is counted from there).
 __device__ __forceinline__ void count_chunk(const PageWork& w, const int* refs, int* new_refs, int chunk, unsigned* part) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     unsigned n = 0;
@@ -139,7 +140,7 @@ __device__ __forceinline__ void count_chunk(const PageWork& w, const int* refs, 
     for (int j = 0; j < kPgChunk / kPgThreads; ++j) {
         const int word = wave * (kPgChunk / kPgThreads) + j, page = chunk * kPgChunk + word * 64 + lane;
         const int r = page < w.pages ? refs[page] : 2;  // (past the last page neither free nor alone)
-        if (page < w.pages && new_refs && new_refs != refs) new_refs[page] = r;
+        if (page < w.pages && new_refs && (new_refs != refs || r < 0)) new_refs[page] = max(r, 0);
         const word_t free = __ballot(r <= 0), alone = __ballot(r == 1);
         if (lane == 0) {
             w.free_mask[(int64_t)chunk * kPgWords + word] = free;

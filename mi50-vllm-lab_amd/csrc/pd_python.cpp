@@ -513,7 +513,7 @@ PyObject* fork_pages(PyObject*, PyObject* const* a, Py_ssize_t n) {
     return guarded([&]() -> PyObject* {
         decltype(&pth_cache_fork_pages) fn;
         decltype(&pth_cache_pages_workspace) need;
-        pd_tensor t[8], wd;
+        pd_tensor t[8]{}, wd;
         std::vector<pd_tensor> caches;
         int64_t v[3];
         if (!count_is(n, 14) || !entry(a[0], fn) || !entry(a[1], need)) return nullptr;
@@ -540,7 +540,7 @@ PyObject* compact_pages(PyObject*, PyObject* const* a, Py_ssize_t n) {
     return guarded([&]() -> PyObject* {
         decltype(&pth_cache_compact_pages) fn;
         decltype(&pth_cache_pages_workspace) need;
-        pd_tensor t[6], wd;
+        pd_tensor t[6]{}, wd;
         std::vector<pd_tensor> caches;
         if (!count_is(n, 9) || !entry(a[0], fn) || !entry(a[1], need) || !describe_all(a + 3, t, 6) || !same_gpu(a + 3, 6) ||
             !take_caches(a[2], a[3], caches))

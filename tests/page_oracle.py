@@ -5,7 +5,7 @@ def fork(refs, table, lens, parents, columns, block_size, grow=0, window=-1, sin
     """(new table, new lengths, new counts, pages wanted, copies [(from, to, keys)])."""
     pages = len(refs)
     free = [p for p in range(pages) if refs[p] <= 0]
-    counts, out, sizes, copies, wanted, met = list(refs), [], [], [], 0, set()
+    counts, out, sizes, copies, wanted, met = [max(0, r) for r in refs], [], [], [], 0, set()
     names = lambda e: 0 <= e < pages  # noqa: E731
     for row in table:
         for e in row:

@@ -106,6 +106,17 @@ def test_fork_of_random_pools(seed):
     check_fork(caches, refs, table, lens, parents, cols, bs, grow, window, sinks, in_place=parents is None and rng.random() < 0.5)
 
 
+@pytest.mark.parametrize("in_place", [False, True])
+def test_counts_below_zero_are_free_pages(in_place):
+    """A page that is taken is counted from 0, whatever said that it was free, and no second call takes it again."""
+    refs, table, lens = [-3, 1, -1, 0, -2 ** 31, 1, -2], [[1, -1, -1], [5, -1, -1]], [16, 20]
+    caches = raw_caches(1, 7, 2, 16, "HND", 3)
+    new_table, new_lens, counts, wanted, _ = check_fork(caches, refs, table, lens, None, 3, 16, grow=1, in_place=in_place)
+    assert counts == [1, 1, 1, 0, 0, 1, 0] and wanted == 2
+    again = check_fork(caches, counts, new_table, [32, 32], None, 3, 16, grow=1, in_place=in_place)
+    assert sorted(e for row in again[0] for e in row if e >= 0) == [0, 1, 2, 3, 4, 5]
+
+
 def test_fork_takes_thousands_of_pages():
     """Rows that take more pages than a workgroup has threads, across many counts of 1,024."""
     rng = random.Random(1)

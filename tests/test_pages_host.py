@@ -160,6 +160,12 @@ def test_pools_and_rows_beyond_the_limits(lib):
     assert w(1, 0, 0) == 66 and w(1025, 3, 5) == 2 * 65 + 3 + 20 + 1
 
 
+def test_more_entries_than_32_bits_count(lib):
+    cols = 2 ** 30 - 1
+    table = lambda rows: strided((rows, cols), (cols, 1), pth_dec.PD_DTYPE_INT32)  # noqa: E731
+    assert call_fork(lib, table=table(3), new_table=table(5)) == (1, "at most 2^31 - 1 entries in the new block table")
+
+
 def test_norm_rotary_refusals(lib):
     c = kvc.make_case([37, 5], [3, 1], num_q_heads=12, num_kv_heads=2, block_size=16, seed=3).cache
     x = torch.zeros((3, 17, 256), dtype=torch.float16)
