@@ -839,20 +839,30 @@ __global__ void __launch_bounds__(kFwWaves * 64, 1) pd_window_kernel(const FaPar
 // out = sum_s 2^(m_s - M) O_s / sum_s 2^(m_s - M) l_s, 0 for a row that saw no key. Rows outside the sequences, and those of
 // sequences without keys, are left alone.
 __global__ void __launch_bounds__(256) pd_window_combine_kernel(const FaParams a, const FaWindow win) {
-    constexpr int kBatch = 8;
+    constexpr int kBatch = 16;
     const int lane = threadIdx.x & 63, head = (int)blockIdx.y;
     const int tok = (int)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
     if (tok >= win.num_tokens) return;
+    const int64_t base = ((int64_t)tok * a.Hq + head) * a.nsplit;
+    // All that the row needs is asked for at once, one trip to memory for up to kBatch splits. (What a row that nobody owns reads lies in
+    // the workspace too, whatever it holds.)
+    const float4_t* po = reinterpret_cast<const float4_t*>(a.part_o + base * kDim) + lane;
+    const float m_mine = lane < a.nsplit ? a.part_m[base + lane] : kNegInf;
+    const float l_mine = lane < a.nsplit ? a.part_l[base + lane] : 0.f;
+    float4_t o[kBatch];
+    auto load = [&](int s0) __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i)
+            if (s0 + i < a.nsplit) o[i] = po[(int64_t)(s0 + i) * (kDim / 4)];
+    };
+    load(0);
     bool mine = false;
     for (int c = 0; c < win.num_seqs; c += 64) {
         const int i = min(c + lane, win.num_seqs - 1);
-        const int first = win.query_start[i], end = win.query_start[i + 1];
-        mine = mine || (tok >= first && tok < end && a.seq_lens[i] > 0);
+        const int first = win.query_start[i], end = win.query_start[i + 1], len = a.seq_lens[i];
+        mine = mine | ((tok >= first) & (tok < end) & (len > 0));
     }
     if (__ballot(mine) == 0) return;
-    const int64_t base = ((int64_t)tok * a.Hq + head) * a.nsplit;
-    const float m_mine = lane < a.nsplit ? a.part_m[base + lane] : kNegInf;
-    const float l_mine = lane < a.nsplit ? a.part_l[base + lane] : 0.f;
     float M = m_mine;
 #pragma unroll
     for (int o = 32; o >= 1; o >>= 1) M = fmaxf(M, __shfl_xor(M, o, 64));
@@ -861,15 +871,13 @@ __global__ void __launch_bounds__(256) pd_window_combine_kernel(const FaParams a
 #pragma unroll
     for (int o = 32; o >= 1; o >>= 1) L += __shfl_xor(L, o, 64);
     float4_t acc = (float4_t)0.f;
-    const float4_t* po = reinterpret_cast<const float4_t*>(a.part_o + base * kDim) + lane;
     for (int s0 = 0; s0 < a.nsplit; s0 += kBatch) {
-        float4_t o[kBatch];
-#pragma unroll
-        for (int i = 0; i < kBatch; ++i) o[i] = s0 + i < a.nsplit ? po[(int64_t)(s0 + i) * (kDim / 4)] : (float4_t)0.f;
+        if (s0 > 0) load(s0);
 #pragma unroll
         for (int i = 0; i < kBatch; ++i) {
-            const float wi = __shfl(w_mine, min(s0 + i, 63), 64);
-            acc += (s0 + i < a.nsplit && wi != 0.f) ? wi * o[i] : (float4_t)0.f;
+            if (s0 + i >= a.nsplit) break;
+            const float wi = __shfl(w_mine, s0 + i, 64);
+            acc += wi != 0.f ? wi * o[i] : (float4_t)0.f;
         }
     }
     const float inv = L > 0.f ? 1.f / L : 0.f;
