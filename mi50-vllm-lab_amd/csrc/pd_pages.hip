@@ -20,8 +20,8 @@
 //
 // What bounds it: small calls their two launches. A step of 48 rows of 1,876 columns takes 3.1 us for masks and plan and 4.9 for the
 // tables, each a few trips to memory that wait for one another. Large calls move pages: 64 rows that each copy a part-filled page in 16
-// layers 2.9 + 7.8 us for 25 MB; a pool of 6,144 pages of 33,280 bytes, 55 % used, in 8 layers 4.8 + 177 us for 807 MB, 4.56 TB/s, where
-// a 4 GiB copy reaches 4.72.
+// layers 2.9 + 7.8 us for 25 MB; a pool of 6,144 pages of 33,280 bytes, 55 % used, in 8 layers 4.7 + 170 us for 807 MB, 4.7 TB/s, the
+// rate of a 4 GiB copy.
 #include "pd_tile.hpp"
 #include "pth_dec.h"
 
