@@ -827,7 +827,8 @@ __global__ void __launch_bounds__(kFwWaves * 64, 1) pd_prefill_wide_kernel(const
 // launch takes any batch of as many rows and sequences.
 // What bounds it: for long chunks the tile loop, as in pd_prefill_wide_kernel: 8,192 tokens of 24 / 4 heads over a window of 4,096 620 to 640 us
 // (619 GFLOP, 980 TFLOP/s; behind 30,000 keys, where every row sees a whole window, 785 us and 1,050), 2,048 tokens over windows of 512 / 1,024 /
-// 2,048 / 4,096 / 8,192 57 / 87 / 146 / 267 / 507. A workgroup's fixed part is about 12 us: block table, first copies, Q and stores. Short
+// 2,048 / 4,096 / 8,192 57 / 86 / 144 / 262 / 460; kExact, which takes both halves of the weights through P.V, 791 us and 67 / 104 / 179 / 330 / 572.
+// A workgroup's fixed part is about 12 us: block table, first copies, Q and stores. Short
 // chunks pay it once and the merge: 64 tokens over 2,048 keys 31 us.
 template <bool kFast, bool kExact, bool kSplit, int kRB>
 __global__ void __launch_bounds__(kFwWaves * 64, 1) pd_window_kernel(const FaParams a, const FaWindow win) {

@@ -29,7 +29,8 @@ few fields the routing reads.
   to 32 suffix sequences run in one launch on the query and output rows as they are (forward_rows),
   others each through the prefill operator (no padding to a tile ladder is needed);
   VLLM_GFX950_PTH_FA_EXACT=1 selects its exact entry (pth_fa_forward_exact: the decode's
-  numerics, for caches with very large per-token scales, at ~26 % more time).
+  numerics, for caches with very large per-token scales, at ~26 % more time). Windowed prefill has the decode's numerics
+  unless the variable is set to 0.
 - route (triton_attn.patch:272-308): prefill first when max_seqlen_q >= MIN_Q, then decode
   when max_seqlen_q <= MAX_Q; causal only, no multimodal prefix, no RSWA prefix, no output
   scale. Returns False when the caller must run its own path.
@@ -54,6 +55,7 @@ PTH_DEC_MAX_Q = int(os.environ.get("VLLM_GFX950_PTH_DEC_MAX_Q", "4"))
 PTH_DEC_SPLITS = int(os.environ.get("VLLM_GFX950_PTH_DEC_SPLITS", "64"))
 PTH_DEC_CUS = int(os.environ.get("VLLM_GFX950_PTH_DEC_CUS", "0"))  # 0: the device's CU count
 PTH_FA_EXACT = os.environ.get("VLLM_GFX950_PTH_FA_EXACT", "0") == "1"  # prefill through pth_fa_forward_exact
+PTH_WINDOW_EXACT = os.environ.get("VLLM_GFX950_PTH_FA_EXACT", "1") == "1"  # windowed prefill: decode's numerics unless it is set otherwise
 MAX_ROWS_PER_KV_HEAD = 48  # qmax * G the decode operator takes
 MAX_GROUP_WINDOW = 256     # G that forward_window takes
 # decode_shared against decode over 461 batches (24 / 4, 12 / 2 and 32 / 8 heads, 1, 2 and 4 query tokens, 2 to 512 sequences, 64 to
@@ -375,7 +377,7 @@ class Gfx950Int8Attention:
             # (sized by the window, and the rows are found on the device: nothing here depends on the lengths)
             self.pth_fa_window.forward_window(query[:qsl[n]], key_cache, value_cache, meta.block_table[p:n], meta.seq_lens[p:n],
                                               self.scale, meta.query_start_loc[p:n + 1], output[:qsl[n]], self.window,
-                                              sinks=self.sink_tokens, exact=PTH_FA_EXACT)
+                                              sinks=self.sink_tokens, **({} if PTH_WINDOW_EXACT else {"exact": False}))
             return True
         # A launch is planned for the keys that its sequences see: the host lengths when they are known and
         # no graph is being captured (vLLM's block table is as wide as the model's maximum length, so the table
