@@ -12,8 +12,10 @@ few fields the routing reads.
   sliding window. Decode accepts a left sliding window (the operator implements the window
   rule) and any GQA group with qmax * G <= 48, where the reference required GQA 6 and no window.
   Layers with a left window whose fp16 rows the operator takes have their prefill in forward_window (not in the reference, which
-  leaves it to Triton); sink_tokens first keys then stay visible to all rows, in decode as well. (`sinks` are vLLM's learned
-  per-head logits, another thing, which no operator here takes.)
+  leaves it to Triton); sink_tokens first keys then stay visible to all rows, in decode as well. The caller's own path knows nothing of
+  them, so a layer with sink_tokens never falls back: rows that decode does not take, of any number, type and strides, go through
+  forward_window, and what that cannot take either raises. (`sinks` are vLLM's learned per-head logits, another thing, which no
+  operator here takes.)
 - forward_pth_dec (triton_attn.patch:116-174): the cache layout is checked once; the call falls
   back (returns False) without the softmax segment buffers, with more query tokens than segment
   rows, or with query / output strides the operator does not take. nsplit = min(splits,
@@ -304,6 +306,7 @@ class Gfx950Int8Attention:
                   and alibi_slopes is None and not logits_soft_cap and chunk_lookback == -1 and not use_td
                   and on_gfx950)
         if not common:
+            self._no_fallback_for_sinks()
             return
         if self.window < 0 and sliding_window[1] < 0:
             self.pth_fa = load_pth_fa()
@@ -311,8 +314,17 @@ class Gfx950Int8Attention:
         if self.window > 0 and sliding_window[1] <= 0 and num_heads % max(num_kv_heads, 1) == 0 and 1 <= G <= MAX_GROUP_WINDOW:
             fa = load_pth_fa()
             self.pth_fa_window = fa if hasattr(fa, "forward_window") else None
-        if num_heads % max(num_kv_heads, 1) == 0 and 1 <= max_q * G <= MAX_ROWS_PER_KV_HEAD and sliding_window[1] < 0:
+        self._no_fallback_for_sinks()
+        # (a right bound of 0 is causal decode's own rule; without sink tokens such layers' decode stays with the caller)
+        if num_heads % max(num_kv_heads, 1) == 0 and 1 <= max_q * G <= MAX_ROWS_PER_KV_HEAD and (
+                sliding_window[1] < 0 or (self.sink_tokens and sliding_window[1] == 0)):
             self.pth_dec = load_pth_dec()
+
+    def _no_fallback_for_sinks(self) -> None:
+        if self.sink_tokens and self.pth_fa_window is None:
+            raise RuntimeError("gfx950: sink_tokens needs forward_window: causal int8 per-token-head attention with a left window, heads of "
+                               "256, at most 256 query heads per kv head, and the prefill operator loaded; the caller's own path knows no sink "
+                               "tokens")
 
     # -------------------------------------------------------------------------------------
     def forward_pth_dec(self, query, key_cache, value_cache, k_scale_cache, v_scale_cache, block_table, seq_lens,
@@ -364,7 +376,7 @@ class Gfx950Int8Attention:
             p -= 1
         if p == n or (self.pth_fa is None and not self._window_takes(query, key_cache, value_cache, k_scale_cache, v_scale_cache,
                                                                      output, qsl[n])):
-            return False
+            return False  # (with sink tokens route() then gives forward_window the whole batch)
         max_q_prefix = max((qsl[i + 1] - qsl[i] for i in range(p)), default=0)
         if p > 0 and not (
             self.pth_dec is not None and max_q_prefix <= self.max_q
@@ -372,7 +384,10 @@ class Gfx950Int8Attention:
                                      meta.block_table[:p], meta.seq_lens[:p], meta.query_start_loc[:p + 1],
                                      output[:qsl[p]], max_q_prefix, meta,
                                      None if meta.seq_lens_cpu is None else meta.seq_lens_cpu[:p])):
-            triton_fallback(0, qsl[p], 0, p, max_q_prefix)
+            if self.sink_tokens:
+                p = 0  # forward_window takes these rows as well
+            else:
+                triton_fallback(0, qsl[p], 0, p, max_q_prefix)
         if self.pth_fa is None:
             # (sized by the window, and the rows are found on the device: nothing here depends on the lengths)
             self.pth_fa_window.forward_window(query[:qsl[n]], key_cache, value_cache, meta.block_table[p:n], meta.seq_lens[p:n],
@@ -417,6 +432,25 @@ class Gfx950Int8Attention:
                     and output.stride(2) == 1 and query.stride(0) % 8 == 0 and query.stride(1) % 8 == 0 and query.data_ptr() % 16 == 0
                     and output.stride(0) % 4 == 0 and output.stride(1) % 4 == 0 and output.data_ptr() % 8 == 0)
 
+    def _window_all(self, query, key_cache, value_cache, k_scale_cache, v_scale_cache, meta: AttnMeta, output) -> None:
+        """The whole batch through forward_window, whatever its rows: those that it does not read and write as they are as fp16 copies."""
+        def takes(q, o):
+            return self._window_takes(q, key_cache, value_cache, k_scale_cache, v_scale_cache, o, q.shape[0])
+
+        q, out, n = query, output, meta.seq_lens.shape[0]
+        if not takes(q, out):
+            q, out = query.to(torch.float16).contiguous(), torch.zeros(output.shape, dtype=torch.float16, device=output.device)
+            if not takes(q, out):
+                raise RuntimeError("gfx950: sink_tokens, and neither operator takes these rows or this KV cache layout: query and output "
+                                   "[tokens, heads, 256] over int8 per-token-head rows")
+        starts = meta.query_start_loc[:n + 1]
+        self.pth_fa_window.forward_window(q, key_cache, value_cache, meta.block_table[:n], meta.seq_lens, self.scale, starts, out,
+                                          self.window, sinks=self.sink_tokens, **({} if PTH_WINDOW_EXACT else {"exact": False}))
+        if out is not output:  # rows of no sequence, or of one without keys, are left as they were
+            at = torch.searchsorted(starts, torch.arange(q.shape[0], dtype=starts.dtype, device=starts.device), right=True) - 1
+            written = (at >= 0) & (at < n) & (meta.seq_lens[at.clamp(0, n - 1)] > 0)
+            output.copy_(torch.where(written[:, None, None], out.to(output.dtype), output))
+
     # -------------------------------------------------------------------------------------
     def route(self, query, key_cache, value_cache, k_scale_cache, v_scale_cache, meta: AttnMeta, output,
               max_seqlen_q: int, num_actual_tokens: int, triton_fallback: Callable[..., None],
@@ -424,13 +458,20 @@ class Gfx950Int8Attention:
         """The forward() glue: True when one of the operators handled the batch."""
         plain = (meta.causal is True and meta.mm_prefix_range_tensor is None and meta.rswa_prefix_lens is None
                  and output_scale is None)
+        if self.sink_tokens and not plain:
+            raise RuntimeError("gfx950: sink_tokens with non-causal rows, a multimodal or RSWA prefix or a scaled output, which no operator takes")
         if ((self.pth_fa is not None or self.pth_fa_window is not None) and max_seqlen_q >= PTH_FA_MIN_Q and plain
                 and self.forward_pth_fa(query, key_cache, value_cache, k_scale_cache, v_scale_cache, meta, output,
                                         triton_fallback)):
             return True
-        if (self.pth_dec is not None and max_seqlen_q <= self.max_q and plain
+        fp16 = query.dtype == torch.float16 and output.dtype == torch.float16
+        if (self.pth_dec is not None and max_seqlen_q <= self.max_q and plain and (fp16 or not self.sink_tokens)
                 and self.forward_pth_dec(query[:num_actual_tokens], key_cache, value_cache, k_scale_cache,
                                          v_scale_cache, meta.block_table, meta.seq_lens, meta.query_start_loc,
                                          output[:num_actual_tokens], max_seqlen_q, meta, meta.seq_lens_cpu)):
+            return True
+        if self.sink_tokens:
+            self._window_all(query[:num_actual_tokens], key_cache, value_cache, k_scale_cache, v_scale_cache, meta,
+                             output[:num_actual_tokens])
             return True
         return False
