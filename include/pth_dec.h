@@ -283,7 +283,8 @@ int64_t pth_fa_balanced_workspace(int64_t num_seqs, const int* query_start, int6
 
 /*
  * Causal chunked prefill of rows that see a sliding window and a few first keys. No counterpart in the reference.
- *   q, out       fp16 [T, Hq, 256], unit dim stride, rows of q 16-byte and of out 8-byte aligned; they must not overlap
+ *   q, out       fp16 [T, Hq, 256], unit dim stride, rows of q 16-byte and of out 8-byte aligned; out and the workspace
+ *                must not overlap each other, q, the cache or the tables
  *   query_start_loc  int32 [>= num_seqs + 1], device: sequence i has rows [query_start_loc[i], query_start_loc[i + 1]) of q and out, the last
  *                tokens of its seq_lens[i] keys (block_table and seq_lens have a row per sequence). Rows outside the sequences, and of
  *                sequences of no keys, are left alone

@@ -566,6 +566,10 @@ static int fa_forward_rows(const pd_tensor* q, const pd_tensor* kc, const pd_ten
     return fa_result(launch_prefill_balanced(p, r, (int)Hkv, q->dtype, stream, exact), err, errlen);
 }
 
+static bool window_tensors_apart(const pd_tensor* q, const pd_tensor* kc, const pd_tensor* block_table, const pd_tensor* seq_lens,
+                                 const pd_tensor* query_start, const pd_tensor* out, const pd_tensor* workspace, int64_t num_seqs,
+                                 int64_t ws_floats);
+
 int64_t pth_fa_window_splits(int64_t tokens, int64_t num_seqs, int64_t heads_q, int64_t heads_kv, int64_t window, int64_t sinks,
                              int64_t table_keys, int64_t exact) {
     if (tokens < 1 || tokens > INT32_MAX || num_seqs < 1 || num_seqs > INT32_MAX || heads_kv < 1 || heads_q < heads_kv ||
@@ -620,6 +624,9 @@ int pth_fa_forward_window(const pd_tensor* q, const pd_tensor* key_cache, const 
                         workspace->sizes[0] >= prefill_workspace_floats(1, T, Hq, nsplit) &&
                         reinterpret_cast<uintptr_t>(workspace->data) % 16 == 0))
         return fail(err, errlen, "workspace must be contiguous 16-byte aligned fp32 of T * Hq * nsplit * 258");
+    if (!window_tensors_apart(q, key_cache, block_table, seq_lens, query_start_loc, out, nsplit > 1 ? workspace : nullptr, num_seqs,
+                              prefill_workspace_floats(1, T, Hq, nsplit)))
+        return fail(err, errlen, "out and the workspace must not overlap each other or what the call reads");
     if (T == 0) return 0;
     FaParams p = {};
     p.q = q->data;
@@ -818,6 +825,23 @@ static bool apart(const ByteRows& a, const ByteRows& b) {
         if (gap >= (uint64_t)width(a) && gap + (uint64_t)width(b) <= (uint64_t)s) return true;
     }
     return false;
+}
+
+// What a windowed prefill writes against all that it touches (workspace: null if the call has none).
+static bool window_tensors_apart(const pd_tensor* q, const pd_tensor* kc, const pd_tensor* block_table, const pd_tensor* seq_lens,
+                                 const pd_tensor* query_start, const pd_tensor* out, const pd_tensor* workspace, int64_t num_seqs,
+                                 int64_t ws_floats) {
+    const ByteRows cache = {reinterpret_cast<uintptr_t>(kc->data), {1, 1}, {0, 0}, kc->sizes[0] > 0 ? cache_span(kc) - 8 + kRowBytes : 0};
+    const ByteRows reads[] = {byte_rows(q, q->sizes[0], kDim, 2), cache, byte_span(block_table, num_seqs, 4), byte_span(seq_lens, num_seqs, 4),
+                              byte_span(query_start, num_seqs + 1, 4)};
+    const ByteRows rows = byte_rows(out, out->sizes[0], kDim, 2);
+    for (const ByteRows& r : reads)
+        if (!apart(rows, r)) return false;
+    if (!workspace) return true;
+    const ByteRows ws = byte_span(workspace, ws_floats, 4);
+    for (const ByteRows& r : reads)
+        if (!apart(ws, r)) return false;
+    return apart(rows, ws);
 }
 
 // The norms of a rotary write's query and key heads.
