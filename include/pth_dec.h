@@ -405,7 +405,8 @@ int pth_cache_write_norm_rotary(const pd_tensor* query, const pd_tensor* query_o
 /*
  * Block tables and reference counts on the device. No counterpart in the reference, whose engine keeps them on the host.
  *   caches       `layers` (1..128) raw caches, int8 [pages <= 2^22, Hkv, block_size, 520], of the same sizes and strides, their rows
- *                8-byte aligned and apart; page numbers are those of all of them
+ *                8-byte aligned and apart, also from other caches' and the other tensors (one given twice counts once); page
+ *                numbers are those of all of them
  *   refs         int32 [pages], how many table entries name each page; 0 (or less): the page is free
  *   block_table  int32 [B, columns], an entry outside [0, pages) names no page
  *   workspace    int32, 16-byte aligned, of pth_cache_pages_workspace(pages, B, N) (0, 0 for compact); its contents need not be

@@ -1109,7 +1109,51 @@ static bool cache_rows_apart(const pd_tensor* kv) {
     return true;
 }
 
-// The caches and the table rows that a page operator takes; null, or why not.
+// Bytes from a raw cache's first row to the end of its last.
+static int64_t raw_extent(const pd_tensor* kv) {
+    int64_t n = kRowBytes;
+    for (int d = 0; d < 3; ++d) n += (kv->sizes[d] - 1) * kv->strides[d];
+    return n;
+}
+// Whether rows of two caches of kv's sizes and strides, `d` bytes apart, share a byte: some sum of a[i] strides[i] with |a[i]| < sizes[i] is less
+// than a row from d. By falling strides; below a stride the others reach less far than it (cache_rows_apart), so only the two
+// multiples beside d can.
+static bool rows_meet(const pd_tensor* kv, int64_t d) {
+    int order[3] = {0, 1, 2};
+    std::sort(order, order + 3, [&](int a, int b) { return kv->strides[a] > kv->strides[b]; });
+    int64_t reach[4] = {0, 0, 0, kRowBytes};
+    for (int i = 2; i >= 0; --i) reach[i] = reach[i + 1] + (kv->sizes[order[i]] - 1) * kv->strides[order[i]];
+    int64_t left[8] = {d};
+    int n = 1;
+    for (int i = 0; i < 3; ++i) {
+        const int64_t most = kv->sizes[order[i]] - 1, st = kv->strides[order[i]];
+        int64_t next[8];
+        int m = 0;
+        for (int j = 0; j < n; ++j) {
+            if (most == 0) {
+                if (std::abs(left[j]) < reach[i + 1]) next[m++] = left[j];
+                continue;
+            }
+            const int64_t a = left[j] / st - (left[j] % st < 0);
+            for (int64_t x = a; x <= a + 1; ++x)
+                if (std::abs(x) <= most && std::abs(left[j] - x * st) < reach[i + 1]) next[m++] = left[j] - x * st;
+        }
+        std::copy(next, next + m, left);
+        n = m;
+    }
+    return n > 0;
+}
+// Whether a tensor lies clear of all caches (sorted, `extent` bytes each).
+static bool clear_of_caches(const PageCaches& k, int64_t extent, const ByteRows& r) {
+    if (r.n[0] <= 0 || r.n[1] <= 0 || r.len <= 0) return true;
+    const uintptr_t end = r.at + (uint64_t)((r.n[0] - 1) * r.st[0] + (r.n[1] - 1) * r.st[1] + r.len);
+    // of the caches that begin before its end the last one ends last
+    int8_t* const* past = std::lower_bound(k.kv, k.kv + k.layers, reinterpret_cast<int8_t*>(end));
+    return past == k.kv || reinterpret_cast<uintptr_t>(past[-1]) + (uint64_t)extent <= r.at;
+}
+
+// The caches and the table rows that a page operator takes; null, or why not. A cache that is given twice (layers that share one) is
+// taken once.
 static const char* page_caches(const pd_tensor* caches, int64_t layers, PageCaches& k) {
     if (!(layers >= 1 && layers <= kMaxPageLayers)) return "1 to 128 caches per call";
     for (int64_t i = 0; i < layers; ++i) {
@@ -1129,10 +1173,15 @@ static const char* page_caches(const pd_tensor* caches, int64_t layers, PageCach
           c.sizes[2] <= (1 << 20) && c.sizes[1] * c.sizes[2] <= (1 << 20)))
         return "caches of 1 to 2^22 pages of 1 to 2^20 rows";
     if (!cache_rows_apart(&c)) return "cache rows must not overlap";
+    std::sort(k.kv, k.kv + layers, [](const int8_t* a, const int8_t* b) { return a < b; });
+    k.layers = (int)(std::unique(k.kv, k.kv + layers) - k.kv);
+    const int64_t extent = raw_extent(&c);
+    for (int i = 0; i < k.layers; ++i)
+        for (int j = i + 1; j < k.layers && k.kv[j] - k.kv[i] < extent; ++j)
+            if (rows_meet(&c, k.kv[j] - k.kv[i])) return "the caches' rows must not overlap";
     k.sb = c.strides[0];
     k.sh = c.strides[1];
     k.ss = c.strides[2];
-    k.layers = (int)layers;
     k.Hkv = (int)c.sizes[1];
     k.block_size = (int)c.sizes[2];
     return nullptr;
@@ -1214,6 +1263,11 @@ int pth_cache_fork_pages(const pd_tensor* caches, int64_t layers, const pd_tenso
             if (parents && !apart(outs[i], byte_span(parents, N, 4)))
                 return fail(err, errlen, "the tensors that are written must not overlap those that are read");
         }
+        const int64_t extent = raw_extent(caches);
+        bool clear = !parents || clear_of_caches(k, extent, byte_span(parents, N, 4));
+        for (const ByteRows& r : outs) clear = clear && clear_of_caches(k, extent, r);
+        for (const ByteRows& r : ins) clear = clear && clear_of_caches(k, extent, r);
+        if (!clear) return fail(err, errlen, "the caches must not overlap the other tensors");
     }
     p.refs = static_cast<const int*>(refs->data);
     p.new_refs = static_cast<int*>(const_cast<void*>(new_refs->data));
@@ -1271,6 +1325,11 @@ int pth_cache_compact_pages(const pd_tensor* caches, int64_t layers, const pd_te
             for (int j = 0; j < 2; ++j)
                 if (i != j && !apart(outs[i], ins[j])) return fail(err, errlen, "the tensors that are written must not overlap those that are read");
         }
+        const int64_t extent = raw_extent(caches);
+        bool clear = true;
+        for (const ByteRows& r : outs) clear = clear && clear_of_caches(k, extent, r);
+        for (const ByteRows& r : ins) clear = clear && clear_of_caches(k, extent, r);
+        if (!clear) return fail(err, errlen, "the caches must not overlap the other tensors");
     }
     p.refs = static_cast<const int*>(refs->data);
     p.new_refs = static_cast<int*>(const_cast<void*>(new_refs->data));

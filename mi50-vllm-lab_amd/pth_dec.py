@@ -502,7 +502,7 @@ def fork_pages(caches, refs: torch.Tensor, block_table: torch.Tensor, seq_lens: 
     """The block tables of a serving step from those before it: rows that go on, fork or end, pages taken and given back (no
     counterpart in the reference, whose engine keeps its tables on the host).
 
-    caches: a kvcache.PagedKVCache or its raw `kv` per layer, all of one geometry, the tables' pages; refs int32 [pages]: how many
+    caches: a kvcache.PagedKVCache or its raw `kv` per layer (layers may share one), all of one geometry, the tables' pages; refs int32 [pages]: how many
     table entries name each page (0: free); block_table int32 [B, columns], entries below 0 name no page; seq_lens int32 [B].
     New row i goes on from old row parents[i] (int32 [N]; outside [0, B): an empty row), None: from row i. It shares the parent's full
     pages and gets room for `grow` more keys. A page that still takes keys is its own: the first child keeps the parent's if no
