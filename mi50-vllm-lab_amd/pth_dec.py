@@ -70,6 +70,16 @@ EXPORTED_SYMBOLS = (
     "pth_cache_compact_pages",
     "pth_cache_pages_workspace",
 )
+# Those that a library given by its path may lack: it loads all the same, and what needs them raises.
+LATER_SYMBOLS = (
+    "pth_dec_decode_sinks",
+    "pth_fa_forward_window",
+    "pth_fa_window_splits",
+    "pth_cache_write_norm_rotary",
+    "pth_cache_fork_pages",
+    "pth_cache_compact_pages",
+    "pth_cache_pages_workspace",
+)
 
 
 class PdTensor(ctypes.Structure):
@@ -150,16 +160,10 @@ def load_library(path: str | None = None) -> ctypes.CDLL:
     lib.pth_fa_forward_balanced.restype = c_int
     lib.pth_fa_balanced_workspace.argtypes = [ctypes.c_int64, ip] + [ctypes.c_int64] * 5
     lib.pth_fa_balanced_workspace.restype = ctypes.c_int64
-    lib.pth_fa_forward_window.argtypes = [tp] * 5 + [c_double, tp, tp, tp] + [ctypes.c_int64] * 5 + [vp, ctypes.c_char_p, c_int]
-    lib.pth_fa_forward_window.restype = c_int
-    lib.pth_fa_window_splits.argtypes = [ctypes.c_int64] * 8
-    lib.pth_fa_window_splits.restype = ctypes.c_int64
     lib.pth_cache_write.argtypes = [tp] * 7 + [vp, ctypes.c_char_p, c_int]
     lib.pth_cache_write.restype = c_int
     lib.pth_dec_decode_lse.argtypes = [tp] * 9 + [c_double, tp, tp, tp, tp] + [ctypes.c_int64] * 5 + [vp, ctypes.c_char_p, c_int]
     lib.pth_dec_decode_lse.restype = c_int
-    lib.pth_dec_decode_sinks.argtypes = [tp] * 9 + [c_double, tp, tp, tp, tp] + [ctypes.c_int64] * 6 + [vp, ctypes.c_char_p, c_int]
-    lib.pth_dec_decode_sinks.restype = c_int
     lib.pth_dec_decode_shared.argtypes = [tp] * 9 + [c_double, tp, tp, tp, tp] + [ctypes.c_int64] * 3 + [vp, ctypes.c_char_p, c_int]
     lib.pth_dec_decode_shared.restype = c_int
     lib.pth_cache_write_rotary.argtypes = [tp] * 11 + [ctypes.c_int64, vp, ctypes.c_char_p, c_int]
@@ -168,31 +172,41 @@ def load_library(path: str | None = None) -> ctypes.CDLL:
     lib.pth_cache_key_weights.restype = c_int
     lib.pth_cache_evict.argtypes = [tp] * 11 + [ctypes.c_int64] * 3 + [vp, ctypes.c_char_p, c_int]
     lib.pth_cache_evict.restype = c_int
-    lib.pth_cache_write_norm_rotary.argtypes = [tp] * 6 + [c_double, c_double] + [tp] * 7 + [ctypes.c_int64, vp, ctypes.c_char_p, c_int]
-    lib.pth_cache_write_norm_rotary.restype = c_int
-    lib.pth_cache_fork_pages.argtypes = [tp, ctypes.c_int64] + [tp] * 9 + [ctypes.c_int64] * 3 + [vp, ctypes.c_char_p, c_int]
-    lib.pth_cache_fork_pages.restype = c_int
-    lib.pth_cache_compact_pages.argtypes = [tp, ctypes.c_int64] + [tp] * 7 + [vp, ctypes.c_char_p, c_int]
-    lib.pth_cache_compact_pages.restype = c_int
-    lib.pth_cache_pages_workspace.argtypes = [ctypes.c_int64] * 3
-    lib.pth_cache_pages_workspace.restype = ctypes.c_int64
+    for name, argtypes, restype in (
+            ("pth_dec_decode_sinks", [tp] * 9 + [c_double, tp, tp, tp, tp] + [ctypes.c_int64] * 6 + [vp, ctypes.c_char_p, c_int], c_int),
+            ("pth_fa_forward_window", [tp] * 5 + [c_double, tp, tp, tp] + [ctypes.c_int64] * 5 + [vp, ctypes.c_char_p, c_int], c_int),
+            ("pth_fa_window_splits", [ctypes.c_int64] * 8, ctypes.c_int64),
+            ("pth_cache_write_norm_rotary", [tp] * 6 + [c_double, c_double] + [tp] * 7 + [ctypes.c_int64, vp, ctypes.c_char_p, c_int], c_int),
+            ("pth_cache_fork_pages", [tp, ctypes.c_int64] + [tp] * 9 + [ctypes.c_int64] * 3 + [vp, ctypes.c_char_p, c_int], c_int),
+            ("pth_cache_compact_pages", [tp, ctypes.c_int64] + [tp] * 7 + [vp, ctypes.c_char_p, c_int], c_int),
+            ("pth_cache_pages_workspace", [ctypes.c_int64] * 3, ctypes.c_int64),
+    ):
+        if hasattr(lib, name):
+            getattr(lib, name).argtypes, getattr(lib, name).restype = argtypes, restype
     lib.pth_dec_version.argtypes = []
     lib.pth_dec_version.restype = ctypes.c_char_p
-    _entries.update({name: ctypes.cast(getattr(lib, name), vp).value
-                     for name in ("pth_dec_decode", "pth_fa_forward", "pth_fa_forward_exact", "pth_fa_forward_split",
-                                  "pth_fa_forward_balanced", "pth_fa_balanced_workspace", "pth_fa_forward_window",
-                                  "pth_fa_window_splits", "pth_cache_write", "pth_dec_decode_lse",
-                                  "pth_dec_decode_sinks", "pth_dec_decode_shared", "pth_cache_write_rotary", "pth_cache_key_weights", "pth_cache_evict",
-                                  "pth_cache_write_norm_rotary", "pth_cache_fork_pages", "pth_cache_compact_pages",
-                                  "pth_cache_pages_workspace")})
+    entries = {name: ctypes.cast(getattr(lib, name), vp).value
+               for name in ("pth_dec_decode", "pth_fa_forward", "pth_fa_forward_exact", "pth_fa_forward_split",
+                            "pth_fa_forward_balanced", "pth_fa_balanced_workspace", "pth_cache_write", "pth_dec_decode_lse",
+                            "pth_dec_decode_shared", "pth_cache_write_rotary", "pth_cache_key_weights", "pth_cache_evict", *LATER_SYMBOLS)
+               if name not in LATER_SYMBOLS or hasattr(lib, name)}
+    _entries.clear()
+    _entries.update(entries)
     _lib, _lib_path = lib, os.path.realpath(p)
     return lib
 
 
-def _entry(name: str) -> int:
-    """Address of an operator entry of the active library (loaded if none is)."""
+def provides(name: str) -> bool:
+    """Whether the active library (loaded if none is) has an operator entry; one built from older sources may lack LATER_SYMBOLS."""
     if _lib is None:
         load_library()
+    return name in _entries
+
+
+def _entry(name: str) -> int:
+    """Address of an operator entry of the active library (loaded if none is)."""
+    if not provides(name):
+        raise RuntimeError(f"{_lib_path} has no {name}: it was built from older sources")
     return _entries[name]
 
 

@@ -225,7 +225,10 @@ class _Operators:
         self.decode_shared = _pd.decode_shared
         self.forward_pth = _pd.forward_pth
         self.forward_rows = _pd.forward_rows
-        self.forward_window = _pd.forward_window
+        # (a library built from older sources may lack these two; then the routing does without)
+        if _pd.provides("pth_fa_forward_window") and _pd.provides("pth_fa_window_splits"):
+            self.forward_window = _pd.forward_window
+        self.takes_sinks = _pd.provides("pth_dec_decode_sinks")
 
 
 def _load(env_switch: str, env_lib: str, what: str):
@@ -318,7 +321,8 @@ class Gfx950Int8Attention:
         # (a right bound of 0 is causal decode's own rule; without sink tokens such layers' decode stays with the caller)
         if num_heads % max(num_kv_heads, 1) == 0 and 1 <= max_q * G <= MAX_ROWS_PER_KV_HEAD and (
                 sliding_window[1] < 0 or (self.sink_tokens and sliding_window[1] == 0)):
-            self.pth_dec = load_pth_dec()
+            dec = load_pth_dec()
+            self.pth_dec = dec if not self.sink_tokens or getattr(dec, "takes_sinks", True) else None
 
     def _no_fallback_for_sinks(self) -> None:
         if self.sink_tokens and self.pth_fa_window is None:
