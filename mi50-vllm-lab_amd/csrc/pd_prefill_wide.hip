@@ -713,9 +713,10 @@ __device__ __forceinline__ void wide_workgroup(const FaParams& a, const FaWindow
         const int ntl = t1 - t0;
         // Where the loop lies matters, because one wave per SIMD hides no instruction fetch, of 32 bytes each: the same loop at eight
         // places, 4 bytes apart, takes 3.65 to 3.75 ms for 2,560 tokens over 61,440 keys with
-        // fp16 rows (4.68 to 4.79 exact), 782 to 792 us for 8,192 tokens with a window of 4,096, 118.5 to 122 for 512 of them split in two.
-        // So it is placed, at what was best for each form. The padding runs once.
-        constexpr int kPlace = kSplit ? 1 : kExact && !kWindow ? 3 : 4;
+        // fp16 rows (4.68 to 4.79 exact), 782 to 792 us for 8,192 tokens with a window of 4,096, 118.5 to 122 for 512 of them split in two; exact and
+        // split, 2,048 over 61,440 keys, 3.66 to 3.69 with fp32 rows and 3.58 to 3.65 with fp16 ones.
+        // So it is placed, at what was best for each form; the alignment keeps it there whatever comes before. The padding runs once.
+        constexpr int kPlace = kExact && !kWindow ? (kSplit ? 0 : 3) : kSplit ? 1 : 4;
         asm volatile(".p2align 5\n\t.rept %0\n\ts_nop 0\n\t.endr" ::"n"(kPlace));
 #pragma unroll 1
         for (int i = 0; i < ntl; ++i) {
