@@ -617,7 +617,8 @@ int pth_fa_forward_window(const pd_tensor* q, const pd_tensor* key_cache, const 
     if (!(nsplit >= 1 && nsplit <= 64)) return fail(err, errlen, "nsplit must be in [1, 64]");
     // a launch's workgroups, and the 32 bits that number query tiles and rows
     const int64_t G = Hq / Hkv, tiles = window_tiles(T, num_seqs, G, kFwNarrowRows);
-    if (!(T * Hq <= ((int64_t)1 << 30) && tiles * nsplit <= (1 << 24) / Hkv - 1))
+    // (the merge of splits takes four tokens a workgroup)
+    if (!(T * Hq <= ((int64_t)1 << 30) && tiles * nsplit <= (1 << 24) / Hkv - 1 && (nsplit == 1 || T <= ((int64_t)1 << 26) - 4)))
         return fail(err, errlen, "at most 2^30 (token, head) rows and 2^24 workgroups per call");
     if (!rows_apart(out, T, kDim)) return fail(err, errlen, "out rows must not overlap");
     if (nsplit > 1 && !(workspace && workspace->dtype == PD_DTYPE_FP32 && workspace->ndim == 1 && is_contig(workspace) &&

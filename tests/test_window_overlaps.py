@@ -91,3 +91,20 @@ def test_heads_of_one_buffer():
                            64, sinks=5)
     ref, _, _ = window_oracle.windowed(case, 64, 5)
     assert kvc.fp16_output_errors(x[:, 24:].double().cpu().numpy(), ref)[2] <= 0
+
+
+def test_more_tokens_than_a_merge_launch_numbers(lib):
+    """Described, never read: 2^24 workgroups of four tokens are one too many, and only splits are merged."""
+    case = kvc.make_case([37], [3], num_q_heads=1, num_kv_heads=1, block_size=16, seed=3)
+    rows = lambda n: case.q[:1].expand(n, 1, 256)  # noqa: E731
+
+    def why(n, nsplit):
+        c = case.cache
+        err = ctypes.create_string_buffer(256)
+        d = [ctypes.byref(pth_dec.describe(t)) for t in (rows(n), c.key_cache, c.value_cache, case.block_table, case.seq_lens,
+                                                        case.query_start_loc, rows(n), torch.zeros(8))]
+        assert lib.pth_fa_forward_window(*d[:5], 0.1, *d[5:], 1, 16, 4, nsplit, 0, None, err, len(err)) == 1
+        return err.value.decode()
+
+    assert "2^24 workgroups" in why(2 ** 26 - 3, 2) and "2^24 workgroups" in why(2 ** 26, 64)
+    assert "out rows must not overlap" in why(2 ** 26 - 4, 2) and "out rows must not overlap" in why(2 ** 26, 1)
