@@ -219,7 +219,7 @@ def _prepare_attention(case, gen, host):
         s["place"] = torch.arange(case["sinks"] + case["window"] + case["qlen"] - 1, device="cuda")
         if own:  # the engine's split count for such a batch
             shim = _package().vllm_shim
-            plan = (_SEGMENTS, case["window"], hkv, n, s["q"].device, s["lens_host"], case["qlen"], hq)
+            plan = (_SEGMENTS, case["window"] + case["sinks"], hkv, n, s["q"].device, s["lens_host"], case["qlen"], hq)
             s["nsplit"] = shim.launched_splits(shim.decode_splits(*plan), *plan)
     return s
 
