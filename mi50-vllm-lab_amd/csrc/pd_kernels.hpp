@@ -202,9 +202,10 @@ constexpr int64_t kRowBytes = 520;
 constexpr int64_t kMaxPages = (int64_t)1 << 22;  // 4,096 counts of 1,024 pages fit the prefix in LDS
 constexpr int kMaxForkRows = 8192;               // old rows' first children in LDS
 constexpr int kMaxPageLayers = 128;              // caches of a call: kernel arguments
-// Workgroups that copy, at the most, and bytes of a copied piece. 1,510 moves of 33,280 bytes in 8 layers take 173 us with 4,096 workgroups, 16 per
-// CU in two rounds, and 182 with 2,048, 176 with 1,024; pieces of 8,192 173, of 32,768 (with 2,048) 173. About 31 of 1.65 MB in two
-// layers, which no more than 2,048 serve: 55.5 with pieces of 16,384, 57.5 of 8,192, 58 of 32,768.
+// Workgroups that copy, at the most, and bytes of a copied piece. 1,510 moves of 33,280 bytes in 8 layers, two runs each: 173 and 175 us with
+// 4,096 workgroups, 16 per CU in two rounds, 173 and 173 with 8,192; 180 and 181 with 2,048, 177 and 180 with 1,024, 177 and 180 with 512. The
+// piece decides where few pages are copied: 64 rows with copies in 16 layers take 11.0 us with pieces of 16,384 or 32,768, 13.2 with
+// 8,192; the compactions, of these pages or of 31 of 1.65 MB in two layers (51 to 55 us), do not tell the three apart.
 constexpr int kPageCopyGroups = 4096;
 constexpr int64_t kPagePiece = 16384;
 enum PageForm { kPageWhole, kPageHeads, kPageRows };

@@ -39,7 +39,8 @@ constexpr double kFaDealMargin = 0.95;
 // tile, exact numerics' tile, set-up and stores with the launch; the merge launch of splits and their partials' way to memory and back.
 // Measured and rated (24 q / 4 kv heads, over 30,000 keys), wide and narrow: 2,048 tokens over 512 keys 58 (56) and 79 (82), over 4,096
 // 265 (263) and 416 (417); 1,024 over 1,024 85 (85) and 65 (64); 64 over 2,048 in 10 splits 39 (42) and 31 (31); 600 over
-// 4,096 in 2 153 (155) and 124 (123); 4,096 in 2 482 (482).
+// 4,096 in 2 153 (155) and 124 (123); 4,096 in 2 482 (482). Exact: 2,048 over 4,096 wide 330 (334), over 512 74 (68); narrow 1,024 over 1,024 74 (74),
+// 64 over 2,048 in 10 33 (33), 600 over 4,096 in 2 139 (141); 4,096 in 2 wide 592 (587).
 struct FwTimes {
     double tile, tile_exact, setup;
 };
