@@ -1110,39 +1110,48 @@ static bool cache_rows_apart(const pd_tensor* kv) {
     return true;
 }
 
-// Bytes from a raw cache's first row to the end of its last.
-static int64_t raw_extent(const pd_tensor* kv) {
-    int64_t n = kRowBytes;
-    for (int d = 0; d < 3; ++d) n += (kv->sizes[d] - 1) * kv->strides[d];
-    return n;
-}
-// Whether rows of two caches of kv's sizes and strides, `d` bytes apart, share a byte: some sum of a[i] strides[i] with |a[i]| < sizes[i] is less
-// than a row from d. By falling strides; below a stride the others reach less far than it (cache_rows_apart), so only the two
-// multiples beside d can.
-static bool rows_meet(const pd_tensor* kv, int64_t d) {
-    int order[3] = {0, 1, 2};
-    std::sort(order, order + 3, [&](int a, int b) { return kv->strides[a] > kv->strides[b]; });
-    int64_t reach[4] = {0, 0, 0, kRowBytes};
-    for (int i = 2; i >= 0; --i) reach[i] = reach[i + 1] + (kv->sizes[order[i]] - 1) * kv->strides[order[i]];
-    int64_t left[8] = {d};
-    int n = 1;
-    for (int i = 0; i < 3; ++i) {
-        const int64_t most = kv->sizes[order[i]] - 1, st = kv->strides[order[i]];
-        int64_t next[8];
-        int m = 0;
-        for (int j = 0; j < n; ++j) {
-            if (most == 0) {
-                if (std::abs(left[j]) < reach[i + 1]) next[m++] = left[j];
-                continue;
-            }
-            const int64_t a = left[j] / st - (left[j] % st < 0);
-            for (int64_t x = a; x <= a + 1; ++x)
-                if (std::abs(x) <= most && std::abs(left[j] - x * st) < reach[i + 1]) next[m++] = left[j] - x * st;
+namespace {
+// Where the rows of caches of one geometry lie: strides that fall, how often each is taken, and how far it and those below reach. Below a
+// stride the others reach less far than it (cache_rows_apart).
+struct RowLattice {
+    int64_t st[3], most[3], reach[4];
+    explicit RowLattice(const pd_tensor* kv) {
+        int order[3] = {0, 1, 2};
+        std::sort(order, order + 3, [&](int a, int b) { return (kv->sizes[a] > 1 ? kv->strides[a] : 0) > (kv->sizes[b] > 1 ? kv->strides[b] : 0); });
+        reach[3] = kRowBytes;
+        for (int i = 2; i >= 0; --i) {
+            st[i] = kv->strides[order[i]], most[i] = kv->sizes[order[i]] - 1;
+            reach[i] = reach[i + 1] + most[i] * st[i];
         }
-        std::copy(next, next + m, left);
-        n = m;
     }
-    return n > 0;
+    // Whether rows of two caches that begin d bytes apart share a byte: some sum of a[i] st[i] with |a[i]| <= most[i] is less than a row
+    // from d. Only the two multiples of a stride beside d can be.
+    bool meet(int64_t d, int i = 0) const {
+        if (std::abs(d) >= reach[i]) return false;
+        if (i == 3) return true;
+        if (most[i] == 0) return meet(d, i + 1);
+        const int64_t a = d / st[i] - (d % st[i] < 0);
+        return (std::abs(a) <= most[i] && meet(d - a * st[i], i + 1)) || (std::abs(a + 1) <= most[i] && meet(d - (a + 1) * st[i], i + 1));
+    }
+};
+}  // namespace
+// Whether rows of different caches (sorted) share a byte.
+static bool caches_meet(const PageCaches& k, const RowLattice& rows) {
+    bool near = false;
+    for (int i = 1; i < k.layers; ++i) near = near || k.kv[i] - k.kv[i - 1] < rows.reach[0];
+    if (!near) return false;
+    if (rows.most[0] > 0) {  // interleaved layers: apart in every period of the largest stride
+        int64_t at[kMaxPageLayers];
+        for (int i = 0; i < k.layers; ++i) at[i] = (k.kv[i] - k.kv[0]) % rows.st[0];
+        std::sort(at, at + k.layers, [](int64_t a, int64_t b) { return a < b; });
+        bool clear = at[0] + rows.st[0] - at[k.layers - 1] >= rows.reach[1];
+        for (int i = 1; i < k.layers; ++i) clear = clear && at[i] - at[i - 1] >= rows.reach[1];
+        if (clear) return false;
+    }
+    for (int i = 0; i < k.layers; ++i)
+        for (int j = i + 1; j < k.layers && k.kv[j] - k.kv[i] < rows.reach[0]; ++j)
+            if (rows.meet(k.kv[j] - k.kv[i])) return true;
+    return false;
 }
 // Whether a tensor lies clear of all caches (sorted, `extent` bytes each).
 static bool clear_of_caches(const PageCaches& k, int64_t extent, const ByteRows& r) {
@@ -1176,10 +1185,7 @@ static const char* page_caches(const pd_tensor* caches, int64_t layers, PageCach
     if (!cache_rows_apart(&c)) return "cache rows must not overlap";
     std::sort(k.kv, k.kv + layers, [](const int8_t* a, const int8_t* b) { return a < b; });
     k.layers = (int)(std::unique(k.kv, k.kv + layers) - k.kv);
-    const int64_t extent = raw_extent(&c);
-    for (int i = 0; i < k.layers; ++i)
-        for (int j = i + 1; j < k.layers && k.kv[j] - k.kv[i] < extent; ++j)
-            if (rows_meet(&c, k.kv[j] - k.kv[i])) return "the caches' rows must not overlap";
+    if (caches_meet(k, RowLattice(&c))) return "the caches' rows must not overlap";
     k.sb = c.strides[0];
     k.sh = c.strides[1];
     k.ss = c.strides[2];
@@ -1264,7 +1270,7 @@ int pth_cache_fork_pages(const pd_tensor* caches, int64_t layers, const pd_tenso
             if (parents && !apart(outs[i], byte_span(parents, N, 4)))
                 return fail(err, errlen, "the tensors that are written must not overlap those that are read");
         }
-        const int64_t extent = raw_extent(caches);
+        const int64_t extent = RowLattice(caches).reach[0];
         bool clear = !parents || clear_of_caches(k, extent, byte_span(parents, N, 4));
         for (const ByteRows& r : outs) clear = clear && clear_of_caches(k, extent, r);
         for (const ByteRows& r : ins) clear = clear && clear_of_caches(k, extent, r);
@@ -1326,7 +1332,7 @@ int pth_cache_compact_pages(const pd_tensor* caches, int64_t layers, const pd_te
             for (int j = 0; j < 2; ++j)
                 if (i != j && !apart(outs[i], ins[j])) return fail(err, errlen, "the tensors that are written must not overlap those that are read");
         }
-        const int64_t extent = raw_extent(caches);
+        const int64_t extent = RowLattice(caches).reach[0];
         bool clear = true;
         for (const ByteRows& r : outs) clear = clear && clear_of_caches(k, extent, r);
         for (const ByteRows& r : ins) clear = clear && clear_of_caches(k, extent, r);

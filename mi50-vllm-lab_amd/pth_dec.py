@@ -520,8 +520,9 @@ def fork_pages(caches, refs: torch.Tensor, block_table: torch.Tensor, seq_lens: 
     [pages]: how many table entries name each page (0: free); block_table int32 [B, columns], entries below 0 name no page; seq_lens
     int32 [B].
     New row i goes on from old row parents[i] (int32 [N]; outside [0, B): an empty row), None: from row i. It shares the parent's full
-    pages and gets room for `grow` more keys, one number for all rows; a later call with less takes back what they do not use. A page that still takes keys is its own: the first child keeps the parent's if no
-    other entry names it, the others take a free page, into which the keys that the parent has in it are copied, for all caches.
+    pages and gets room for `grow` more keys, one number for all rows; a later call with less takes back what they do not use. A page that
+    still takes keys is its own: the first child keeps the parent's if no other entry names it, the others take a free page, into
+    which the keys that the parent has in it are copied, for all caches.
     window > 0: a page whose keys all lie at or past `sinks` and before what the next token sees (seq_len + 1 - window) becomes
     -1, as decode and forward_window never read it. Old rows lose their references: a page that nothing names any more is free
     for the next call. Pages are taken in the order of (row, column), the lowest that were free before the call first.
