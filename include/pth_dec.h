@@ -165,8 +165,8 @@ int pth_dec_decode_lse(const pd_tensor* q, const pd_tensor* key_cache, const pd_
  *   lse          null, or as for pth_dec_decode_lse
  *   sinks        >= 0: row j (absolute position p_j) sees key k < seq_len, k <= p_j where causal, if p_j - k < window or k < sinks;
  *                without a window (<= 0) every row sees those keys anyway
- * Pages in which no row of the sequence sees a key are not addressed: their table entries may name anything. Other arguments, checks
- * and return codes are those of pth_dec_decode.
+ * Pages in which no row of the sequence sees a key are not addressed: their table entries may name anything. A key whose scale is not
+ * finite makes the rows that see it so and no others. Other arguments, checks and return codes are those of pth_dec_decode.
  */
 int pth_dec_decode_sinks(const pd_tensor* q, const pd_tensor* key_cache, const pd_tensor* value_cache,
                          const pd_tensor* k_scale, const pd_tensor* v_scale, const pd_tensor* block_table,
@@ -294,7 +294,8 @@ int64_t pth_fa_balanced_workspace(int64_t num_seqs, const int* query_start, int6
  *   workspace    fp32, contiguous, 16-byte aligned, of T * Hq * nsplit * 258 floats (null or ignored when nsplit is 1)
  *   exact        0: each softmax weight enters P.V as one fp16; else as fp16 hi + lo. K and V are widened exactly in both
  * Pages in which no row of a query tile sees a key are not addressed for it: the table's entries for pages between the sinks and
- * the first row's window may name anything. Returns 0, 1 or 2 as above.
+ * the first row's window may name anything. A key whose scale is not finite makes the rows that see it so and no others. Returns 0, 1
+ * or 2 as above.
  */
 int pth_fa_forward_window(const pd_tensor* q, const pd_tensor* key_cache, const pd_tensor* value_cache,
                           const pd_tensor* block_table, const pd_tensor* seq_lens, double scale,

@@ -475,6 +475,7 @@ __device__ __forceinline__ void partial_body(const PartialParams& a, const Work&
     //      products), times k_scale, relative to the running max: sv = s - m (log2 units; s itself
     //      while a row has no max yet); masked scores are -inf. Returns whether some row has to
     //      raise its max: its tile max exceeds the running max by more than kLazy, or it has none ----
+    bool unfinite = false;  // (with sinks) some v_scale of the tile is not finite
     auto tile_scores = [&](const TileOps& o, float (&sv)[NRB][8], bool& interior) __attribute__((always_inline)) {
         float4_t sacc[NRB][2];
 #pragma unroll
@@ -509,6 +510,13 @@ __device__ __forceinline__ void partial_body(const PartialParams& a, const Work&
             if (a.causal) interior = interior && kb + kTile - 1 <= ctx0;
             if (a.window > 0) interior = interior && (ctx0 + ql - 1) - kb < a.window;
         }
+        if constexpr (kSinks) {
+            // v_scales of a tile that some row does not see all of: any that is not finite?
+            float sum = o.vs[0] * 0.f;
+#pragma unroll
+            for (int e = 1; e < 8; ++e) sum = __builtin_fmaf(o.vs[e], 0.f, sum);
+            unfinite = !interior && __builtin_amdgcn_ballot_w64(sum != 0.f) != 0;
+        }
         bool need = false;
 #pragma unroll
         for (int rb = 0; rb < NRB; ++rb) {
@@ -530,6 +538,14 @@ __device__ __forceinline__ void partial_body(const PartialParams& a, const Work&
                         vis = rvalid[rb] & (t >= lo) & (t < hi) & (!a.causal | (t <= rp)) &
                               ((a.window <= 0) | ((rp - t) < a.window));
                     sv[rb][e] = vis ? sv[rb][e] : kNegInf;
+                }
+            }
+            // Such a scale counts as 0 in tile_values, lest 0 times it reach the rows that do not see the key. To those that do its
+            // score says so, as +inf: NaN here and through the merge.
+            if constexpr (kSinks) {
+                if (__builtin_expect(unfinite, 0)) {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) sv[rb][e] = fabsf(o.vs[e]) < kInf || sv[rb][e] == kNegInf ? sv[rb][e] : kInf;
                 }
             }
             float mx = kNegInf;
@@ -593,6 +609,12 @@ __device__ __forceinline__ void partial_body(const PartialParams& a, const Work&
             for (int e = 0; e < 8; ++e) {
                 const int t = seen.base(tile_cur) + 16 * (e >> 2) + 4 * lg + (e & 3);
                 vsc[e] = seen.has(t) ? vsc[e] : 0.f;
+            }
+            if constexpr (kSinks) {
+                if (__builtin_expect(unfinite, 0)) {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) vsc[e] = fabsf(o.vs[e]) < kInf ? vsc[e] : 0.f;
+                }
             }
         }
         half8_t phi[NRB], plo[NRB];
@@ -786,7 +808,8 @@ __device__ __forceinline__ void partial_body(const PartialParams& a, const Work&
         for (int rb = 0; rb < NRB; ++rb) {
             const float l_row = xor_sum(xor_sum(l_run[rb], 16), 32);
             if (lg == 0) {
-                wm[(w * NRB + rb) * 16 + li] = m_run[rb];
+                // (with sinks: a row whose only scores here are NaN is not one that saw no key)
+                wm[(w * NRB + rb) * 16 + li] = kSinks && l_row != l_row ? kInf : m_run[rb];
                 wl[(w * NRB + rb) * 16 + li] = l_row;
             }
         }

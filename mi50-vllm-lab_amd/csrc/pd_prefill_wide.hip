@@ -527,6 +527,20 @@ __device__ __forceinline__ void wide_workgroup(const FaParams& a, const FaWindow
                         sv[rb][e] = sees ? sv[rb][e] : kNegInf;
                     }
                 }
+                // A seen key whose v_scale is not finite: 0 too, lest 0 times it reach the rows that do not see it. To those that do its
+                // score says so, as +inf: NaN here and through the merge. (Rare and out of line: a select per score took 1 to 5 %.)
+                float sum = vs[0] * 0.f;
+#pragma unroll
+                for (int e = 1; e < 8; ++e) sum = __builtin_fmaf(vs[e], 0.f, sum);
+                if (__builtin_expect(__builtin_amdgcn_ballot_w64(sum != 0.f) != 0, 0)) {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        const bool finite = fabsf(vs[e]) < kInf;
+#pragma unroll
+                        for (int rb = 0; rb < kRB; ++rb) sv[rb][e] = finite || sv[rb][e] == kNegInf ? sv[rb][e] : kInf;
+                        vs[e] = finite ? vs[e] : 0.f;
+                    }
+                }
             }
         } else if (n >= n_int) {  // the tile crosses the causal diagonal or seq_len
             const int key = n * kTile + 4 * (lane_here() >> 4);
@@ -713,10 +727,10 @@ __device__ __forceinline__ void wide_workgroup(const FaParams& a, const FaWindow
         const int ntl = t1 - t0;
         // Where the loop lies matters, because one wave per SIMD hides no instruction fetch, of 32 bytes each: the same loop at eight
         // places, 4 bytes apart, takes 3.65 to 3.75 ms for 2,560 tokens over 61,440 keys with
-        // fp16 rows (4.68 to 4.79 exact), 782 to 792 us for 8,192 tokens with a window of 4,096, 118.5 to 122 for 512 of them split in two; exact and
-        // split, 2,048 over 61,440 keys, 3.66 to 3.69 with fp32 rows and 3.58 to 3.65 with fp16 ones.
+        // fp16 rows (4.68 to 4.79 exact), 2,048 exact and split 3.66 to 3.69 with fp32 rows and 3.58 to 3.65 with fp16 ones; over a window of 4,096
+        // behind 30,000 keys 994 to 1,011 us for 8,192 tokens (exact), 120 to 123 for 512 split in two.
         // So it is placed, at what was best for each form; the alignment keeps it there whatever comes before. The padding runs once.
-        constexpr int kPlace = kExact && !kWindow ? (kSplit ? 0 : 3) : kSplit ? 1 : 4;
+        constexpr int kPlace = kWindow ? (kSplit ? 5 : 1) : kExact ? (kSplit ? 0 : 3) : kSplit ? 1 : 4;
         asm volatile(".p2align 5\n\t.rept %0\n\ts_nop 0\n\t.endr" ::"n"(kPlace));
 #pragma unroll 1
         for (int i = 0; i < ntl; ++i) {
@@ -801,7 +815,8 @@ __device__ __forceinline__ void wide_workgroup(const FaParams& a, const FaWindow
 #pragma unroll
             for (int m = 0; m < 16; ++m) *reinterpret_cast<float4_t*>(prow + 16 * m) = oacc[rb][m];
             if (lg == 0) {
-                a.part_m[pr] = thr_run[rb] == kNegInf ? kNegInf : kPLog2 - nm_run[rb];
+                // (a row whose only scores here are NaN is not one that saw no key: +inf, lest the merge leave its sum out)
+                a.part_m[pr] = kWindow && l_row != l_row ? kInf : thr_run[rb] == kNegInf ? kNegInf : kPLog2 - nm_run[rb];
                 a.part_l[pr] = l_row;
             }
         } else {

@@ -32,6 +32,7 @@ typedef const __attribute__((address_space(4))) int* const_int_ptr;  // scalar-c
 
 constexpr int kTile = 32;             // keys per tile
 constexpr float kNegInf = -__builtin_inff();
+constexpr float kInf = __builtin_inff();
 // The running max m of a row is only raised when a tile's max exceeds it by more than
 // kLazy (log2 units), so p = 2^(s - m) <= 2^kLazy and most tiles skip the O rescale.
 // P' = p * v_scale * kPScale then spans the same fp16 range as p * v_scale * 256 with p <= 1.
